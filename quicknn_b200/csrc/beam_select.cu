@@ -1,0 +1,257 @@
+// The best continuations of every request over its beams and the vocabulary, for beam search.
+//
+// Beam b of a request has the score t_b (a sum of logarithms of probabilities); with z = logits[b] its continuation by token v scores
+//     t_b + z_v - log(sum_u exp(z_u)).
+// Wanted are the `take` best of a request's beams x V continuations in descending order, equal scores by the lowest (beam, token).
+//
+// Within a beam the order of the scores is that of the logits, so one pass over the logits is enough for everything but a few of them:
+//   1. a warp per segment of a row (SEGMENT logits) leaves the segment's maximum and sum of exp(z - maximum);
+//   2. a block per request joins them to log(sum exp) of every beam, turns the segments' maxima into scores, and finds a threshold that at
+//      least `take` segments reach.  As each of these holds a score that reaches it, so do the `take` best of all; they lie in the segments
+//      that reach it, which are read again (a few KB) into a short list, whose best are found by counting.
+// Scores are formed in 64 bits: those of different beams may differ by less than 32 bits resolve after a sum over the vocabulary.
+// A logit that is not finite is no continuation and not in the sum (bit 0 of the error word says so); nor is any of a beam whose score is
+// -inf or NaN.  Where fewer than `take` are left, the places behind them hold score -inf, beam -1, token -1.
+#include "common.cuh"
+#include <float.h>
+#include <math_constants.h>
+
+using namespace qnn;
+
+namespace {
+
+constexpr int SELECT_MOST = 64;               // continuations per request, at most
+constexpr int SELECT_THREADS = 1024;
+constexpr int LIST = 2048;                    // places of the short list
+
+// One maximum and sum per segment: warp w of the grid takes segment w of the row.
+template <int SEGMENT>
+__global__ void __launch_bounds__(256)
+beam_segments_kernel(const float* __restrict__ logits, int V, int segments, float2* __restrict__ stats, int* __restrict__ error_flag) {
+    pdl_wait();
+    const int seg = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, r = blockIdx.y;
+    if (seg >= segments) return;
+    const float* row = logits + (size_t)r * V;
+    float z[SEGMENT / 32];
+    float m = -CUDART_INF_F;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < SEGMENT / 32; ++i) {
+        const int v = seg * SEGMENT + i * 32 + lane;
+        z[i] = v < V ? row[v] : -CUDART_INF_F;
+        if (v < V && !isfinite(z[i])) {
+            bad = true;
+            z[i] = -CUDART_INF_F;
+        }
+        m = fmaxf(m, z[i]);
+    }
+    m = warp_max(m);
+    float s = 0.f;
+    if (m != -CUDART_INF_F)
+#pragma unroll
+        for (int i = 0; i < SEGMENT / 32; ++i) s += expf(z[i] - m);
+    s = warp_sum(s);
+    if (lane == 0) stats[(size_t)r * segments + seg] = make_float2(m, s);
+    if (error_flag != nullptr && __any_sync(0xffffffffu, bad) && lane == 0) atomicOr(error_flag, 1);
+}
+
+__device__ __forceinline__ double warp_sum(double v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+// finite floats as unsigned numbers of the same order
+__device__ __forceinline__ unsigned ordered(float f) {
+    const unsigned u = __float_as_uint(f);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ bool before(double a, unsigned ia, double b, unsigned ib) { return a > b || (a == b && ia < ib); }
+
+struct Found {
+    double score[LIST];
+    unsigned at[LIST];                        // beam * V + token
+};
+
+template <int SEGMENT>
+__global__ void __launch_bounds__(SELECT_THREADS)
+beam_pick_kernel(const float* __restrict__ logits, int V, int beams, int take, int segments, const float* __restrict__ scores,
+                 const float2* __restrict__ stats, float* __restrict__ out_scores, int* __restrict__ out_beams, int* __restrict__ out_tokens,
+                 const int* __restrict__ status_in, int* __restrict__ error_flag) {
+    pdl_wait();
+    if (blockIdx.x == 0 && threadIdx.x == 0 && status_in != nullptr && error_flag != nullptr) {
+        const int s = *status_in;             // what the step's kernels reported: bit 1 and their status from bit 8 up
+        if (s != 0) atomicOr(error_flag, 2 | (s << 8));
+    }
+    extern __shared__ __align__(16) unsigned char smem[];
+    Found* found = reinterpret_cast<Found*>(smem);
+    double* base = reinterpret_cast<double*>(found + 1);      // [beams] t_b - log(sum exp)
+    unsigned* best = reinterpret_cast<unsigned*>(base + beams);   // [beams * segments] the segments' best scores, ordered
+    __shared__ int n_found, sum;
+    __shared__ double last_score;
+    __shared__ unsigned last_at;
+    const int q = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const size_t row0 = (size_t)q * beams;
+    if (threadIdx.x == 0) n_found = 0;
+    for (int b = warp; b < beams; b += SELECT_THREADS / 32) {
+        const float2* st = stats + (row0 + b) * segments;
+        float m = -CUDART_INF_F;
+        for (int i = lane; i < segments; i += 32) m = fmaxf(m, st[i].x);
+        m = qnn::warp_max(m);
+        double s = 0.0;
+        for (int i = lane; i < segments; i += 32)
+            if (st[i].x != -CUDART_INF_F) s += (double)st[i].y * exp((double)st[i].x - (double)m);
+        s = warp_sum(s);
+        const double t = (double)scores[row0 + b];
+        const bool alive = m != -CUDART_INF_F && t > -CUDART_INF && t < CUDART_INF;
+        const double add = alive ? t - (double)m - log(s) : -CUDART_INF;
+        if (lane == 0) base[b] = add;
+        for (int i = lane; i < segments; i += 32)
+            best[b * segments + i] = alive && st[i].x != -CUDART_INF_F ? ordered((float)(add + (double)st[i].x)) : 0u;    // 0: none
+    }
+    __syncthreads();
+    // The threshold: the largest number that `take` segments reach or a little below (up to twice as many segments), bit by bit.
+    const int n = beams * segments;
+    unsigned threshold = 0u;
+    for (int bit = 31; bit >= 0; --bit) {
+        const unsigned tried = threshold | (1u << bit);
+        int mine = 0;
+        for (int i = threadIdx.x; i < n; i += SELECT_THREADS) mine += best[i] >= tried;
+        if (threadIdx.x == 0) sum = 0;
+        __syncthreads();
+        mine = __reduce_add_sync(0xffffffffu, mine);
+        if (lane == 0 && mine) atomicAdd(&sum, mine);
+        __syncthreads();
+        const int reach = sum;
+        __syncthreads();
+        if (reach >= take) {
+            threshold = tried;
+            if (reach <= 2 * take) break;
+        }
+    }
+    if (threshold == 0u) threshold = 1u;      // fewer segments than wanted: all that hold anything
+    for (int i = warp; i < n; i += SELECT_THREADS / 32) {
+        if (best[i] < threshold) continue;
+        const int b = i / segments, v0 = (i - b * segments) * SEGMENT;
+        const float* row = logits + (row0 + b) * V;
+#pragma unroll
+        for (int j = 0; j < SEGMENT / 32; ++j) {
+            const int v = v0 + j * 32 + lane;
+            if (v >= V) continue;
+            const float z = row[v];
+            if (!isfinite(z)) continue;
+            const double s = base[b] + (double)z;
+            if (ordered((float)s) < threshold) continue;
+            const int at = atomicAdd(&n_found, 1);
+            if (at < LIST) {
+                found->score[at] = s;
+                found->at[at] = (unsigned)b * (unsigned)V + (unsigned)v;
+            }
+        }
+    }
+    __syncthreads();
+    const int have = n_found;
+    float* os = out_scores + (size_t)q * take;
+    int* ob = out_beams + (size_t)q * take;
+    int* ot = out_tokens + (size_t)q * take;
+    if (have <= LIST) {
+        for (int i = threadIdx.x; i < have; i += SELECT_THREADS) {
+            const double s = found->score[i];
+            const unsigned a = found->at[i];
+            int rank = 0;
+            for (int j = 0; j < have; ++j) rank += before(found->score[j], found->at[j], s, a);
+            if (rank < take) {
+                os[rank] = (float)s;
+                ob[rank] = (int)(a / (unsigned)V);
+                ot[rank] = (int)(a % (unsigned)V);
+            }
+        }
+        for (int i = have + threadIdx.x; i < take; i += SELECT_THREADS) {
+            os[i] = -CUDART_INF_F;
+            ob[i] = ot[i] = -1;
+        }
+        return;
+    }
+    // More scores at the threshold than the list holds (thousands of equal ones): `take` rounds over the segments that reach it, each for
+    // the best behind the one before.
+    for (int k = 0; k < take; ++k) {
+        double s_best = -CUDART_INF;
+        unsigned a_best = 0xffffffffu;
+        for (int i = warp; i < n; i += SELECT_THREADS / 32) {
+            if (best[i] < threshold) continue;
+            const int b = i / segments, v0 = (i - b * segments) * SEGMENT;
+            const float* row = logits + (row0 + b) * V;
+            for (int j = 0; j < SEGMENT / 32; ++j) {
+                const int v = v0 + j * 32 + lane;
+                if (v >= V) continue;
+                const float z = row[v];
+                if (!isfinite(z)) continue;
+                const double s = base[b] + (double)z;
+                const unsigned a = (unsigned)b * (unsigned)V + (unsigned)v;
+                if ((k == 0 || before(last_score, last_at, s, a)) && before(s, a, s_best, a_best)) {
+                    s_best = s;
+                    a_best = a;
+                }
+            }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const double s = __shfl_xor_sync(0xffffffffu, s_best, o);
+            const unsigned a = __shfl_xor_sync(0xffffffffu, a_best, o);
+            if (before(s, a, s_best, a_best)) {
+                s_best = s;
+                a_best = a;
+            }
+        }
+        __syncthreads();                      // the round before has been read
+        if (lane == 0) {
+            found->score[warp] = s_best;
+            found->at[warp] = a_best;
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            for (int w = 1; w < SELECT_THREADS / 32; ++w)
+                if (before(found->score[w], found->at[w], s_best, a_best)) {
+                    s_best = found->score[w];
+                    a_best = found->at[w];
+                }
+            last_score = s_best;
+            last_at = a_best;
+            os[k] = (float)s_best;
+            ob[k] = (int)(a_best / (unsigned)V);
+            ot[k] = (int)(a_best % (unsigned)V);
+        }
+        __syncthreads();
+    }
+}
+
+// Logits per segment: small vocabularies get short ones, so that the threshold, the `take`-th best segment, stays near the best.
+int segment_of(int V) { return V >= 16384 ? 512 : 128; }
+
+}  // namespace
+
+QNN_API int qnn_beam_select_segments(int V) { return V <= 0 ? 0 : (V + segment_of(V) - 1) / segment_of(V); }
+
+// logits: [requests * beams, V] float32; scores: [requests * beams]; the outputs [requests, take].  Scratch: requests * beams *
+// qnn_beam_select_segments(V) float2.  take <= 64; beams * V < 2^32.
+QNN_API int qnn_beam_select(const float* logits, const float* scores, int requests, int beams, int V, int take, void* scratch, float* out_scores,
+                            int* out_beams, int* out_tokens, const int* status_in, int* error_flag, cudaStream_t st) {
+    if (requests <= 0) return 0;
+    if (beams < 1 || V < 1 || take < 1 || take > SELECT_MOST) return QNN_ERR_ARGUMENT;
+    if ((long long)requests * beams > 65535 || (long long)beams * V >= 0xffffffffLL) return QNN_ERR_UNSUPPORTED;
+    const int segments = qnn_beam_select_segments(V);
+    const size_t smem = sizeof(Found) + (size_t)beams * sizeof(double) + (size_t)beams * segments * sizeof(unsigned);
+    if (smem > 200 * 1024) return QNN_ERR_UNSUPPORTED;
+    const dim3 grid((segments + 7) / 8, requests * beams);
+    float2* stats = (float2*)scratch;
+#define QNN_SELECT(SEG)                                                                                                                        \
+    {                                                                                                                                          \
+        static OncePerDevice asked;                                                                                                            \
+        if (const int rc = allow_shared(asked, beam_pick_kernel<SEG>, 200 * 1024)) return rc;                                                  \
+        launch_pdl(beam_segments_kernel<SEG>, grid, dim3(256), 0, st, logits, V, segments, stats, error_flag);                                 \
+        launch_pdl(beam_pick_kernel<SEG>, dim3(requests), dim3(SELECT_THREADS), smem, st, logits, V, beams, take, segments, scores,             \
+                   (const float2*)stats, out_scores, out_beams, out_tokens, status_in, error_flag);                                            \
+    }
+    if (segment_of(V) == 512) QNN_SELECT(512) else QNN_SELECT(128)
+#undef QNN_SELECT
+    QNN_LAUNCH_CHECK();
+}

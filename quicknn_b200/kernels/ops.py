@@ -14,7 +14,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -2304,3 +2304,226 @@ def stream_update(resid: torch.Tensor, y: torch.Tensor, mult: float, w_post: tor
         return causal_conv(normed, cw, state, None, None, pos, slots, T, add_input=True)
     _lib.check(code, "stream_update")
     return normed
+
+
+# ---- sequences that share what they hold: attention, beam search, copies ----------------------------------
+
+class SharedKeys:
+    """Which rows of a decode step hold a stretch of positions in the same pages of the cache.
+
+    ``groups`` (int32, [groups, 4] on the device): first row, number of rows, first position, position behind the last; the page
+    tables of these rows name the same pages for those positions, as far as a row still holds them.  ``row_group`` (int32, one per row):
+    a row's group, or -1.  ``rows``, ``keys`` and ``own`` bound the rows of a group, the positions of a group and the keys that a row has
+    beside them: host numbers, from which the work is divided (``rows`` must hold; the others are a matter of speed)."""
+
+    __slots__ = ("groups", "row_group", "rows", "keys", "own")
+
+    def __init__(self, groups: torch.Tensor, row_group: torch.Tensor, *, rows: int, keys: int, own: int):
+        _req(groups, "groups", torch.int32, 2)
+        _req(row_group, "row_group", torch.int32, 1)
+        if groups.shape[1] != 4:
+            raise ValueError("shared keys: a group is (first row, rows, begin, end)")
+        if rows < 0 or keys < 0 or own < 0 or (groups.shape[0] and rows < 1):
+            raise ValueError("shared keys: bounds of rows and keys cannot be negative, and a group has a row")
+        self.groups, self.row_group, self.rows, self.keys, self.own = groups, row_group, int(rows), int(keys), int(own)
+
+
+class SharedPlan(NamedTuple):
+    """Into how many ranges ``attn_decode_shared`` cuts the common keys of a group and a row's own, and the scratch that takes."""
+
+    common_ranges: int
+    own_ranges: int
+    scratch_bytes: int
+
+
+SHARED_ITEM_COST = 64.0          # what a CTA of that attention costs beside its keys, in keys
+
+
+def shared_attention_plan(dtype: torch.dtype, n_rows: int, n_heads: int, n_kv: int, head_dim: int, shared: SharedKeys,
+                          window: Optional[int] = None, ranges: Optional[Tuple[int, int]] = None) -> SharedPlan:
+    """How ``attn_decode_shared`` divides its work for so many rows: the cut of common and own keys into ranges of about one length
+    with the shortest estimated time.  ``ranges``: fixed numbers instead."""
+    if n_kv < 1 or n_heads % n_kv or n_rows < 0:
+        raise ValueError(f"shared attention: {n_kv} kv heads do not divide {n_heads} heads")
+    heads = n_heads // n_kv
+    tile = _lib.load().qnn_attn_shared_tile(BF16 if dtype == torch.bfloat16 else F32, head_dim, max(shared.rows, 1) * heads)
+    if dtype not in (torch.bfloat16, torch.float32) or tile <= 0:
+        raise ValueError(f"shared attention does not take head size {head_dim} in {dtype}")
+    if ranges is None:
+        keys, own = max(shared.keys, 1), max(shared.own, 1)
+        if window:
+            keys, own = min(keys, window), min(own, window)
+        resident = _sm_count(shared.groups.device) * max(1, min(8, 512 // head_dim))       # CTAs at a time
+        common = shared.groups.shape[0] * (-(-shared.rows * heads // tile)) * n_kv         # walks over common keys
+        alone = n_rows * (-(-heads // tile)) * n_kv                                        # walks over own keys
+        best = None
+        for c in _SHARED_CHUNKS:
+            s, p = -(-keys // c), -(-own // c)
+            if s > 64 or p > 64:
+                continue
+            items = common * s + alone * p
+            longest = max(-(-keys // s) if common else 0, -(-own // p))
+            t = longest + SHARED_ITEM_COST
+            if items > resident:
+                t = max(t, (common * (keys + s * SHARED_ITEM_COST) + alone * (own + p * SHARED_ITEM_COST)) / resident + longest / 2)
+            t += 2.0 * n_rows * n_heads * (s + p) / resident                               # the parts, written and read as float32
+            if best is None or t < best[0] * 0.999:
+                best = (t, s, p)
+        ranges = best[1:]
+    s, p = ranges
+    if s < 1 or p < 1:
+        raise ValueError("shared attention: at least one range of each kind")
+    return SharedPlan(s, p, max(n_rows, 1) * n_heads * (s + p) * (head_dim + 2) * 4)
+
+
+_SHARED_CHUNKS = tuple(sorted({16 * int(round(2 ** (i / 2))) for i in range(4, 28)}))       # 64 keys .. 128 K
+
+
+def _on_current_device(*ts: torch.Tensor) -> None:
+    here = torch.cuda.current_device()
+    for t in ts:
+        if t.device.index != here:
+            raise ValueError(f"a tensor is on {t.device}, the current device is cuda:{here}")
+
+
+def attn_decode_shared(qkv: torch.Tensor, n_heads: int, n_kv: int, head_dim: int, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                       page_table: torch.Tensor, page_size: int, ring: int, slots: torch.Tensor, slot_len: torch.Tensor,
+                       shared: SharedKeys, scale: float, cap: Optional[float], window: Optional[int], plan: SharedPlan,
+                       scratch: torch.Tensor, slopes: Optional[torch.Tensor] = None, sinks: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``attn_decode`` for rows that share pages: the same results up to rounding, with the keys that a group's rows hold in the same
+    pages (and all see) read once for the group.  ``plan`` comes from ``shared_attention_plan``; ``scratch`` (uint8 or float32, 16-byte
+    aligned) holds ``plan.scratch_bytes`` and is overwritten.  ``slots``, ``slot_len``, ``page_table`` and what ``shared`` holds must be
+    complete before the kernel that runs just before this one on the stream starts, as for ``attn_decode``."""
+    ld = _rows(qkv, "qkv")
+    _check_per_head(slopes, sinks, n_heads)
+    B = qkv.shape[0]
+    _req(k_pool, "k_pool", qkv.dtype, 4)
+    _req(v_pool, "v_pool", qkv.dtype, 4)
+    _req(page_table, "page_table", torch.int32, 2)
+    _req(slots, "slots", torch.int32, 1)
+    _req(slot_len, "slot_len", torch.int32, 1)
+    _req(scratch, "scratch")
+    if n_kv < 1 or n_heads % n_kv:
+        raise ValueError(f"shared attention: {n_kv} kv heads do not divide {n_heads} heads")
+    if qkv.shape[1] < n_heads * head_dim:
+        raise ValueError(f"shared attention: rows of {qkv.shape[1]} do not hold {n_heads} heads of {head_dim}")
+    if tuple(k_pool.shape[1:]) != (n_kv, page_size, head_dim) or k_pool.shape != v_pool.shape:
+        raise ValueError(f"shared attention: pools {tuple(k_pool.shape)} and {tuple(v_pool.shape)} are not pages of {page_size} positions "
+                         f"of {n_kv} heads of {head_dim}")
+    if slots.numel() != B or shared.row_group.numel() != B or slot_len.numel() != page_table.shape[0]:
+        raise ValueError("shared attention: slots, groups of rows or lengths do not fit the batch and the page table")
+    if ring and not (window and window <= ring <= page_table.shape[1] * page_size):
+        raise ValueError(f"shared attention: a ring of {ring} positions needs a window within it and a page table that holds it")
+    if window is not None and window < 0:
+        raise ValueError("shared attention: a negative window")
+    if scratch.numel() * scratch.element_size() < plan.scratch_bytes or plan.scratch_bytes < B * n_heads * (plan.common_ranges + plan.own_ranges) * (head_dim + 2) * 4:
+        raise ValueError("shared attention: scratch is too small for the plan, or the plan for the batch")
+    _on_current_device(qkv, k_pool, v_pool, page_table, slots, slot_len, shared.groups, shared.row_group, scratch)
+    out = torch.empty((B, n_heads * head_dim), dtype=qkv.dtype, device=qkv.device)
+    part_o = scratch.data_ptr()
+    part_ml = part_o + B * n_heads * (plan.common_ranges + plan.own_ranges) * head_dim * 4
+    _lib.check(_lib.load().qnn_attn_decode_shared(
+        _p(qkv), ld, dt_code(qkv), _p(k_pool), _p(v_pool), _p(page_table), page_table.shape[1], page_size, ring, _p(slots), _p(slot_len), B,
+        _p(shared.groups), shared.groups.shape[0], shared.rows, _p(shared.row_group), n_heads, n_kv, head_dim, float(scale), float(cap or 0.0),
+        int(window or 0), plan.common_ranges, plan.own_ranges, part_o, part_ml, _p(out), out.shape[1], _p(slopes), _p(sinks), _stream()),
+        "attn_decode_shared", 2)
+    return out
+
+
+BEAM_MOST = 64                   # continuations per request that beam_select returns at most
+
+
+def beam_select_scratch_bytes(rows: int, vocab: int, take: int) -> int:
+    """Scratch of ``beam_select`` for so many rows (requests x beams)."""
+    if not 1 <= take <= BEAM_MOST:
+        raise ValueError(f"beam selection returns 1..{BEAM_MOST} continuations per request, not {take}")
+    return 8 * rows * int(_lib.load().qnn_beam_select_segments(vocab))
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, take: int, scratch: torch.Tensor,
+                out: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]] = None, error_flag: Optional[torch.Tensor] = None,
+                status: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The ``take`` best continuations of every request over its ``beams`` beams and the vocabulary.
+
+    ``logits`` [requests * beams, vocab] float32, ``scores`` [requests * beams] float32 (the beams' sums of log-probabilities; -inf: a beam
+    that is not there).  Returns (scores, beams, tokens), each [requests, take], best first: score + log softmax(logits) of a continuation
+    (formed in 64 bits, rounded once), its beam within the request and its token; equal scores in the order of (beam, token).  Places that
+    nothing is left for hold -inf, -1, -1.  A logit that is not finite is never chosen and sets bit 0 of ``error_flag``; ``status`` joins the
+    error word as in ``sample``."""
+    _req(logits, "logits", torch.float32, 2)
+    _req(scores, "scores", torch.float32, 1)
+    R, V = logits.shape
+    if beams < 1 or R % beams or scores.numel() != R:
+        raise ValueError(f"beam selection: {R} rows and {scores.numel()} scores are not requests of {beams} beams")
+    if not 1 <= take <= BEAM_MOST:
+        raise ValueError(f"beam selection returns 1..{BEAM_MOST} continuations per request, not {take}")
+    if scratch.numel() * scratch.element_size() < beam_select_scratch_bytes(R, V, take):
+        raise ValueError("beam selection: scratch is too small")
+    _req(scratch, "scratch")
+    Q = R // beams
+    if out is None:
+        out = (torch.empty((Q, take), dtype=torch.float32, device=logits.device),
+               torch.empty((Q, take), dtype=torch.int32, device=logits.device), torch.empty((Q, take), dtype=torch.int32, device=logits.device))
+    for t, dt, what in zip(out, (torch.float32, torch.int32, torch.int32), ("scores", "beams", "tokens")):
+        _req(t, f"out {what}", dt, 2)
+        if tuple(t.shape) != (Q, take):
+            raise ValueError(f"beam selection: the output {what} are {tuple(t.shape)}, not {(Q, take)}")
+    _on_current_device(logits, scores, scratch, *out)
+    _lib.check(_lib.load().qnn_beam_select(_p(logits), _p(scores), Q, beams, V, take, _p(scratch), _p(out[0]), _p(out[1]), _p(out[2]), _p(status),
+                                           _p(error_flag), _stream()), "beam_select", 2)
+    return out
+
+
+def _check_moves(src: Sequence[int], dst: Sequence[int], lowest: int, n: int, what: str) -> None:
+    if len(src) != len(dst):
+        raise ValueError(f"{what}: {len(src)} sources for {len(dst)} destinations")
+    if len(set(dst)) != len(dst):
+        raise ValueError(f"{what}: a destination appears twice")
+    if not set(dst).isdisjoint(src):
+        raise ValueError(f"{what}: a destination is a source as well")
+    if min(min(src), min(dst)) < lowest or max(max(src), max(dst)) >= n:
+        raise ValueError(f"{what}: {lowest}..{n - 1} can be copied, asked for {sorted(set(src) | set(dst))}")
+
+
+def copy_slots(tensors: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[int]) -> None:
+    """``t[dst[i]] = t[src[i]]`` for every tensor (rows along its first dimension, any type) and every pair, in one launch for up to 64
+    tensors and 128 pairs.  A row may be copied to several others; no destination may appear twice or be a source."""
+    if not len(src) and not len(dst):
+        return
+    if not tensors:
+        _check_moves(src, dst, 0, 1 << 31, "copy_slots")
+        return
+    _check_moves(src, dst, 0, min(t.shape[0] if t.dim() else 0 for t in tensors), "copy_slots")
+    for t in tensors:
+        _req(t, "a tensor of copy_slots")
+    _on_current_device(*tensors)
+    n, p = len(tensors), len(src)
+    launched = ctypes.c_int(0)
+    base = (ctypes.c_void_p * n)(*[t.data_ptr() for t in tensors])
+    size = (ctypes.c_longlong * n)(*[t.numel() // t.shape[0] * t.element_size() for t in tensors])
+    code = _lib.load().qnn_copy_slots(base, size, n, (ctypes.c_int * p)(*src), (ctypes.c_int * p)(*dst), p, ctypes.byref(launched), _stream())
+    _lib.check(code, "copy_slots", launched.value)
+
+
+def copy_pages(k: torch.Tensor, v: torch.Tensor, src: Sequence[int], dst: Sequence[int], used: Sequence[int]) -> None:
+    """The first ``used[i]`` positions of page ``src[i]`` to page ``dst[i]``, in every line and head of the pools ``k`` and ``v``
+    ([lines, pages, kv heads, positions, head size]; the same tensor twice for lines without values).  Cells behind them keep what they
+    hold.  No destination may appear twice, be a source, or be page 0, which belongs to nobody."""
+    if len(used) != len(src):
+        raise ValueError(f"copy_pages: {len(used)} lengths for {len(src)} pages")
+    if not len(src) and not len(dst):
+        return
+    _req(k, "k", None, 5)
+    _req(v, "v", k.dtype, 5)
+    if k.shape != v.shape:
+        raise ValueError(f"copy_pages: pools of different shapes, {tuple(k.shape)} and {tuple(v.shape)}")
+    lines, pages, heads, page, dim = k.shape
+    _check_moves(src, dst, 1, pages, "copy_pages")
+    if min(used) < 0 or max(used) > page:
+        raise ValueError(f"copy_pages: a page holds {page} positions")
+    _on_current_device(k, v)
+    p = len(src)
+    launched = ctypes.c_int(0)
+    code = _lib.load().qnn_copy_pages(_p(k), _p(v), lines, pages, heads, page, dim, k.element_size(), (ctypes.c_int * p)(*src), (ctypes.c_int * p)(*dst),
+                                      (ctypes.c_int * p)(*used), p, ctypes.byref(launched), _stream())
+    _lib.check(code, "copy_pages", launched.value)
