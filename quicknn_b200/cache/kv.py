@@ -13,6 +13,8 @@ the window only limits reads, shaders/attention.comp:24):
   per sequence: position p lives at ring index ``p mod ring``;
 * sizes are in tokens: ``max_tokens`` is the most tokens that live sequences hold
   at one time, each rounded up to a whole page;
+* sequences that go on from a common one (``fork``) hold its pages together; whoever has to write into such a page
+  gets a copy of its own first (``extend``), so nobody sees another's tokens;
 * fixed-size state per (state line, slot), zeroed when the slot is handed out,
   never rewound (the reference keeps such state inside its recurrent models and
   resets it on a prefix mismatch, src/models/QuickNN.Models.LLM.pas:723-731).
@@ -26,6 +28,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 import numpy as np
 import torch
 
+from ..kernels import ops as kernel_ops
 from ..parts.base import CacheNeed, StateNeed
 from .pages import PAGE, CacheFull, PagePool, SlotTable
 from .upload import PinnedUploader
@@ -50,6 +53,7 @@ class LineView:
     index: int = -1                 # which cache line this is (a key for what layers hand each other within a step)
     block_state: Optional[torch.Tensor] = None   # [slots, *shape]: fixed-size state of the block around the mixer, or None
     has_readers: bool = False       # another scheduled layer reads this line after its writer (set by the model)
+    group: int = -1                 # which group of the cache the line is in (a key for what a step knows of shared pages)
 
 
 # Page tables and lengths up to this size go to the device together, however few rows changed: a copy of 32 KB takes the stream
@@ -140,6 +144,11 @@ class KVCache:
 
         self.state = regions(states)
         self.block_state = regions(block_states)
+        # sequences that came from one another by ``fork`` are of one family; how many live ones each family has
+        self._family: List[int] = [-1] * max_slots
+        self._members: Dict[int, int] = {}
+        self._families = 0
+        self.sharing = 0                           # live families of two or more
         # a slot's part of every state, made when the slot is first used: one call clears a new sequence's
         self._slot_states: List[Optional[List[torch.Tensor]]] = [None] * max_slots
 
@@ -152,6 +161,8 @@ class KVCache:
         self.lengths_host[slot] = 0
         self.longest_host[slot] = 0
         self._lengths_dirty = True
+        self._join(slot, self._families)
+        self._families += 1
         if self.state or self.block_state:
             parts = self._slot_states[slot]
             if parts is None:
@@ -159,8 +170,55 @@ class KVCache:
             torch._foreach_zero_(parts)
         return slot
 
+    def _join(self, slot: int, family: int) -> None:
+        n = self._members.get(family, 0) + 1
+        self._members[family] = n
+        self._family[slot] = family
+        self.sharing += n == 2
+
+    def _leave(self, slot: int) -> None:
+        family = self._family[slot]
+        self._family[slot] = -1
+        n = self._members[family] - 1
+        self.sharing -= n == 1
+        if n:
+            self._members[family] = n
+        else:
+            del self._members[family]
+
+    def fork(self, sources: Sequence[int]) -> List[int]:
+        """A new sequence for every entry of ``sources`` (slots, some perhaps several times) that holds what the source holds:
+        its pages together with it, its states copied.  Either all are made or, with ``CacheFull``, none."""
+        for s in sources:
+            if not self.slots.is_live(s):
+                raise RuntimeError(f"slot {s} is not in use")
+        if len(sources) > self.slots.n_free:
+            raise CacheFull(f"{len(sources)} sequence slots wanted, {self.slots.n_free} free of {self.max_slots}")
+        made: List[int] = []
+        for s in sources:
+            slot = self.slots.take()
+            made.append(slot)
+            for g in self.groups:
+                g.pool.share(g.held[s])
+                g.held[slot] = list(g.held[s])
+                g.table_host[slot] = g.table_host[s]
+                g.dirty.add(slot)
+            self.lengths_host[slot] = self.lengths_host[s]
+            self.longest_host[slot] = self.longest_host[s]
+            self._join(slot, self._family[s])
+        self._lengths_dirty = True
+        states = self._all_states()
+        if states and made:
+            if states[0].is_cuda:
+                kernel_ops.copy_slots(states, list(sources), made)
+            else:
+                for t in states:
+                    t[made] = t[list(sources)]
+        return made
+
     def free(self, slot: int) -> None:
         self.slots.give_back(slot)                      # raises on a double free
+        self._leave(slot)
         for g in self.groups:
             g.pool.give_back(g.held[slot])
             g.held[slot] = []
@@ -181,6 +239,8 @@ class KVCache:
         """Grow sequences to new lengths: ``[(slot, new_length), ...]``.  Either all fit or
         nothing changes."""
         want: List[List[Tuple[int, int]]] = [[] for _ in self.groups]
+        # pages that the new tokens go into and that other sequences hold too, by group: (slot, index, cells in use)
+        split: List[List[Tuple[int, int, int]]] = [[] for _ in self.groups]
         for slot, new_len in slot_lengths:
             if not self.slots.is_live(slot):
                 raise RuntimeError(f"slot {slot} is not in use")
@@ -193,12 +253,27 @@ class KVCache:
                 extra = g.pages_for(new_len) - len(g.held[slot])
                 if extra > 0:
                     want[gi].append((slot, extra))
+            if self._members[self._family[slot]] > 1:
+                self._written_shared(slot, new_len, split)
         for gi, g in enumerate(self.groups):
-            total = sum(e for _, e in want[gi])
+            if split[gi]:                       # the last holder of a page writes into it as it is
+                left: Dict[int, int] = {}
+                kept = []
+                for slot, i, used in split[gi]:
+                    p = g.held[slot][i]
+                    n = left.get(p, g.pool.holders(p))
+                    if n > 1:
+                        kept.append((slot, i, used))
+                        left[p] = n - 1
+                split[gi] = kept
+        for gi, g in enumerate(self.groups):
+            total = sum(e for _, e in want[gi]) + len(split[gi])
             if total > g.pool.n_free:
                 raise CacheFull(f"the cache holds at most {self.max_tokens} tokens "
                                 f"({g.pool.n_free} free pages of {PAGE}, {total} needed)")
         for gi, g in enumerate(self.groups):
+            if split[gi]:
+                self._split(g, split[gi])
             for slot, extra in want[gi]:
                 start = len(g.held[slot])
                 pages = g.pool.take(extra)
@@ -209,6 +284,43 @@ class KVCache:
             self.lengths_host[slot] = new_len
             self.longest_host[slot] = max(int(self.longest_host[slot]), new_len)
         self._lengths_dirty = True
+
+    def _written_shared(self, slot: int, new_len: int, split) -> None:
+        """Note the pages that tokens up to ``new_len`` are written into and that have other holders."""
+        length = int(self.lengths_host[slot])
+        if new_len <= length:
+            return
+        for gi, g in enumerate(self.groups):
+            held = g.held[slot]
+            first, last = length // PAGE, (new_len - 1) // PAGE
+            for n in range(first, min(last, first + g.pages_per_seq) + 1):
+                i = n % g.pages_per_seq if g.ring else n
+                if i >= len(held):               # a page that is taken anew (in a ring older ones may follow)
+                    continue
+                if g.pool.holders(held[i]) > 1 and not any(s == slot and j == i for s, j, _ in split[gi]):
+                    # in a later lap of a ring the cells behind the new tokens still hold the lap before
+                    again = g.ring and n >= g.pages_per_seq
+                    split[gi].append((slot, i, PAGE if again else max(0, length - n * PAGE)))
+
+    def _split(self, g: "CacheGroup", pages: Sequence[Tuple[int, int, int]]) -> None:
+        """Give every (slot, index) of ``pages`` a page of its own with a copy of the cells in use."""
+        new = g.pool.take(len(pages))
+        old = [g.held[slot][i] for slot, i, _ in pages]
+        moves = [(s, d, u) for s, d, (_, _, u) in zip(old, new, pages) if u]
+        if moves:
+            src, dst, used = (list(x) for x in zip(*moves))
+            if g.k.is_cuda:
+                kernel_ops.copy_pages(g.k, g.v, src, dst, used)
+            else:
+                for pool in (g.k, g.v) if g.need.values else (g.k,):
+                    for s, d, u in moves:
+                        pool[:, d, :, :u] = pool[:, s, :, :u]
+        # only now, with every copy queued, do the old pages lose a holder
+        for (slot, i, _), o, n in zip(pages, old, new):
+            g.held[slot][i] = n
+            g.table_host[slot, i] = n
+            g.dirty.add(slot)
+        g.pool.give_back(old)
 
     def truncate(self, slot_lengths: Sequence[Tuple[int, int]]) -> None:
         """Shorten sequences to earlier lengths and give back the pages beyond them: the undo of
@@ -264,6 +376,52 @@ class KVCache:
             self.uploader.send(self.lengths_dev, self.lengths_host)
             self._lengths_dirty = False
 
+    # ---- what the rows of a step share ----------------------------------------------------
+    def families(self, slots: Sequence[int]) -> List[Tuple[int, int]]:
+        """(first row, rows) of the stretches of two or more neighbouring rows whose sequences came from one another."""
+        out: List[Tuple[int, int]] = []
+        if not self.sharing:
+            return out
+        start = 0
+        for r in range(1, len(slots) + 1):
+            if r == len(slots) or self._family[slots[r]] != self._family[slots[start]]:
+                if r - start > 1:
+                    out.append((start, r - start))
+                start = r
+        return out
+
+    def shared_positions(self, slots: Sequence[int], runs: Sequence[Tuple[int, int]]) -> List[np.ndarray]:
+        """For every group of the cache and every run (first row, rows) of rows: the positions begin .. end - 1 that lie in the same
+        pages in all of the run's sequences, as int32 [runs, 2]; the last such stretch where a ring leaves several.  Whole pages:
+        ``end`` may lie behind what some row holds."""
+        first = np.asarray([r for r, _ in runs])
+        rows = np.concatenate([np.arange(r, r + n) for r, n in runs])
+        of = np.repeat(np.arange(len(runs)), [n for _, n in runs])
+        starts = np.concatenate([[0], np.cumsum([n for _, n in runs])[:-1]])
+        slot = np.asarray(slots)[rows]
+        shortest = np.minimum.reduceat(self.lengths_host[slot], starts)
+        out = []
+        for g in self.groups:
+            lead = g.table_host[np.asarray(slots)[first]]                       # [runs, pages per sequence]
+            same = np.logical_and.reduceat(g.table_host[slot] == lead[of], starts) & (lead != 0)
+            n = g.pages_per_seq
+            # page numbers in the order of positions; in a ring the newest `n` of the shortest row
+            base = np.maximum((shortest - 1) // PAGE - n + 1, 0) if g.ring else np.zeros(len(runs), dtype=np.int64)
+            if g.ring:
+                same = np.take_along_axis(same, (base[:, None] + np.arange(n)) % n, axis=1)
+                last = n - 1 - np.argmax(same[:, ::-1], axis=1)                 # the last shared page, and the one behind the hole before it
+                hole = np.where((np.arange(n) < last[:, None]) & ~same, np.arange(n), -1).max(axis=1)
+                begin, end = hole + 1, last + 1
+                none = ~same.any(axis=1)
+            else:
+                begin = np.zeros(len(runs), dtype=np.int64)
+                end = np.where(same.all(axis=1), n, np.argmin(same, axis=1))
+                none = end == 0
+            both = np.stack([(base + begin) * PAGE, (base + end) * PAGE], axis=1)
+            both[none] = 0
+            out.append(both.astype(np.int32))
+        return out
+
     # ---- views ------------------------------------------------------------------------
     def line(self, line: int, writes: bool = True) -> Optional[LineView]:
         st, bst = self.state.get(line), self.block_state.get(line)
@@ -274,7 +432,7 @@ class KVCache:
         gi, li = self._line_group[line]
         g = self.groups[gi]
         return LineView(g.k[li], g.v[li], g.table_dev, g.ring, PAGE, self.lengths_dev, st, writes, g.need.values, index=line,
-                        block_state=bst)
+                        block_state=bst, group=gi)
 
     def bytes(self) -> int:
         return sum(g.bytes() for g in self.groups) + sum(t.numel() * t.element_size() for t in self._all_states())
@@ -306,17 +464,17 @@ class KVCache:
             raise AssertionError("the lengths on the device differ from the host's")
 
     def audit(self) -> None:
-        """No page lost, held twice or freed twice; tables agree with what slots hold."""
+        """No page lost or freed twice, none held by sequences that did not come from one another; tables agree with what slots hold."""
         for g in self.groups:
             g.pool.audit()
-            seen = set()
+            seen: Dict[int, int] = {}
             for slot, pages in enumerate(g.held):
                 if pages and not self.slots.is_live(slot):
                     raise AssertionError(f"free slot {slot} still holds pages")
                 for i, p in enumerate(pages):
-                    if p in seen:
-                        raise AssertionError(f"page {p} is held twice")
-                    seen.add(p)
+                    if p in pages[:i]:
+                        raise AssertionError(f"page {p} is held twice by slot {slot}")
+                    seen[p] = seen.get(p, 0) + 1
                     if g.table_host[slot, i] != p:
                         raise AssertionError(f"page table of slot {slot} disagrees with its pages")
                 if len(pages) != g.pages_for(int(self.lengths_host[slot])) and self.slots.is_live(slot):
@@ -324,3 +482,8 @@ class KVCache:
                                          f"{self.lengths_host[slot]} tokens")
             if len(seen) != g.pool.n_held:
                 raise AssertionError("the pool counts pages that no slot holds")
+            for p, n in seen.items():
+                if g.pool.holders(p) != n:
+                    raise AssertionError(f"page {p} is held by {n} sequences, the pool counts {g.pool.holders(p)}")
+                if n > 1 and len({self._family[s] for s, pages in enumerate(g.held) if p in pages}) != 1:
+                    raise AssertionError(f"page {p} is shared by sequences that have nothing in common")

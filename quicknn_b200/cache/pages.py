@@ -18,14 +18,15 @@ class CacheFull(RuntimeError):
 class PagePool:
     """Pages 1..n_pages-1 can be handed out; page 0 is never handed out: unused
     page-table entries point at it, so a stray read or a padding row's write lands
-    in memory that no sequence owns."""
+    in memory that no sequence owns.  A page may have several holders (sequences that
+    went on from a common one); it is free again when the last one gives it back."""
 
     def __init__(self, n_pages: int):
         if n_pages < 2:
             raise ValueError("a page pool needs at least one usable page besides page 0")
         self.n_pages = n_pages
         self._free: List[int] = list(range(n_pages - 1, 0, -1))   # pop() gives the lowest id first
-        self._held = [False] * n_pages
+        self._held = [0] * n_pages                                # holders of every page
 
     @property
     def n_free(self) -> int:
@@ -42,8 +43,18 @@ class PagePool:
         out = self._free[keep:][::-1]
         del self._free[keep:]
         for p in out:
-            self._held[p] = True
+            self._held[p] = 1
         return out
+
+    def share(self, pages: Iterable[int]) -> None:
+        """One more holder for pages that have one."""
+        for p in pages:
+            if p <= 0 or p >= self.n_pages or not self._held[p]:
+                raise RuntimeError(f"page {p} is not held by anyone")
+            self._held[p] += 1
+
+    def holders(self, page: int) -> int:
+        return self._held[page]
 
     def give_back(self, pages: Iterable[int]) -> None:
         for p in pages:
@@ -51,15 +62,16 @@ class PagePool:
                 raise ValueError(f"page {p} is not a page of this pool")
             if not self._held[p]:
                 raise RuntimeError(f"page {p} is freed twice or was never handed out")
-            self._held[p] = False
-            self._free.append(p)
+            self._held[p] -= 1
+            if not self._held[p]:
+                self._free.append(p)
 
     def audit(self) -> None:
         free = set(self._free)
         if len(free) != len(self._free):
             raise AssertionError("a page is on the free list twice")
         for p in range(1, self.n_pages):
-            if self._held[p] == (p in free):
+            if bool(self._held[p]) == (p in free):
                 raise AssertionError(f"page {p} is {'both held and free' if self._held[p] else 'lost'}")
         if self._held[0] or 0 in free:
             raise AssertionError("page 0 left its place")

@@ -5,6 +5,7 @@ generation options carry the reference's names and defaults
 Examples/LLMChat/QuickNN.LLMChat.Settings.pas:38).
 
     python -m quicknn_b200 generate --model DIR --prompt-ids "5,17,3;9,4" --max-new-tokens 16 --temperature 0
+    python -m quicknn_b200 generate --model DIR --prompt-ids "5,17,3" --beams 4 --max-new-tokens 16
     python -m quicknn_b200 random   --config config.json --seed 0 --out DIR
     python -m quicknn_b200 replay   --model DIR --dtype float32 --out DIR --max-tokens 4096 < trace.jsonl
     python -m quicknn_b200 info     --model DIR
@@ -41,16 +42,25 @@ def _prompts(args) -> List[List[int]]:
 
 def cmd_generate(args) -> int:
     from .engine import LLM
-    from .sampling import GenerationOptions
+    from .sampling import BeamOptions, GenerationOptions
     import torch
     if not torch.cuda.is_available():
         print("generate: no CUDA device; quicknn_b200 has no CPU path", file=sys.stderr)
         return 3
     prompts = _prompts(args)
+    prefix = [int(x) for x in args.prefix_ids.replace(",", " ").split()] if args.prefix_ids else None
+    if args.beams and (args.turns or args.stream or prefix):
+        raise SystemExit("generate: --beams goes without --turns, --stream and --prefix-ids")
+    if args.turns and prefix:
+        raise SystemExit("generate: --turns goes without --prefix-ids")
     opts = GenerationOptions(max_new_tokens=args.max_new_tokens, hard_max_new_tokens=args.hard_max_new_tokens,
                              top_k=args.top_k, auto_continue=args.auto_continue, temperature=args.temperature,
                              top_p=args.top_p, repetition_penalty=args.repetition_penalty, seed=args.seed)
     opts.validate()
+    if args.beams:
+        beam_opts = BeamOptions(beams=args.beams, max_new_tokens=args.max_new_tokens, length_penalty=args.length_penalty,
+                                early_stopping=args.early_stopping, replies=args.replies)
+        beam_opts.validate()
     llm = LLM(args.model, max_context=args.max_context, max_batch=args.max_batch, dtype=args.dtype,
               device=args.device)
     stops = None if args.stop_ids is None else [int(x) for x in args.stop_ids.replace(",", " ").split()]
@@ -60,8 +70,10 @@ def cmd_generate(args) -> int:
             print(json.dumps({"request": i, "token": tok}), flush=True)
 
     def run():
+        if args.beams:
+            return llm.beam_search(prompts, beam_opts, stop_ids=stops)
         if not args.turns:
-            return llm.generate(prompts, opts, on_token=on_token, stop_ids=stops)
+            return llm.generate(prompts, opts, on_token=on_token, stop_ids=stops, prefix=prefix)
         # the prompts are the turns of one conversation: each is appended to what was said so far, and only
         # what the cache does not hold yet is run
         out, said = [], []
@@ -84,6 +96,12 @@ def cmd_generate(args) -> int:
     except KeyboardInterrupt:
         print("cancelled", file=sys.stderr)
         return 130
+    if args.beams:
+        for r in results:
+            print(json.dumps({"request": r.index, "prompt_tokens": r.prompt_tokens,
+                              "replies": [{"tokens": h.tokens, "score": round(h.score, 6), "logprob": round(h.logprob, 6),
+                                           "finish_reason": h.finish_reason} for h in r.replies]}))
+        results = []
     for r in results:
         print(json.dumps({"request": r.index, "prompt_tokens": r.prompt_tokens, "tokens": r.tokens,
                           "finish_reason": r.finish_reason, "reused_tokens": r.reused_tokens,
@@ -254,6 +272,11 @@ def main(argv=None) -> int:
     g.add_argument("--turns", action="store_true",
                    help="the prompts are successive turns of one conversation that keeps its cache (reused_tokens "
                         "says how much of each turn's prompt was found there)")
+    g.add_argument("--prefix-ids", default=None, help="ids that stand in front of every prompt; they run once for all of them")
+    g.add_argument("--beams", type=int, default=0, help="beam search with so many beams per prompt (the sampling options do not apply)")
+    g.add_argument("--length-penalty", type=float, default=1.0, help="beams: a reply scores its log-probability over length ** this")
+    g.add_argument("--early-stopping", action="store_true", help="beams: a request is over once as many replies as beams have ended")
+    g.add_argument("--replies", type=int, default=1, help="beams: how many of the best replies to print")
     g.add_argument("--profile", action="store_true",
                    help="time every step and every kind of part with CUDA events (steps then run eagerly) and print a table")
     g.set_defaults(fn=cmd_generate)

@@ -27,6 +27,20 @@ class WholeSequences:
 
 
 @dataclasses.dataclass
+class StepSharing:
+    """The rows of a decode step whose sequences came from one another (``KVCache.fork``) and hold pages together: ``n_groups`` stretches
+    of at most ``rows`` neighbouring rows; bounds of the keys that a group holds together and that a row has beside them, over all
+    groups of the cache (classes: powers of two); and, on the device, what the attention reads of them for each group of the cache
+    (``kernels.ops.SharedKeys``)."""
+
+    n_groups: int
+    rows: int
+    keys: int
+    own: int
+    by_group: Tuple[Any, ...] = ()
+
+
+@dataclasses.dataclass
 class DepthHistory:
     """What the layers of a model that averages over depth leave for the layers after them, for one step."""
 
@@ -79,6 +93,7 @@ class StepBatch:
     whole: Optional[WholeSequences] = None    # extend steps: the sequences with their cached tokens in front
     longest: int = 0                          # decode: class of the longest sequence (an upper bound), 0 = unknown
     spread: float = 0.0                       # decode: class of longest / mean length (1.0, 1.25, 1.6 or 2.2), 0 = unknown
+    sharing: Optional[StepSharing] = None     # decode: rows that hold pages together, None = none do
     # What the writer of a cache line leaves, under the line's index, for the layers that read the line later in the
     # same step: its packed rows with this step's keys and values as the cache gets them (and their head shape).  A
     # prompt longer than a ring has lost its first keys from the cache by then; its own rows still have them.

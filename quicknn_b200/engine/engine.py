@@ -11,6 +11,7 @@ LLM.pas:459-493, 715-745), or start some sequences beside others that go on.
 """
 from __future__ import annotations
 
+import dataclasses
 from array import array
 from typing import Any, Dict, List, Mapping, Optional, Sequence, Tuple, Union
 
@@ -20,7 +21,7 @@ import torch
 from ..cache import PAGE, CacheFull, KVCache
 from ..kernels import lib as _klib
 from ..kernels import ops as _kops
-from .batch import StepBatch, WholeSequences
+from .batch import StepBatch, StepSharing, WholeSequences
 from .model import Model
 
 MAX_DECODE_GRAPHS = 256       # decode states (graph, buffers, scratch) kept at a time, over batch sizes, samplers and schedules
@@ -74,6 +75,12 @@ class Engine:
     # ---- sequences -------------------------------------------------------------------
     def new_sequence(self) -> int:
         return self.cache.allocate()
+
+    def fork(self, slots: Sequence[int]) -> List[int]:
+        """A new sequence for every entry of ``slots`` (one may be named several times) that goes on from there: it holds what the
+        source holds, the source stays as it is.  Nothing is run; pages are held together until somebody writes into them, states are
+        copied.  A decode step whose neighbouring rows came from one another reads what they hold together once."""
+        return self.cache.fork(slots)
 
     def release(self, slot: int) -> None:
         self.cache.free(slot)
@@ -256,6 +263,34 @@ class Engine:
         ratio = longest * len(lengths) / max(1, sum(lengths))
         return bound, (1.0 if ratio < 1.1 else (1.25 if ratio < 1.4 else (1.6 if ratio < 1.9 else 2.2)))
 
+    def _sharing(self, slots, lengths):
+        """What the rows of a decode step hold together: (bounds as ``StepSharing``, what the kernels read of it as one int32 array per
+        group of the cache, a row's group) or None.  The numbers of groups and rows are rounded up to powers of two, as the other bounds
+        are, so that a graph serves many steps."""
+        runs = self.cache.families(slots)
+        if not runs:
+            return None
+        ranges = self.cache.shared_positions(slots, runs)
+        up = lambda n: 1 << max(int(n) - 1, 0).bit_length()  # noqa: E731
+        n_groups, most = up(len(runs)), up(max(n for _, n in runs))
+        row_group = np.full(len(slots), -1, np.int32)
+        tables, keys, own = [], 0, 1
+        lens = np.asarray(lengths)
+        for i, (r, n) in enumerate(runs):
+            row_group[r:r + n] = i
+        for g, ab in zip(self.cache.groups, ranges):
+            table = np.zeros((n_groups, 4), np.int32)
+            table[:len(runs), :2] = runs
+            table[:len(runs), 2:] = ab
+            tables.append(table)
+            together = np.where(row_group >= 0, (ab[:, 1] - ab[:, 0])[row_group], 0)
+            keys = max(keys, int(together.max()))
+            held = np.minimum(lens, g.need.window) if g.ring else lens
+            own = max(own, int((held - np.minimum(together, held)).max()))
+        if not tables or not keys:
+            return None
+        return StepSharing(n_groups, most, up(keys), up(max(own, 64))), tables, row_group
+
     def _decode(self, slots, starts, tokens_dev, use_graph, tail, rows):
         n_seqs, B = len(slots), rows                 # B rows, of which the last B - n_seqs belong to no sequence
         self.cache.sync()
@@ -263,31 +298,43 @@ class Engine:
         longest, spread = self.length_classes([p + 1 for p in starts])
         # a graph per batch size, sampler and schedule that the parts derive from the length classes (classes
         # that lead to the same decisions share one); the schedule of a class is asked once
-        shape = (B, longest, spread, tuple(sorted(self.tuning.items())))
+        shared = self._sharing(slots, [p + 1 for p in starts])
+        bounds = shared[0] if shared is not None else None
+        held = (bounds.n_groups, bounds.rows, bounds.keys, bounds.own) if shared is not None else None
+        shape = (B, longest, spread, held, tuple(sorted(self.tuning.items())))
         sched = self._schedules.get(shape)
         if sched is None:
             probe = StepBatch("decode", B, B, None, None, None, None, None, None, self.model.dtype, max_seq=self.max_seq,
-                              tuning=self.tuning, want_every_row=True, longest=longest, spread=spread)
+                              tuning=self.tuning, want_every_row=True, longest=longest, spread=spread, sharing=bounds)
             sched = self._schedules[shape] = hash(self.model.schedule(probe))
-        key = (B, id(tail) if tail is not None else None, sched)
+        key = (B, id(tail) if tail is not None else None, sched, held and held[:2])
         st = self._decode_state.pop(key, None)
         if st is not None:
             self._decode_state[key] = st                          # most recently used last
         else:
             if len(self._decode_state) >= MAX_DECODE_GRAPHS:     # the least recently used goes (graph, buffers, scratch)
                 del self._decode_state[next(iter(self._decode_state))]
-            meta = torch.zeros(2 * B, dtype=torch.int32, device=self.device)
+            # positions and slots of the rows; with shared pages the groups of rows in front (16-byte pieces) and a row's group behind
+            front = 4 * len(self.cache.groups) * bounds.n_groups if shared is not None else 0
+            whole = torch.zeros(front + (3 if shared is not None else 2) * B, dtype=torch.int32, device=self.device)
+            meta = whole[front:]
             ar = torch.arange(B, dtype=torch.int32, device=self.device)
             tokens = torch.zeros(B, dtype=torch.int32, device=self.device)
-            step = StepBatch("decode", B, B, tokens, meta[:B], meta[B:], ar, meta[B:], ar, self.model.dtype,
+            step = StepBatch("decode", B, B, tokens, meta[:B], meta[B:2 * B], ar, meta[B:2 * B], ar, self.model.dtype,
                              max_seq=self.max_seq, tuning=self.tuning, want_every_row=True, longest=longest,
                              spread=spread)
+            if shared is not None:
+                step.sharing = dataclasses.replace(bounds, by_group=tuple(
+                    _kops.SharedKeys(t, meta[2 * B:], rows=bounds.rows, keys=bounds.keys, own=bounds.own)
+                    for t in whole[:front].view(len(self.cache.groups), bounds.n_groups, 4).unbind(0)))
             self._give_scratch(step)
-            st = {"meta": meta, "step": step, "graph": None, "logits": None, "tail": tail}    # holds `tail` alive: its id is the key
+            st = {"meta": whole, "step": step, "graph": None, "logits": None, "tail": tail}    # holds `tail` alive: its id is the key
             self._decode_state[key] = st
         pad_rows = B - n_seqs
-        self.cache.uploader.send(st["meta"], np.concatenate([np.asarray(list(starts) + [0] * pad_rows, np.int32),
-                                                             np.asarray(list(slots) + [-1] * pad_rows, np.int32)]))
+        parts = [np.asarray(list(starts) + [0] * pad_rows, np.int32), np.asarray(list(slots) + [-1] * pad_rows, np.int32)]
+        if shared is not None:
+            parts = [t.reshape(-1) for t in shared[1]] + parts + [shared[2], np.full(pad_rows, -1, np.int32)]
+        self.cache.uploader.send(st["meta"], np.concatenate(parts))
         st["step"].tokens[:n_seqs].copy_(tokens_dev.reshape(-1))
         self.steps_run += 1
         if pad_rows:

@@ -13,10 +13,12 @@ import torch
 from ..config.base import Architecture, ModelConfig, find_architecture
 from ..config.generation import stop_ids_of_folder
 from ..cache.pages import PAGE, CacheFull
-from ..sampling import GenerationOptions, Sampler
+from ..sampling import BeamOptions, BeamSelector, GenerationOptions, Sampler
+from ..sampling.beam import check_beams
 from ..weights.random_init import random_tensors
+from .beam import BeamResult, EngineBeams, beam_search
 from .engine import Engine
-from .generate import GenerationBackend, GenerationResult, generate
+from .generate import GenerationBackend, GenerationResult, PromptError, generate, plan_batches
 from .model import Model, as_dtype
 
 class _Backend(GenerationBackend):
@@ -66,14 +68,18 @@ class _Backend(GenerationBackend):
             return None
 
     def begin(self, first_index: int, prompts: Sequence[Sequence[int]]) -> np.ndarray:
+        self.slots = [self.engine.new_sequence() for _ in prompts]
+        return self._start(first_index, prompts, prompts)
+
+    def _start(self, first_index: int, prompts: Sequence[Sequence[int]], new: Sequence[Sequence[int]]) -> np.ndarray:
+        """Run ``new``, what the sequences do not hold of ``prompts`` yet, and sample."""
         eng = self.engine
-        self.slots = [eng.new_sequence() for _ in prompts]
         self.sampler.start(first_index, len(prompts), self.seed)
         if self.sampler.penalised:
             toks = torch.tensor([t for p in prompts for t in p], dtype=torch.int32, device=eng.device)
             rows = torch.tensor([r for r, p in enumerate(prompts) for _ in p], dtype=torch.int32, device=eng.device)
             self.sampler.mark_prompt(toks, rows)
-        logits = eng.step(list(zip(self.slots, prompts)), "last")
+        logits = eng.step(list(zip(self.slots, new)), "last")
         self.cur = self.sampler(logits).clone()
         self.sampler.post(self.cur)
         self.ahead = self._launch_ahead()
@@ -105,6 +111,36 @@ class _Backend(GenerationBackend):
         self.slots = []
         self.cur = None
         self.ahead = None
+
+
+class _PrefixBackend(_Backend):
+    """The backend of requests behind one common text: the text runs once, on a sequence that every request forks.  With ``one_batch``
+    the last of its users is the sequence itself; otherwise it keeps a slot until ``close``."""
+
+    def __init__(self, engine: Engine, sampler: Sampler, max_batch: int, run_ahead: bool, seed: Optional[int], prefix: List[int],
+                 one_batch: bool):
+        super().__init__(engine, sampler, max_batch if one_batch else max_batch - 1, run_ahead, seed)
+        self.prefix, self.one_batch = prefix, one_batch
+        self.base: Optional[int] = None
+        if not one_batch:
+            self.max_tokens -= (len(prefix) + PAGE - 1) // PAGE * PAGE
+
+    def begin(self, first_index: int, prompts: Sequence[Sequence[int]]) -> np.ndarray:
+        eng, n = self.engine, len(prompts)
+        if self.base is None:
+            self.base = eng.new_sequence()
+            eng.step([(self.base, self.prefix)], [()])
+        if self.one_batch:
+            self.slots, self.base = [self.base], None
+            self.slots += eng.fork(self.slots * (n - 1))
+        else:
+            self.slots = eng.fork([self.base] * n)
+        return self._start(first_index, prompts, [p[len(self.prefix):] for p in prompts])
+
+    def close(self) -> None:
+        if self.base is not None:
+            self.engine.release(self.base)
+            self.base = None
 
 
 class _ConversationBackend(_Backend):
@@ -255,6 +291,7 @@ class LLM:
         self.run_ahead = True            # queue each decode step before the host reads the ids of the one before
         self.last_io: Dict[str, float] = {}
         self._samplers: Dict[tuple, Sampler] = {}
+        self._selectors: Dict[tuple, BeamSelector] = {}
 
     @classmethod
     def random(cls, config: Dict, seed: int = 0, *, dtype="bfloat16", device="cuda:0", norm_std: Optional[float] = None,
@@ -290,19 +327,60 @@ class LLM:
     def generate(self, prompts: Sequence[Sequence[int]], options: Optional[GenerationOptions] = None,
                  on_token: Optional[Callable[[int, int], Optional[bool]]] = None,
                  stop_ids: Optional[Sequence[int]] = None,
-                 should_cancel: Optional[Callable[[], bool]] = None) -> List[GenerationResult]:
+                 should_cancel: Optional[Callable[[], bool]] = None, prefix: Optional[Sequence[int]] = None) -> List[GenerationResult]:
         """Generate for a list of prompts (lists of token ids).  Requests are run in batches of
-        up to ``max_batch``, one batch after another."""
+        up to ``max_batch``, one batch after another.  ``prefix``: ids that stand in front of every prompt (each of which has at least
+        one id of its own): they run once, every request goes on from there, and the attention of the replies' steps reads their keys
+        once for all requests.  The results count them as part of the prompts, reused ones.  With more requests than a batch holds the
+        prefix keeps one of the ``max_batch`` sequences."""
         options = options or GenerationOptions()
         options.validate()
-        backend = _Backend(self.engine, self._sampler(options), self.max_batch, self.run_ahead, options.seed)
         stops = self.stop_ids if stop_ids is None else list(stop_ids)
+        prefix = list(prefix) if prefix is not None else []
+        if prefix:
+            for i, p in enumerate(prompts):
+                if not len(p):
+                    raise PromptError(f"request {i}: an empty prompt")
+            prompts = [prefix + list(p) for p in prompts]
+            cache = self.engine.cache
+            one = len(plan_batches([len(p) for p in prompts], options, self.max_batch, cache.max_tokens, self.engine.max_seq)) <= 1
+            if not one and self.max_batch < 2:
+                raise PromptError("several batches behind one prefix need a max_batch of 2 at least: the prefix keeps a sequence")
+            backend = _PrefixBackend(self.engine, self._sampler(options), self.max_batch, self.run_ahead, options.seed, prefix, one)
+        else:
+            backend = _Backend(self.engine, self._sampler(options), self.max_batch, self.run_ahead, options.seed)
         try:
-            return generate(backend, prompts, options, stops, on_token, should_cancel)
+            results = generate(backend, prompts, options, stops, on_token, should_cancel)
+            if prefix:
+                for r in results:
+                    r.reused_tokens = len(prefix)
+            return results
         finally:
+            if prefix:
+                backend.close()
             n = max(backend.decode_steps, 1)
             self.last_io = {"decode_steps": backend.decode_steps, "h2d_bytes_per_step": backend.h2d_bytes / n,
                             "d2h_bytes_per_step": backend.d2h_bytes / n}
+
+    def beam_search(self, prompts: Sequence[Sequence[int]], options: Optional[BeamOptions] = None,
+                    stop_ids: Optional[Sequence[int]] = None) -> List[BeamResult]:
+        """Replies with the highest score that beam search finds, for a list of prompts (lists of token ids): ``options.beams``
+        sequences of the batch for each, as many requests at a time as ``max_batch`` has room for."""
+        options = options or BeamOptions()
+        stops = self.stop_ids if stop_ids is None else list(stop_ids)
+        take = check_beams(options, stops)
+        if options.beams > self.max_batch:
+            raise PromptError(f"{options.beams} beams do not fit a batch of {self.max_batch}")
+        key = (options.beams, take)
+        selector = self._selectors.get(key)
+        if selector is None:
+            if len(self._selectors) > 4:
+                for old in self._selectors.values():
+                    self.engine.forget_tail(old)
+                self._selectors.clear()
+            selector = self._selectors[key] = BeamSelector(self.model.spec.embedding.vocab_size, self.max_batch // options.beams, options.beams,
+                                                           take, self.engine.device)
+        return beam_search(EngineBeams(self.engine, selector, self.max_batch), prompts, options, stops)
 
     def warm_up(self, options: Optional[GenerationOptions] = None, batch_sizes: Optional[Sequence[int]] = None,
                 context: Optional[int] = None) -> int:

@@ -2327,6 +2327,10 @@ class SharedKeys:
             raise ValueError("shared keys: bounds of rows and keys cannot be negative, and a group has a row")
         self.groups, self.row_group, self.rows, self.keys, self.own = groups, row_group, int(rows), int(keys), int(own)
 
+    @property
+    def n_groups(self) -> int:
+        return self.groups.shape[0]
+
 
 class SharedPlan(NamedTuple):
     """Into how many ranges ``attn_decode_shared`` cuts the common keys of a group and a row's own, and the scratch that takes."""
@@ -2342,7 +2346,7 @@ SHARED_ITEM_COST = 64.0          # what a CTA of that attention costs beside its
 def shared_attention_plan(dtype: torch.dtype, n_rows: int, n_heads: int, n_kv: int, head_dim: int, shared: SharedKeys,
                           window: Optional[int] = None, ranges: Optional[Tuple[int, int]] = None) -> SharedPlan:
     """How ``attn_decode_shared`` divides its work for so many rows: the cut of common and own keys into ranges of about one length
-    with the shortest estimated time.  ``ranges``: fixed numbers instead."""
+    with the shortest estimated time.  Of ``shared`` only the bounds and ``n_groups`` matter.  ``ranges``: fixed numbers instead."""
     if n_kv < 1 or n_heads % n_kv or n_rows < 0:
         raise ValueError(f"shared attention: {n_kv} kv heads do not divide {n_heads} heads")
     heads = n_heads // n_kv
@@ -2353,8 +2357,8 @@ def shared_attention_plan(dtype: torch.dtype, n_rows: int, n_heads: int, n_kv: i
         keys, own = max(shared.keys, 1), max(shared.own, 1)
         if window:
             keys, own = min(keys, window), min(own, window)
-        resident = _sm_count(shared.groups.device) * max(1, min(8, 512 // head_dim))       # CTAs at a time
-        common = shared.groups.shape[0] * (-(-shared.rows * heads // tile)) * n_kv         # walks over common keys
+        resident = _sm_count("cuda") * max(1, min(8, 512 // head_dim))       # CTAs at a time
+        common = shared.n_groups * (-(-shared.rows * heads // tile)) * n_kv         # walks over common keys
         alone = n_rows * (-(-heads // tile)) * n_kv                                        # walks over own keys
         best = None
         for c in _SHARED_CHUNKS:
@@ -2374,6 +2378,11 @@ def shared_attention_plan(dtype: torch.dtype, n_rows: int, n_heads: int, n_kv: i
     if s < 1 or p < 1:
         raise ValueError("shared attention: at least one range of each kind")
     return SharedPlan(s, p, max(n_rows, 1) * n_heads * (s + p) * (head_dim + 2) * 4)
+
+
+def shared_attention_pays(dtype: torch.dtype, n_heads: int, n_kv: int, head_dim: int, shared, window: Optional[int] = None) -> bool:
+    """Whether a decode step should read common keys once (``attn_decode_shared``) rather than once per row (``attn_decode``)."""
+    return min(shared.keys, window or shared.keys) >= 256
 
 
 _SHARED_CHUNKS = tuple(sorted({16 * int(round(2 ** (i / 2))) for i in range(4, 28)}))       # 64 keys .. 128 K

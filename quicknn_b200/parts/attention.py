@@ -242,18 +242,32 @@ class AttentionMixer(Mixer):
         spread = step.spread or 1.0
         return spread > 1.0 and not (self.window and step.longest >= 4 * self.window * spread)
 
+    def shared_plan(self, step):
+        """How a decode step whose rows share pages divides its attention, or None where every row walks its own keys: ``ops.SharedPlan``."""
+        sharing = getattr(step, "sharing", None)
+        if sharing is None or not ops.shared_attention_pays(step.act_dtype, self.n_heads, self.n_kv, self.head_dim, sharing, self.window):
+            return None
+        return ops.shared_attention_plan(step.act_dtype, step.n_seqs, self.n_heads, self.n_kv, self.head_dim, sharing, self.window)
+
     def schedule(self, step) -> tuple:
         if step.mode != "decode":
             return ()
+        plan = self.shared_plan(step)
+        if plan is not None:
+            return ("shared",) + plan[:2]
         splits = self.decode_splits(step)
         blocks = splits * step.n_seqs * self.n_kv * ((self.n_heads // self.n_kv + 7) // 8)
         # the kernel's layout depends on the lengths at head size 256 and beyond one round of blocks
         return (splits, self._uneven(step)) if self.head_dim == 256 and blocks > self._resident else (splits,)
 
     def scratch_need(self, step) -> int:
-        """Partial (maximum, sum, output) of every key range: float32, [rows, heads, ranges, head_dim + 2]."""
+        """Partial (maximum, sum, output) of every key range: float32, [rows, heads, ranges, head_dim + 2]; where rows share pages, what
+        their plan says."""
         if step.mode != "decode":
             return 0
+        plan = self.shared_plan(step)
+        if plan is not None:
+            return plan.scratch_bytes
         return step.n_seqs * self.n_heads * self.decode_splits(step) * (self.head_dim + 2) * 4
 
     def input_matrix(self) -> torch.Tensor:
@@ -386,6 +400,10 @@ class AttentionMixer(Mixer):
             a = ops.attn_prefill(qkv, self.n_heads, self.n_kv, self.head_dim, step.tok_pos, step.tok_row0,
                                  self.scale, self.softcap, self.window, step.seq_row0, step.seq_len, step.max_q_len,
                                  slopes=self.slopes, sinks=self.sinks)
+        elif (plan := self.shared_plan(step)) is not None:
+            a = ops.attn_decode_shared(qkv, self.n_heads, self.n_kv, self.head_dim, line.k, line.v, line.page_table, line.page_size,
+                                       line.ring, step.slots, line.slot_len, step.sharing.by_group[line.group], self.scale, self.softcap,
+                                       self.window, plan, step.scratch, slopes=self.slopes, sinks=self.sinks)
         else:
             splits = self.decode_splits(step)
             n = step.n_seqs * self.n_heads * splits
