@@ -6,8 +6,8 @@
 //
 // Within a beam the order of the scores is that of the logits, so one pass over the logits is enough for everything but a few of them:
 //   1. a warp per segment of a row (SEGMENT logits) leaves the segment's maximum and sum of exp(z - maximum);
-//   2. a block per request joins them to log(sum exp) of every beam, turns the segments' maxima into scores, and finds a threshold that at
-//      least `take` segments reach.  As each of these holds a score that reaches it, so do the `take` best of all; they lie in the segments
+//   2. a block per request joins them to log(sum exp) of every beam, turns the segments' maxima into scores, and takes as a threshold the
+//      `take`-th largest of 256 groups' maxima, so that at least `take` segments reach it.  As each of these holds a score that reaches it, so do the `take` best of all; they lie in the segments
 //      that reach it, which are read again (a few KB) into a short list, whose best are found by counting.
 // Scores are formed in 64 bits: those of different beams may differ by less than 32 bits resolve after a sum over the vocabulary.
 // A logit that is not finite is no continuation and not in the sum (bit 0 of the error word says so); nor is any of a beam whose score is
@@ -23,36 +23,71 @@ namespace {
 constexpr int SELECT_MOST = 64;               // continuations per request, at most
 constexpr int SELECT_THREADS = 1024;
 constexpr int LIST = 2048;                    // places of the short list
+constexpr int MOST_REACHED = 512;             // segments that are looked at again
 
-// One maximum and sum per segment: warp w of the grid takes segment w of the row.
+// One maximum and sum per segment: warp w of the grid takes segments w, w + warps, ... of all rows, and asks for the next one's logits before it
+// works on those it has.  Whether all are finite is read off the maximum, the minimum and the sum; only where they are not does a
+// second look leave the others out.
 template <int SEGMENT>
-__global__ void __launch_bounds__(256)
-beam_segments_kernel(const float* __restrict__ logits, int V, int segments, float2* __restrict__ stats, int* __restrict__ error_flag) {
+__global__ void __launch_bounds__(256, 4)
+beam_segments_kernel(const float* __restrict__ logits, int V, int segments, int total, float2* __restrict__ stats, int* __restrict__ error_flag) {
+    constexpr int PER = SEGMENT / 32;
     pdl_wait();
-    const int seg = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, r = blockIdx.y;
-    if (seg >= segments) return;
-    const float* row = logits + (size_t)r * V;
-    float z[SEGMENT / 32];
-    float m = -CUDART_INF_F;
-    bool bad = false;
+    const int lane = threadIdx.x & 31, warps = gridDim.x * 8;
+    float ahead[PER];
+    auto ask = [&](int i) {
+        if (i >= total) return;
+        const int r = i / segments, v0 = (i - r * segments) * SEGMENT;
+        const float* p = logits + (size_t)r * V + v0 + lane;
+        if (v0 + SEGMENT <= V) {
 #pragma unroll
-    for (int i = 0; i < SEGMENT / 32; ++i) {
-        const int v = seg * SEGMENT + i * 32 + lane;
-        z[i] = v < V ? row[v] : -CUDART_INF_F;
-        if (v < V && !isfinite(z[i])) {
-            bad = true;
-            z[i] = -CUDART_INF_F;
+            for (int j = 0; j < PER; ++j) ahead[j] = p[j * 32];
+        } else {                                              // behind the row: its last logit again, taken out below
+#pragma unroll
+            for (int j = 0; j < PER; ++j) ahead[j] = p[min(j * 32, V - 1 - v0 - lane)];
         }
-        m = fmaxf(m, z[i]);
-    }
-    m = warp_max(m);
-    float s = 0.f;
-    if (m != -CUDART_INF_F)
+    };
+    int i = blockIdx.x * 8 + (threadIdx.x >> 5);
+    ask(i);
+    for (; i < total; i += warps) {
+        float z[PER];
 #pragma unroll
-        for (int i = 0; i < SEGMENT / 32; ++i) s += expf(z[i] - m);
-    s = warp_sum(s);
-    if (lane == 0) stats[(size_t)r * segments + seg] = make_float2(m, s);
-    if (error_flag != nullptr && __any_sync(0xffffffffu, bad) && lane == 0) atomicOr(error_flag, 1);
+        for (int j = 0; j < PER; ++j) z[j] = ahead[j];
+        ask(i + warps);
+        const int left = V - i % segments * SEGMENT;          // logits from the segment's first on
+        float m = -CUDART_INF_F, least = CUDART_INF_F;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            m = fmaxf(m, z[j]);
+            least = fminf(least, z[j]);
+        }
+        if (left < SEGMENT) {
+#pragma unroll
+            for (int j = 0; j < PER; ++j)
+                if (j * 32 + lane >= left) z[j] = -CUDART_INF_F;
+        }
+        m = warp_max(m);
+        float s = 0.f;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) s += expf(z[j] - m);
+        s = warp_sum(s);
+        if (__any_sync(0xffffffffu, least == -CUDART_INF_F) || !(s < CUDART_INF_F)) {      // (NaN, or an infinity in the maximum, make s a NaN)
+            m = -CUDART_INF_F;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                if (!isfinite(z[j])) z[j] = -CUDART_INF_F;
+                m = fmaxf(m, z[j]);
+            }
+            m = warp_max(m);
+            s = 0.f;
+            if (m != -CUDART_INF_F)
+#pragma unroll
+                for (int j = 0; j < PER; ++j) s += expf(z[j] - m);
+            s = warp_sum(s);
+            if (lane == 0 && error_flag != nullptr) atomicOr(error_flag, 1);
+        }
+        if (lane == 0) stats[i] = make_float2(m, s);
+    }
 }
 
 __device__ __forceinline__ double warp_sum(double v) {
@@ -86,60 +121,99 @@ beam_pick_kernel(const float* __restrict__ logits, int V, int beams, int take, i
     Found* found = reinterpret_cast<Found*>(smem);
     double* base = reinterpret_cast<double*>(found + 1);      // [beams] t_b - log(sum exp)
     unsigned* best = reinterpret_cast<unsigned*>(base + beams);   // [beams * segments] the segments' best scores, ordered
-    __shared__ int n_found, sum;
+    constexpr int WARPS = SELECT_THREADS / 32, GROUPS = 256;
+    __shared__ float part_m[WARPS];
+    __shared__ double part_s[WARPS];
+    __shared__ unsigned group_best[GROUPS], threshold_s;
+    __shared__ int reached[MOST_REACHED], n_reached, n_found;
     __shared__ double last_score;
     __shared__ unsigned last_at;
     const int q = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const size_t row0 = (size_t)q * beams;
-    if (threadIdx.x == 0) n_found = 0;
-    for (int b = warp; b < beams; b += SELECT_THREADS / 32) {
-        const float2* st = stats + (row0 + b) * segments;
+    if (threadIdx.x == 0) {
+        n_found = n_reached = 0;
+        threshold_s = 1u;                     // fewer groups than wanted: all that hold anything
+    }
+    // log(sum exp) of every beam, by as many warps as there are for each
+    const int share = beams >= WARPS ? 1 : WARPS / beams;
+    for (int b0 = 0; b0 < beams; b0 += WARPS / share) {
+        const int b = b0 + warp / share, p = warp % share;
+        const bool mine = warp / share < WARPS / share && b < beams;
+        const float2* st = stats + (row0 + (mine ? b : 0)) * segments;
         float m = -CUDART_INF_F;
-        for (int i = lane; i < segments; i += 32) m = fmaxf(m, st[i].x);
+        if (mine)
+#pragma unroll 4
+            for (int i = p * 32 + lane; i < segments; i += share * 32) m = fmaxf(m, st[i].x);
         m = qnn::warp_max(m);
+        if (lane == 0) part_m[warp] = m;
+        __syncthreads();
+        for (int i = 0; i < share; ++i) m = fmaxf(m, part_m[warp / share * share + i]);
         double s = 0.0;
-        for (int i = lane; i < segments; i += 32)
-            if (st[i].x != -CUDART_INF_F) s += (double)st[i].y * exp((double)st[i].x - (double)m);
+        if (mine && m != -CUDART_INF_F)
+#pragma unroll 4
+            for (int i = p * 32 + lane; i < segments; i += share * 32) s += (double)(st[i].y * expf(st[i].x - m));
         s = warp_sum(s);
-        const double t = (double)scores[row0 + b];
-        const bool alive = m != -CUDART_INF_F && t > -CUDART_INF && t < CUDART_INF;
-        const double add = alive ? t - (double)m - log(s) : -CUDART_INF;
-        if (lane == 0) base[b] = add;
-        for (int i = lane; i < segments; i += 32)
-            best[b * segments + i] = alive && st[i].x != -CUDART_INF_F ? ordered((float)(add + (double)st[i].x)) : 0u;    // 0: none
+        if (lane == 0) part_s[warp] = s;
+        __syncthreads();
+        if (mine) {
+            s = 0.0;
+            for (int i = 0; i < share; ++i) s += part_s[warp / share * share + i];
+            const double t = (double)scores[row0 + b];
+            const bool alive = m != -CUDART_INF_F && t > -CUDART_INF && t < CUDART_INF;
+            const double add = alive ? t - (double)m - log(s) : -CUDART_INF;
+            if (p == 0 && lane == 0) base[b] = add;
+            for (int i = p * 32 + lane; i < segments; i += share * 32) {
+                const float z = st[i].x;
+                best[b * segments + i] = alive && z != -CUDART_INF_F ? ordered((float)(add + (double)z)) : 0u;    // 0: none
+            }
+        }
+        __syncthreads();
+    }
+    // The threshold: segments in 256 groups, the `take`-th largest of the groups' maxima (found by counting).
+    const int n = beams * segments;
+    unsigned top = 0u;                        // (segment i is in group i % 256)
+    for (int i = (threadIdx.x >> 2) + (threadIdx.x & 3) * GROUPS; i < n; i += SELECT_THREADS) top = max(top, best[i]);
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    if ((threadIdx.x & 3) == 0) group_best[threadIdx.x >> 2] = top;
+    __syncthreads();
+    {
+        const int g = threadIdx.x >> 2;       // four threads a group, each counts a quarter
+        int rank = 0;
+#pragma unroll 16
+        for (int j = 0; j < GROUPS / 4; ++j) {
+            const int o = j * 4 + (threadIdx.x & 3);
+            const unsigned other = group_best[o];
+            rank += other > top || (other == top && o < g);
+        }
+        rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+        rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+        if (rank == take - 1 && (threadIdx.x & 3) == 0 && top > 1u) threshold_s = top;
     }
     __syncthreads();
-    // The threshold: the largest number that `take` segments reach or a little below (up to twice as many segments), bit by bit.
-    const int n = beams * segments;
-    unsigned threshold = 0u;
-    for (int bit = 31; bit >= 0; --bit) {
-        const unsigned tried = threshold | (1u << bit);
-        int mine = 0;
-        for (int i = threadIdx.x; i < n; i += SELECT_THREADS) mine += best[i] >= tried;
-        if (threadIdx.x == 0) sum = 0;
-        __syncthreads();
-        mine = __reduce_add_sync(0xffffffffu, mine);
-        if (lane == 0 && mine) atomicAdd(&sum, mine);
-        __syncthreads();
-        const int reach = sum;
-        __syncthreads();
-        if (reach >= take) {
-            threshold = tried;
-            if (reach <= 2 * take) break;
+    const unsigned threshold = threshold_s;
+    for (int i = threadIdx.x; i < n; i += SELECT_THREADS)
+        if (best[i] >= threshold) {
+            const int at = atomicAdd(&n_reached, 1);
+            if (at < MOST_REACHED) reached[at] = i;
         }
-    }
-    if (threshold == 0u) threshold = 1u;      // fewer segments than wanted: all that hold anything
-    for (int i = warp; i < n; i += SELECT_THREADS / 32) {
+    __syncthreads();
+    // (of more than the list holds every segment is looked at)
+    const int n_look = n_reached <= MOST_REACHED ? n_reached : n;
+    for (int l = warp; l < n_look; l += WARPS) {
+        const int i = n_reached <= MOST_REACHED ? reached[l] : l;
         if (best[i] < threshold) continue;
         const int b = i / segments, v0 = (i - b * segments) * SEGMENT;
         const float* row = logits + (row0 + b) * V;
+        const double add = base[b];
+        float z[SEGMENT / 32];
+#pragma unroll
+        for (int j = 0; j < SEGMENT / 32; ++j) z[j] = row[min(v0 + j * 32 + lane, V - 1)];
 #pragma unroll
         for (int j = 0; j < SEGMENT / 32; ++j) {
             const int v = v0 + j * 32 + lane;
-            if (v >= V) continue;
-            const float z = row[v];
-            if (!isfinite(z)) continue;
-            const double s = base[b] + (double)z;
+            if (v >= V || !isfinite(z[j])) continue;
+            const double s = add + (double)z[j];
             if (ordered((float)s) < threshold) continue;
             const int at = atomicAdd(&n_found, 1);
             if (at < LIST) {
@@ -154,12 +228,13 @@ beam_pick_kernel(const float* __restrict__ logits, int V, int beams, int take, i
     int* ob = out_beams + (size_t)q * take;
     int* ot = out_tokens + (size_t)q * take;
     if (have <= LIST) {
-        for (int i = threadIdx.x; i < have; i += SELECT_THREADS) {
+        for (int i = warp; i < have; i += WARPS) {
             const double s = found->score[i];
             const unsigned a = found->at[i];
             int rank = 0;
-            for (int j = 0; j < have; ++j) rank += before(found->score[j], found->at[j], s, a);
-            if (rank < take) {
+            for (int j = lane; j < have; j += 32) rank += before(found->score[j], found->at[j], s, a);
+            rank = __reduce_add_sync(0xffffffffu, rank);
+            if (rank < take && lane == 0) {
                 os[rank] = (float)s;
                 ob[rank] = (int)(a / (unsigned)V);
                 ot[rank] = (int)(a % (unsigned)V);
@@ -241,13 +316,16 @@ QNN_API int qnn_beam_select(const float* logits, const float* scores, int reques
     const int segments = qnn_beam_select_segments(V);
     const size_t smem = sizeof(Found) + (size_t)beams * sizeof(double) + (size_t)beams * segments * sizeof(unsigned);
     if (smem > 200 * 1024) return QNN_ERR_UNSUPPORTED;
-    const dim3 grid((segments + 7) / 8, requests * beams);
+    const long long total = (long long)requests * beams * segments;
+    if (total > 0x7fffffff) return QNN_ERR_UNSUPPORTED;
+    const int wave = device_sms() * 4;        // blocks of the first kernel at a time
+    const int blocks = (int)((total + 7) / 8 < wave ? (total + 7) / 8 : wave);
     float2* stats = (float2*)scratch;
 #define QNN_SELECT(SEG)                                                                                                                        \
     {                                                                                                                                          \
         static OncePerDevice asked;                                                                                                            \
         if (const int rc = allow_shared(asked, beam_pick_kernel<SEG>, 200 * 1024)) return rc;                                                  \
-        launch_pdl(beam_segments_kernel<SEG>, grid, dim3(256), 0, st, logits, V, segments, stats, error_flag);                                 \
+        launch_pdl(beam_segments_kernel<SEG>, dim3(blocks), dim3(256), 0, st, logits, V, segments, (int)total, stats, error_flag);                                 \
         launch_pdl(beam_pick_kernel<SEG>, dim3(requests), dim3(SELECT_THREADS), smem, st, logits, V, beams, take, segments, scores,             \
                    (const float2*)stats, out_scores, out_beams, out_tokens, status_in, error_flag);                                            \
     }
