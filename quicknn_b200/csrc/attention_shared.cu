@@ -12,14 +12,16 @@
 // (an Inf, a NaN) stays with the rows that see it.  The keys of [begin, end) outside C are among each row's own.
 //
 // Work is cut into items, a CTA each: (group, tile of query rows, range of C) and (row, tile of query heads, range of its own keys),
-// per kv head.  An item leaves (m, l, O) in scratch (m in units of log2), and a second kernel joins a row's items in ascending order:
+// per kv head; keys are walked in tiles of 16 positions.  An item leaves (m, l, O) in scratch (m in units of log2), and a second kernel joins a row's items in ascending order:
 // results depend on the numbers of ranges, not on what runs when.
 #include "attention_generic.cuh"
+#include "tcgen05.cuh"
 
 using namespace qnn;
 
 namespace {
 
+constexpr int TILE = 16;                      // positions
 constexpr float LOG2E = 1.4426950408889634f;
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -44,15 +46,17 @@ struct Cells {                                // where keys and values lie
     int window;
 };
 
-// What an item works on, the same in all threads of its CTA.
+// What an item works on, the same in all threads of its CTA: tiles t0 .. t1 - 1 of 16 positions each, the first `tiles_a` of the walk from
+// position a0 on, the others from b0 on (both multiples of 16; a row's own keys lie on both sides of C).  Positions outside lo .. hi - 1 that
+// a tile holds do not count.
 struct Item {
     int row0, rows;                           // its rows of the batch
     int slot;                                 // whose page table says where the keys are
     int part;                                 // which part of those rows
     int query0;                               // first query of the tile: query m is row row0 + m / G, head m % G of the kv head
-    int begin, end;                           // logical keys: key i stands at position first + i, from gap_at on gap further
-    int first, gap_at, gap;
-    __device__ __forceinline__ int position(int i) const { return first + i + (i >= gap_at ? gap : 0); }
+    int t0, t1;
+    int tiles_a, a0, b0, lo, hi;
+    __device__ __forceinline__ int position(int t) const { return t < tiles_a ? a0 + t * TILE : b0 + (t - tiles_a) * TILE; }
 };
 
 // The window's start and the length of a row (slot < 0: a row of no sequence, which sees nothing).
@@ -62,9 +66,11 @@ __device__ __forceinline__ int2 sees(const Cells& c, int slot) {
     return make_int2(c.window > 0 && n > c.window ? n - c.window : 0, n);
 }
 
-// C of a group, by one warp (every lane gets it), and the slot of its first row that belongs to a sequence.
+// C of a group, by one warp (every lane gets it), and the slot of its first row that belongs to a sequence.  Of what all rows see only
+// whole pages: no tile then holds a cell that nobody has written.
 __device__ int3 common_keys(const Cells& c, int4 g) {
     int lo = g.z, hi = g.w, slot = -1;
+#pragma unroll 4
     for (int i = threadIdx.x & 31; i < g.y; i += 32) {
         const int s = c.slots[g.x + i];
         if (s < 0) continue;
@@ -78,63 +84,64 @@ __device__ int3 common_keys(const Cells& c, int4 g) {
     const unsigned have = __ballot_sync(0xffffffffu, slot >= 0);
     if (have == 0) return make_int3(0, 0, -1);
     slot = __shfl_sync(0xffffffffu, slot, __ffs(have) - 1);
+    const int mask = (1 << c.page_shift) - 1;
+    lo = (lo + mask) & ~mask;
+    hi &= ~mask;
     return make_int3(lo, max(lo, hi), slot);
 }
 
-// Item x of the launch: common_tiles x S items of every group first, then own_tiles x P items of every row.  Every warp works it out.
-// `tile`: queries of an item.  Ranges are cut to whole multiples of 16 keys.
-__device__ Item item_of(const Shared& sh, const Cells& c, int x, int G, int tile) {
+__device__ __forceinline__ void take_range(Item& it, int tiles, int range, int ranges) {
+    const int per = (tiles + ranges - 1) / ranges;
+    it.t0 = min(range * per, tiles);
+    it.t1 = min(it.t0 + per, tiles);
+}
+
+// Range `range` of C of group `group` for the queries from tile `q_tile` on.  Every warp works it out.
+__device__ Item common_item(const Shared& sh, const Cells& c, int group, int q_tile, int range, int tile) {
     Item it;
-    const int common_items = sh.n_groups * sh.common_tiles * sh.common_ranges;
-    int ranges, range, keys;
-    if (x < common_items) {
-        ranges = sh.common_ranges;
-        range = x % ranges;
-        const int rest = x / ranges;
-        const int4 g = sh.groups[rest / sh.common_tiles];
-        it.query0 = rest % sh.common_tiles * tile;
-        it.row0 = g.x;
-        it.rows = g.y;
-        it.part = range;
-        const int3 k = common_keys(c, g);
-        it.slot = k.z;
-        it.first = k.x;
-        it.gap_at = 0x7fffffff;
-        it.gap = 0;
-        keys = k.y - k.x;
-    } else {
-        const int own_tiles = (G + tile - 1) / tile;
-        ranges = sh.own_ranges;
-        x -= common_items;
-        range = x % ranges;
-        const int rest = x / ranges;
-        it.query0 = rest % own_tiles * tile;
-        it.row0 = rest / own_tiles;
-        it.rows = 1;
-        it.part = sh.common_ranges + range;
-        it.slot = c.slots[it.row0];
-        const int g = sh.row_group[it.row0];
-        const int2 w = sees(c, it.slot);
-        it.first = w.x;
-        it.gap_at = 0x7fffffff;
-        it.gap = 0;
-        keys = w.y - w.x;
-        if (g >= 0 && it.slot >= 0) {
-            const int3 k = common_keys(c, sh.groups[g]);
-            it.gap_at = k.x - w.x;            // C lies inside what the row sees
-            it.gap = k.y - k.x;
-            keys -= it.gap;
+    const int4 g = sh.groups[group];
+    it.row0 = g.x;
+    it.rows = g.y;
+    it.query0 = q_tile * tile;
+    it.part = range;
+    const int3 k = common_keys(c, g);
+    it.slot = k.z;
+    it.tiles_a = 0;
+    it.a0 = it.b0 = it.lo = k.x;
+    it.hi = k.y;
+    take_range(it, (k.y - k.x) / TILE, range, sh.common_ranges);
+    return it;
+}
+
+// Range `range` of row `row`'s own keys.
+__device__ Item own_item(const Shared& sh, const Cells& c, int row, int q_tile, int range, int tile) {
+    Item it;
+    it.row0 = row;
+    it.rows = 1;
+    it.query0 = q_tile * tile;
+    it.part = sh.common_ranges + range;
+    it.slot = c.slots[row];
+    const int g = sh.row_group[row];
+    const int2 w = sees(c, it.slot);
+    it.lo = w.x;
+    it.hi = w.y;
+    it.a0 = w.x & ~(TILE - 1);
+    it.tiles_a = 0;
+    it.b0 = it.a0;
+    if (g >= 0 && it.slot >= 0) {
+        const int3 k = common_keys(c, sh.groups[g]);
+        if (k.y > k.x) {                      // C lies inside what the row sees, and starts and ends with pages
+            it.tiles_a = (k.x - it.a0) / TILE;
+            it.b0 = k.y;
         }
     }
-    const int per = ((keys + ranges - 1) / ranges + 15) & ~15;
-    it.begin = min(range * per, keys);
-    it.end = min(it.begin + per, keys);
+    take_range(it, it.tiles_a + max(0, it.hi - it.b0 + TILE - 1) / TILE, range, sh.own_ranges);
     return it;
 }
 
 // The page ids of an item's keys, pages from that of its first position on; returns the number of that page.
 __device__ __forceinline__ int load_pages(const Item& it, const Cells& c, int* pages) {
-    const int first = it.position(it.begin) >> c.page_shift, last = it.position(it.end - 1) >> c.page_shift;
+    const int first = it.position(it.t0) >> c.page_shift, last = it.position(it.t1 - 1) >> c.page_shift;
     const int* row = c.page_table + (size_t)it.slot * c.max_pages;
     for (int u = threadIdx.x; u <= last - first; u += blockDim.x) {
         const int p = first + u;
@@ -151,18 +158,14 @@ __device__ __forceinline__ size_t part_of(const Item& it, const Shared& sh, int 
 // ---- tensor cores, bfloat16 -------------------------------------------------------------------------------------------------
 // As in attention_decode_mma.cu the keys fill the 16-row side of mma.m16n8k16 and queries the 8-column side,
 //     S^T[16 keys x 8 q] = K Q^T,    O^T[hd x 8 q] += V^T P^T,
-// here with NT column tiles (8 NT queries) for every fragment of K and V that ldmatrix brings.  A warp walks its own tiles of 16 keys
-// (cp.async, a ring of STAGES), so nothing but the last merge is shared between the warps of a CTA.  P^T is the transpose of S^T's
-// accumulator, eight by eight (movmatrix).  The exponentials are taken against a reference that is raised only when a score
+// here with NT column tiles (8 NT queries) for every fragment of K and V that ldmatrix brings.  A warp walks its own tiles of 16 keys: one
+// lane asks the copy engine for them (a tile lies within a page; boxes of 64 elements x 16 positions, 128-byte swizzle, so that ldmatrix does
+// not conflict), STAGES deep, an mbarrier each.  Nothing but the last merge is shared between the warps of a CTA.  P^T is the transpose
+// of S^T's accumulator, eight by eight (movmatrix).  The exponentials are taken against a reference that is raised only when a score
 // exceeds it by more than 8 (in log2): the stale reference cancels in the division, P stays below 2^8.
-constexpr int TILE = 16;
 constexpr float REFERENCE_STEP = 8.f;
+constexpr int WARPS = 2, STAGES = 3;
 
-__device__ __forceinline__ void cp_async_16(unsigned dst, const void* src, bool valid) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0));   // 0 bytes: zeros
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::); }
-template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N)); }
 __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], unsigned addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
@@ -182,36 +185,44 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-    __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<uint32_t*>(&h);
-}
 
-constexpr int WARPS = 2, STAGES = 3;
+struct Scores {
+    float scale, cap;
+    const float* slopes;
+};
+
+// The walk of one item.  smem: the warps' rings, which the merge reuses, then the barriers, then the page ids.
+template <int HD>
+struct Layout {
+    static constexpr int TILE_BYTES = TILE * HD * 2, WARP_BYTES = STAGES * 2 * TILE_BYTES;
+    static __host__ __device__ constexpr int merge_bytes(int nt) { return WARPS * 8 * nt * (HD + 2) * 4; }
+    static __host__ __device__ constexpr int ring_bytes(int nt) { return WARPS * WARP_BYTES > merge_bytes(nt) ? WARPS * WARP_BYTES : (merge_bytes(nt) + 15) / 16 * 16; }
+    static constexpr int BARRIERS = WARPS * STAGES * 8;
+};
 
 template <int HD, int NT, bool BIAS>
-__global__ void __launch_bounds__(WARPS * 32)
-attn_shared_mma_kernel(const bf16* __restrict__ q, size_t q_stride, const bf16* __restrict__ k_pool, const bf16* __restrict__ v_pool,
-                       const Cells cells, const Shared sh, int nq, int nkv, float scale, float cap, float* __restrict__ part_o,
-                       float2* __restrict__ part_ml, const float* __restrict__ slopes) {
-    constexpr int KSTEPS = HD / 16, CH = HD / 8, ROW_BYTES = HD * 2, TILE_BYTES = TILE * ROW_BYTES, PER_LANE = TILE * CH / 32, QT = 8 * NT;
-    extern __shared__ __align__(128) unsigned char smem_raw[];
-    const int kh = blockIdx.y, G = nq / nkv;
+__device__ __forceinline__ void walk(const Item& it, int queries, const CUtensorMap& map_k, const CUtensorMap& map_v, const bf16* __restrict__ q, size_t q_stride,
+                                     const Cells& cells, const Shared& sh, int kh, int nq, int nkv, const Scores& sc, float* __restrict__ part_o,
+                                     float2* __restrict__ part_ml, int* __restrict__ status, unsigned char* smem, const int* pages, int first_page, unsigned bars) {
+    using L = Layout<HD>;
+    constexpr int KSTEPS = HD / 16, QT = 8 * NT;
+    const int G = nq / nkv;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    // slots, lengths, page tables and groups come from the host before the step: they are read before the wait for the kernel in front
-    const Item it = item_of(sh, cells, blockIdx.x, G, QT);
-    const int queries = min(QT, it.rows * G - it.query0);
-    const unsigned wbase = (unsigned)__cvta_generic_to_shared(smem_raw) + warp * STAGES * 2 * TILE_BYTES;
-    int* pages = reinterpret_cast<int*>(smem_raw + (size_t)WARPS * STAGES * 2 * TILE_BYTES);
-    int first_page = 0;
-    if (it.begin < it.end) first_page = load_pages(it, cells, pages);
-    pdl_wait();
-    if (queries <= 0) return;
-    if (it.begin >= it.end) {                                 // a range without keys
-        for (int m = threadIdx.x; m < queries; m += blockDim.x) part_ml[part_of(it, sh, it.query0 + m, kh, G, nq)] = make_float2(-CUDART_INF_F, 0.f);
-        return;
-    }
-    __syncthreads();
+    const unsigned ring = tc::smem_u32(smem) + warp * L::WARP_BYTES, bar0 = bars + warp * STAGES * 8;
+    const int my_tiles = it.t1 - it.t0 > warp ? (it.t1 - it.t0 - warp + WARPS - 1) / WARPS : 0;
+
+    const auto fetch = [&](int n) {                           // one lane
+        const int p = it.position(it.t0 + warp + n * WARPS), s = n % STAGES;
+        const int y = ((pages[(p >> cells.page_shift) - first_page] * nkv + kh) << cells.page_shift) + (p & ((1 << cells.page_shift) - 1));
+        const unsigned kst = ring + s * 2 * L::TILE_BYTES, bar = bar0 + s * 8;
+        tc::mbar_expect_tx(bar, 2 * L::TILE_BYTES);
+#pragma unroll
+        for (int d = 0; d < HD / 64; ++d) tc::tma_load_2d(kst + d * TILE * 128, &map_k, bar, d * 64, y);
+#pragma unroll
+        for (int d = 0; d < HD / 64; ++d) tc::tma_load_2d(kst + L::TILE_BYTES + d * TILE * 128, &map_v, bar, d * 64, y);
+    };
+    if (tc::elect_one())
+        for (int n = 0; n < STAGES && n < my_tiles; ++n) fetch(n);
 
     float o[NT][KSTEPS][4], m0[NT], m1[NT], l0[NT], l1[NT];   // queries 8 nt + 2t and 8 nt + 2t + 1
     uint32_t qf[NT][KSTEPS][2];                               // Q^T: query 8 nt + g, elements 16 ks + 2t, +1 and 16 ks + 8 + 2t, +1
@@ -238,7 +249,7 @@ attn_shared_mma_kernel(const bf16* __restrict__ q, size_t q_stride, const bf16* 
                 float sl = 0.f;
                 int nw = 0;
                 if (c < queries) {
-                    sl = slopes[kh * G + mm % G] * LOG2E;
+                    sl = sc.slopes[kh * G + mm % G] * LOG2E;
                     const int slot = cells.slots[it.row0 + mm / G];
                     nw = slot >= 0 ? cells.slot_len[slot] - 1 : 0;
                 }
@@ -247,68 +258,52 @@ attn_shared_mma_kernel(const bf16* __restrict__ q, size_t q_stride, const bf16* 
             }
         }
     }
-
-    const int first = it.begin + warp * TILE, stride = WARPS * TILE;
-    const int my_tiles = first < it.end ? (it.end - first + stride - 1) / stride : 0;
-    const int page_mask = (1 << cells.page_shift) - 1;
-    auto fetch = [&](int n) {
-        if (n < my_tiles) {
-            const int base = first + n * stride;
-            const unsigned kst = wbase + (n % STAGES) * 2 * TILE_BYTES, vst = kst + TILE_BYTES;
-#pragma unroll
-            for (int i = 0; i < PER_LANE; ++i) {
-                const int idx = i * 32 + lane, row = idx / CH, chunk = idx % CH;
-                const bool valid = base + row < it.end;
-                const int p = it.position(valid ? base + row : it.begin);
-                const size_t off = ((((size_t)pages[(p >> cells.page_shift) - first_page] * nkv + kh) << cells.page_shift) + (p & page_mask)) * HD + chunk * 8;
-                const unsigned dst = row * ROW_BYTES + ((chunk ^ (row & 7)) << 4);
-                cp_async_16(kst + dst, k_pool + off, valid);
-                cp_async_16(vst + dst, v_pool + off, valid);
-            }
-        }
-        cp_async_commit();                                    // an empty group keeps the count uniform
-    };
-#pragma unroll
-    for (int n = 0; n < STAGES - 1; ++n) fetch(n);
-
-    const float k1 = cap > 0.f ? scale / cap : scale * LOG2E, k2 = cap * LOG2E;
+    const float k1 = sc.cap > 0.f ? sc.scale / sc.cap : sc.scale * LOG2E, k2 = sc.cap * LOG2E;
     for (int n = 0; n < my_tiles; ++n) {
-        fetch(n + STAGES - 1);
-        cp_async_wait<STAGES - 1>();
-        __syncwarp();
-        const int base = first + n * stride;
-        const unsigned kst = wbase + (n % STAGES) * 2 * TILE_BYTES, vst = kst + TILE_BYTES;
-        float s[NT][4];
+        const int s_at = n % STAGES;
+        if (!tc::mbar_wait_warp(bar0 + s_at * 8, (n / STAGES) & 1)) {
+            if (lane == 0) atomicOr(status, 512);
+            // what else was asked for: wait for it, within the limit, before the memory is used again
+            for (int i = n; i < my_tiles && i < n + STAGES; ++i) (void)tc::mbar_wait_warp(bar0 + (i % STAGES) * 8, (i / STAGES) & 1);
+            break;
+        }
+        const int base = it.position(it.t0 + warp + n * WARPS);
+        const unsigned kst = ring + s_at * 2 * L::TILE_BYTES, vst = kst + L::TILE_BYTES;
+        const bool v_lo = base + g >= it.lo && base + g < it.hi, v_hi = base + g + 8 >= it.lo && base + g + 8 < it.hi;
+        if (base < it.lo || base + TILE > it.hi) {
+            // positions that do not count: their weights are zero, but zero times what an unused cell holds need not be
+            unsigned char* v = smem + (vst - tc::smem_u32(smem));
+            for (int i = lane; i < TILE * HD / 8; i += 32) {
+                const int r = i / 8 % TILE;                   // 16-byte piece i: block i / (8 TILE), row, piece of the row
+                if (base + r < it.lo || base + r >= it.hi) *reinterpret_cast<uint4*>(v + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // before the copy engine writes here again
+            __syncwarp();
+        }
+        float s[NT][4], s2[NT][4];                            // two chains of products
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[nt][j] = 0.f;
+            for (int j = 0; j < 4; ++j) s[nt][j] = s2[nt][j] = 0.f;
         {
             const int row = lane & 15, half = lane >> 4;
 #pragma unroll
             for (int ks = 0; ks < KSTEPS; ++ks) {
                 uint32_t a[4];
-                ldmatrix_x4(a, kst + row * ROW_BYTES + (((ks * 2 + half) ^ (row & 7)) << 4));
+                ldmatrix_x4(a, kst + (ks / 4) * (TILE * 128) + row * 128 + ((((ks % 4) * 2 + half) ^ (row & 7)) << 4));
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-                    if (nt == 0 || nt * 8 < queries) mma_16816(s[nt], a, qf[nt][ks][0], qf[nt][ks][1]);
+                for (int nt = 0; nt < NT; ++nt) mma_16816(ks % 2 ? s2[nt] : s[nt], a, qf[nt][ks][0], qf[nt][ks][1]);
             }
         }
         // s[nt][0], [1]: key base + g, queries 2t, 2t + 1; [2], [3]: key base + g + 8
-        const bool v_lo = base + g < it.end, v_hi = base + g + 8 < it.end;
-        int p_lo = 0, p_hi = 0;
-        if (BIAS) {
-            p_lo = it.position(base + g);
-            p_hi = it.position(base + g + 8);
-        }
         bool above = false;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                float x = s[nt][j] * k1;
-                if (cap > 0.f) x = k2 * tanh_approx(x);
-                if (BIAS) x -= ((j & 1) ? slope1[nt] : slope0[nt]) * (float)(((j & 1) ? newest1[nt] : newest0[nt]) - ((j < 2) ? p_lo : p_hi));
+                float x = (s[nt][j] + s2[nt][j]) * k1;
+                if (sc.cap > 0.f) x = k2 * tanh_approx(x);
+                if (BIAS) x -= ((j & 1) ? slope1[nt] : slope0[nt]) * (float)(((j & 1) ? newest1[nt] : newest0[nt]) - (base + g + (j < 2 ? 0 : 8)));
                 s[nt][j] = ((j < 2) ? v_lo : v_hi) ? x : -CUDART_INF_F;
             }
             above |= fmaxf(s[nt][0], s[nt][2]) > m0[nt] + REFERENCE_STEP || fmaxf(s[nt][1], s[nt][3]) > m1[nt] + REFERENCE_STEP;
@@ -324,7 +319,7 @@ attn_shared_mma_kernel(const bf16* __restrict__ q, size_t q_stride, const bf16* 
                 }
                 x0 = fmaxf(m0[nt], x0);
                 x1 = fmaxf(m1[nt], x1);
-                // -inf only before the first key (every tile has one; a score of -inf counts as no key)
+                // -inf only before the first key (a score of -inf counts as no key)
                 const float c0 = m0[nt] == -CUDART_INF_F ? 0.f : exp2_fast(m0[nt] - x0), c1 = m1[nt] == -CUDART_INF_F ? 0.f : exp2_fast(m1[nt] - x1);
                 m0[nt] = x0;
                 m1[nt] = x1;
@@ -346,26 +341,25 @@ attn_shared_mma_kernel(const bf16* __restrict__ q, size_t q_stride, const bf16* 
             const float a0 = exp2_fast(s[nt][0] - r0), a1 = exp2_fast(s[nt][1] - r1), a2 = exp2_fast(s[nt][2] - r0), a3 = exp2_fast(s[nt][3] - r1);
             l0[nt] += a0 + a2;
             l1[nt] += a1 + a3;
-            pb[nt][0] = transposed_8x8(pack_bf16(a0, a1));
-            pb[nt][1] = transposed_8x8(pack_bf16(a2, a3));
+            pb[nt][0] = transposed_8x8(tc::pack_bf16(a0, a1));
+            pb[nt][1] = transposed_8x8(tc::pack_bf16(a2, a3));
         }
         {
             const int row = (lane & 7) + ((lane >> 4) << 3), sub = (lane >> 3) & 1;
 #pragma unroll
             for (int mt = 0; mt < KSTEPS; ++mt) {
                 uint32_t a[4];
-                ldmatrix_x4_trans(a, vst + row * ROW_BYTES + (((mt * 2 + sub) ^ (row & 7)) << 4));
+                ldmatrix_x4_trans(a, vst + (mt / 4) * (TILE * 128) + row * 128 + ((((mt % 4) * 2 + sub) ^ (row & 7)) << 4));
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-                    if (nt == 0 || nt * 8 < queries) mma_16816(o[nt][mt], a, pb[nt][0], pb[nt][1]);
+                for (int nt = 0; nt < NT; ++nt) mma_16816(o[nt][mt], a, pb[nt][0], pb[nt][1]);
             }
         }
-        __syncwarp();                                         // the stage may be refilled
+        __syncwarp();                                         // everybody has read the stage: it may be filled again
+        if (n + STAGES < my_tiles && tc::elect_one()) fetch(n + STAGES);
     }
-    cp_async_wait<0>();
     __syncthreads();
     // the warps' states through shared memory, [warp][query][HD + 2], joined in warp order
-    float* ms = reinterpret_cast<float*>(smem_raw);
+    float* ms = reinterpret_cast<float*>(smem);
     constexpr int ROW = HD + 2;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -392,25 +386,74 @@ attn_shared_mma_kernel(const bf16* __restrict__ q, size_t q_stride, const bf16* 
         }
     }
     __syncthreads();
-    for (int m = 0; m < queries; ++m) {
+    for (int m = warp; m < queries; m += WARPS) {             // a warp per query
         float mm = -CUDART_INF_F, coef[WARPS], ll = 0.f;
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) mm = fmaxf(mm, ms[((size_t)w * QT + m) * ROW + HD]);
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
-            const float mw = ms[((size_t)w * QT + m) * ROW + HD];
-            coef[w] = mw == -CUDART_INF_F ? 0.f : exp2_fast(mw - mm);
-            ll += coef[w] * ms[((size_t)w * QT + m) * ROW + HD + 1];
+            const float mw = ms[((size_t)w * QT + m) * ROW + HD], lw = ms[((size_t)w * QT + m) * ROW + HD + 1];
+            coef[w] = mw == -CUDART_INF_F ? (lw != lw ? lw : 0.f) : exp2_fast(mw - mm);
+            ll += coef[w] * lw;
         }
         const size_t at = part_of(it, sh, it.query0 + m, kh, G, nq);
-        for (int d = threadIdx.x; d < HD; d += blockDim.x) {
-            float acc = 0.f;
 #pragma unroll
-            for (int w = 0; w < WARPS; ++w) acc += coef[w] * ms[((size_t)w * QT + m) * ROW + d];
-            part_o[at * HD + d] = acc;
+        for (int d = lane * 2; d < HD; d += 64) {
+            float2 acc = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                const float2 v = *reinterpret_cast<const float2*>(ms + ((size_t)w * QT + m) * ROW + d);
+                acc.x += coef[w] * v.x;
+                acc.y += coef[w] * v.y;
+            }
+            *reinterpret_cast<float2*>(part_o + at * HD + d) = acc;
         }
-        if (threadIdx.x == 0) part_ml[at] = make_float2(mm, ll);
+        if (lane == 0) part_ml[at] = make_float2(mm, ll);
     }
+}
+
+// Items: those of C first (group, tile of queries, range; the range fastest), then the rows' own (row, tile of heads, range).  NT: column tiles
+// of an item of C; a row's own heads take one where they fit it.
+template <int HD, int NT, bool BIAS>
+__global__ void __launch_bounds__(WARPS * 32)
+attn_shared_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const bf16* __restrict__ q, size_t q_stride,
+                       const Cells cells, const Shared sh, int common_items, int own_tile, int nq, int nkv, const Scores sc, float* __restrict__ part_o,
+                       float2* __restrict__ part_ml, int* __restrict__ status) {
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    const unsigned bars = tc::smem_u32(smem) + Layout<HD>::ring_bytes(NT);
+    int* pages = reinterpret_cast<int*>(smem + Layout<HD>::ring_bytes(NT) + Layout<HD>::BARRIERS);
+    const int kh = blockIdx.y, G = nq / nkv;
+    const bool own = (int)blockIdx.x >= common_items;
+    if (threadIdx.x < WARPS * STAGES) tc::mbar_init(bars + threadIdx.x * 8, 1);
+    // slots, lengths, page tables and groups come from the host before the step: they are read before the wait for the kernel in front
+    Item it;
+    int tile;
+    if (own) {
+        const int own_tiles = (G + own_tile - 1) / own_tile, x = (int)blockIdx.x - common_items, rest = x / sh.own_ranges;
+        tile = own_tile;
+        it = own_item(sh, cells, rest / own_tiles, rest % own_tiles, x % sh.own_ranges, own_tile);
+    } else {
+        const int rest = blockIdx.x / sh.common_ranges;
+        tile = 8 * NT;
+        it = common_item(sh, cells, rest / sh.common_tiles, rest % sh.common_tiles, blockIdx.x % sh.common_ranges, 8 * NT);
+    }
+    const int queries = min(tile, it.rows * G - it.query0);
+    int first_page = 0;
+    if (it.t0 < it.t1) first_page = load_pages(it, cells, pages);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();
+    pdl_wait();
+    if (queries <= 0) return;
+    if (it.t0 >= it.t1) {                                     // a range without keys
+        for (int m = threadIdx.x; m < queries; m += blockDim.x) part_ml[part_of(it, sh, it.query0 + m, kh, G, nq)] = make_float2(-CUDART_INF_F, 0.f);
+        return;
+    }
+    if (NT > 1 && own && own_tile == 8)
+        walk<HD, 1, BIAS>(it, queries, map_k, map_v, q, q_stride, cells, sh, kh, nq, nkv, sc, part_o, part_ml, status, smem, pages, first_page, bars);
+    else
+        walk<HD, NT, BIAS>(it, queries, map_k, map_v, q, q_stride, cells, sh, kh, nq, nkv, sc, part_o, part_ml, status, smem, pages, first_page, bars);
 }
 
 // ---- any head size, float32 or bfloat16 ----------------------------------------------------------------------------------------
@@ -427,7 +470,15 @@ attn_shared_generic_kernel(const T* __restrict__ q, size_t q_stride, const T* __
     extern __shared__ __align__(16) float sm[];
     const int kh = blockIdx.y, G = nq / nkv;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const Item it = item_of(sh, cells, blockIdx.x, G, GEN_QT);
+    const int common_items = sh.n_groups * sh.common_tiles * sh.common_ranges;
+    Item it;
+    if ((int)blockIdx.x < common_items) {
+        const int rest = blockIdx.x / sh.common_ranges;
+        it = common_item(sh, cells, rest / sh.common_tiles, rest % sh.common_tiles, blockIdx.x % sh.common_ranges, GEN_QT);
+    } else {
+        const int own_tiles = (G + GEN_QT - 1) / GEN_QT, x = (int)blockIdx.x - common_items, rest = x / sh.own_ranges;
+        it = own_item(sh, cells, rest / own_tiles, rest % own_tiles, x % sh.own_ranges, GEN_QT);
+    }
     const int queries = min(GEN_QT, it.rows * G - it.query0);
     pdl_wait();
     if (queries <= 0) return;
@@ -457,12 +508,17 @@ attn_shared_generic_kernel(const T* __restrict__ q, size_t q_stride, const T* __
         for (int d = 0; d < DPL; ++d) o[i][d] = 0.f;
     }
     const int chunks = hd / VEC, page_mask = (1 << cells.page_shift) - 1;
-    for (int base = it.begin; base < it.end; base += tile_keys) {
-        const int n = min(tile_keys, it.end - base);
-        __syncthreads();                                      // the tile before has been read
+    for (int t = it.t0; t < it.t1; t += tile_keys / TILE) {
+        const int n = min(tile_keys, (it.t1 - t) * TILE);
+        __syncthreads();                                      // the tiles before have been read
         const int* table = cells.page_table + (size_t)it.slot * cells.max_pages;
         for (int i = threadIdx.x; i < n * chunks; i += blockDim.x) {
-            const int j = i / chunks, c = i % chunks, p = it.position(base + j);
+            const int j = i / chunks, c = i % chunks, p = it.position(t + j / TILE) + j % TILE;
+            if (p < it.lo || p >= it.hi) {                    // zero weights, and zeros for them to meet
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) sv[j * pitch + c * VEC + e] = 0.f;
+                continue;
+            }
             const int pn = p >> cells.page_shift, page = table[cells.ring_pages > 0 ? pn % cells.ring_pages : pn];
             const size_t off = ((((size_t)page * nkv + kh) << cells.page_shift) + (p & page_mask)) * hd + c * VEC;
             Vec16<T> kv, vv;
@@ -478,8 +534,8 @@ attn_shared_generic_kernel(const T* __restrict__ q, size_t q_stride, const T* __
             }
         }
         __syncthreads();
-        const bool valid = lane < n;
-        const int pos = valid ? it.position(base + lane) : 0;
+        const int pos = lane < n ? it.position(t + lane / TILE) + lane % TILE : 0;
+        const bool valid = lane < n && pos >= it.lo && pos < it.hi;
 #pragma unroll
         for (int i = 0; i < GEN_Q; ++i) {
             const int m = warp * GEN_Q + i;
@@ -520,61 +576,108 @@ attn_shared_generic_kernel(const T* __restrict__ q, size_t q_stride, const T* __
 }
 
 // ---- the parts of a row joined ---------------------------------------------------------------------------------------------------
-// A block per (row, head): threads in groups of hd / 4, group g adds parts g, g + groups, ...; the groups' sums in ascending order.  Parts
-// without keys (l = 0) are not read.
-template <typename T>
-__global__ void attn_shared_join_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml, T* __restrict__ out, size_t out_stride,
-                                        int nq, int hd, int S, int P, const int* __restrict__ row_group, const int* __restrict__ slots,
-                                        const float* __restrict__ sinks) {
-    pdl_wait();
-    extern __shared__ __align__(16) float js[];               // [groups][hd], then the parts' weights
-    const int row = blockIdx.x / nq, h = blockIdx.x % nq, parts = S + P;
-    const int lpg = hd / 4, groups = blockDim.x / lpg;
-    float* weight = js + (size_t)groups * hd;
-    float* inverse = weight + parts;
+// A warp per (row, head), or JOIN_WARPS of them where a row has many parts: warp i adds parts i, i + warps, ...; the warps' sums in ascending
+// order.  Weights are in the lanes' registers (part p: lane p % 32), the first parts are asked for before the weights are known.  Of parts
+// without keys (l = 0) nothing counts.
+constexpr int JOIN_WARPS = 8, MOST_PARTS = 128;
+
+template <typename T, int PIECES>                             // pieces of 128 elements that a head has, at most
+__global__ void __launch_bounds__(JOIN_WARPS * 32)
+attn_shared_join_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml, T* __restrict__ out, size_t out_stride, int outputs, int nq,
+                        int hd, int S, int P, int warps, const int* __restrict__ row_group, const int* __restrict__ slots, const float* __restrict__ sinks) {
+    extern __shared__ __align__(16) float js[];               // [warps][hd] where several warps share an output
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, parts = S + P;
+    const int i = blockIdx.x * (JOIN_WARPS / warps) + warp / warps, wi = warp % warps;
+    const bool mine = i < outputs;
+    const int row = mine ? i / nq : 0, h = mine ? i % nq : 0;
     const int from = row_group[row] >= 0 && slots[row] >= 0 ? 0 : S;      // a row of no group or no sequence has no part in C
-    const size_t at = (size_t)blockIdx.x * parts;
-    if (threadIdx.x < 32) {
-        float M = -CUDART_INF_F;
-        for (int p = from + threadIdx.x; p < parts; p += 32) {
-            const float2 ml = part_ml[at + p];
-            if (ml.y != 0.f) M = fmaxf(M, ml.x);
-        }
-        M = warp_max(M);
-        float sum = 0.f;
-        for (int p = from + threadIdx.x; p < parts; p += 32) {
-            const float2 ml = part_ml[at + p];
-            const float w = ml.y != ml.y ? ml.y : (ml.y != 0.f ? exp2f(ml.x - M) : 0.f);      // a NaN among the scores has to come out
-            weight[p] = w;
-            sum += w != 0.f ? w * ml.y : 0.f;
-        }
-        sum = warp_sum(sum);
-        if (threadIdx.x == 0) {
-            const float all = sinks != nullptr ? sum + exp2f(sinks[h] * LOG2E - M) : sum;
-            *inverse = sum != 0.f ? 1.f / all : 0.f;
-        }
+    pdl_wait();
+    const size_t at = (size_t)(mine ? i : 0) * parts;
+    float2 ml[MOST_PARTS / 32];
+#pragma unroll
+    for (int k = 0; k < MOST_PARTS / 32; ++k) {
+        const int p = k * 32 + lane;
+        ml[k] = p >= from && p < parts ? part_ml[at + p] : make_float2(-CUDART_INF_F, 0.f);
     }
-    __syncthreads();
-    const int g = threadIdx.x / lpg, c = (threadIdx.x % lpg) * 4;
-    if (g < groups) {
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int p = from + g; p < parts; p += groups) {
-            const float w = weight[p];
-            if (w == 0.f) continue;
-            const float4 v = *reinterpret_cast<const float4*>(part_o + (at + p) * hd + c);
-            acc.x += w * v.x;
-            acc.y += w * v.y;
-            acc.z += w * v.z;
-            acc.w += w * v.w;
+    constexpr int AHEAD = 4;
+    float4 v[AHEAD][PIECES];
+    const auto ask = [&](int p0) {
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            const int p = p0 + j * warps;
+#pragma unroll
+            for (int k = 0; k < PIECES; ++k) {
+                const int c = k * 128 + lane * 4;
+                v[j][k] = p < parts && c < hd ? *reinterpret_cast<const float4*>(part_o + (at + p) * hd + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
         }
-        *reinterpret_cast<float4*>(js + (size_t)g * hd + c) = acc;
+    };
+    ask(from + wi);
+    float M = -CUDART_INF_F, sum = 0.f, w[MOST_PARTS / 32];
+#pragma unroll
+    for (int k = 0; k < MOST_PARTS / 32; ++k)
+        if (ml[k].y != 0.f) M = fmaxf(M, ml[k].x);
+    M = warp_max(M);
+#pragma unroll
+    for (int k = 0; k < MOST_PARTS / 32; ++k) {
+        w[k] = ml[k].y != ml[k].y ? ml[k].y : (ml[k].y != 0.f ? exp2f(ml[k].x - M) : 0.f);       // a NaN among the scores has to come out
+        sum += w[k] != 0.f ? w[k] * ml[k].y : 0.f;
     }
-    __syncthreads();
-    const float inv = *inverse;
-    for (int d = threadIdx.x; d < hd; d += blockDim.x) {
-        float acc = 0.f;
-        for (int i = 0; i < groups; ++i) acc += js[(size_t)i * hd + d];
-        out[(size_t)row * out_stride + (size_t)h * hd + d] = from_f<T>(acc * inv);
+    sum = warp_sum(sum);
+    const float all = sinks != nullptr ? sum + exp2f(sinks[h] * LOG2E - M) : sum;
+    const float inverse = sum != 0.f ? 1.f / all : 0.f;
+    float4 acc[PIECES];
+#pragma unroll
+    for (int k = 0; k < PIECES; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p0 = from + wi; p0 < parts; p0 += AHEAD * warps) {
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            const int p = p0 + j * warps;
+            float mine_w = 0.f;
+#pragma unroll
+            for (int k = 0; k < MOST_PARTS / 32; ++k) {
+                const float x = __shfl_sync(0xffffffffu, w[k], p & 31);
+                if (p >> 5 == k) mine_w = x;
+            }
+            if (mine_w != 0.f)
+#pragma unroll
+                for (int k = 0; k < PIECES; ++k) {
+                    acc[k].x += mine_w * v[j][k].x;
+                    acc[k].y += mine_w * v[j][k].y;
+                    acc[k].z += mine_w * v[j][k].z;
+                    acc[k].w += mine_w * v[j][k].w;
+                }
+        }
+        if (p0 + AHEAD * warps < parts) ask(p0 + AHEAD * warps);
+    }
+    if (warps > 1) {
+        float* mine_s = js + (size_t)warp * hd;
+#pragma unroll
+        for (int k = 0; k < PIECES; ++k) {
+            const int c = k * 128 + lane * 4;
+            if (c < hd) *reinterpret_cast<float4*>(mine_s + c) = acc[k];
+        }
+        __syncthreads();
+        if (mine)
+            for (int d = wi * 32 + lane; d < hd; d += warps * 32) {
+                float a = 0.f;
+                for (int x = 0; x < warps; ++x) a += js[(size_t)(warp / warps * warps + x) * hd + d];
+                out[(size_t)row * out_stride + (size_t)h * hd + d] = from_f<T>(a * inverse);
+            }
+        return;
+    }
+    if (!mine) return;
+#pragma unroll
+    for (int k = 0; k < PIECES; ++k) {
+        const int c = k * 128 + lane * 4;
+        if (c >= hd) continue;
+        T* dst = out + (size_t)row * out_stride + (size_t)h * hd + c;
+        const float r[4] = {acc[k].x * inverse, acc[k].y * inverse, acc[k].z * inverse, acc[k].w * inverse};
+        if constexpr (sizeof(T) == 2) {
+            *reinterpret_cast<uint2*>(dst) = make_uint2(tc::pack_bf16(r[0], r[1]), tc::pack_bf16(r[2], r[3]));
+        } else {
+            *reinterpret_cast<float4*>(dst) = make_float4(r[0], r[1], r[2], r[3]);
+        }
     }
 }
 
@@ -585,17 +688,21 @@ bool on_tensor_cores(int dtype, int hd) { return dtype == QNN_DT_BF16 && (hd == 
 int column_tiles(int hd, int queries) { return queries <= 8 ? 1 : (queries <= 16 || hd > 128 ? 2 : 4); }
 
 template <int HD, int NT, bool BIAS>
-int launch_mma(const void* q, long long q_stride, const void* k_pool, const void* v_pool, const Cells& cells, const Shared& sh, int items, int nq,
-               int nkv, float scale, float cap, float* part_o, float2* part_ml, const float* slopes, cudaStream_t st) {
-    size_t smem = (size_t)WARPS * STAGES * 2 * TILE * HD * 2 + ((size_t)cells.max_pages + 2) * sizeof(int);
-    const size_t merge = (size_t)WARPS * 8 * NT * (HD + 2) * sizeof(float);
-    if (smem < merge) smem = merge;
+int launch_mma(const void* q, long long q_stride, const void* k_pool, const void* v_pool, long long pool_rows, const Cells& cells, const Shared& sh,
+               int B, int nq, int nkv, const Scores& sc, float* part_o, float2* part_ml, int* status, cudaStream_t st) {
+    const int G = nq / nkv, own_tile = G <= 8 ? 8 : 8 * NT;
+    const long long common = (long long)sh.n_groups * sh.common_tiles * sh.common_ranges, own = (long long)B * ((G + own_tile - 1) / own_tile) * sh.own_ranges;
+    if (common + own > 0x7fffffff) return QNN_ERR_UNSUPPORTED;
+    const size_t smem = 1024 + Layout<HD>::ring_bytes(NT) + Layout<HD>::BARRIERS + ((size_t)cells.max_pages + 2) * sizeof(int);
     if (smem > 220 * 1024) return QNN_ERR_UNSUPPORTED;
+    CUtensorMap map_k, map_v;
+    if (const int rc = tc::make_map_bf16(&map_k, k_pool, pool_rows, HD, TILE)) return rc;
+    if (const int rc = tc::make_map_bf16(&map_v, v_pool, pool_rows, HD, TILE)) return rc;
     auto kern = attn_shared_mma_kernel<HD, NT, BIAS>;
     static OncePerDevice asked;
     if (const int rc = allow_shared(asked, kern, 220 * 1024)) return rc;
-    launch_pdl(kern, dim3(items, nkv), dim3(WARPS * 32), smem, st, (const bf16*)q, (size_t)q_stride, (const bf16*)k_pool, (const bf16*)v_pool, cells,
-               sh, nq, nkv, scale, cap, part_o, part_ml, slopes);
+    launch_pdl(kern, dim3((unsigned)(common + own), nkv), dim3(WARPS * 32), smem, st, map_k, map_v, (const bf16*)q, (size_t)q_stride, cells, sh, (int)common,
+               own_tile, nq, nkv, sc, part_o, part_ml, status);
     return (int)cudaGetLastError();
 }
 
@@ -615,16 +722,16 @@ int launch_generic(const void* q, long long q_stride, const void* k_pool, const 
 template <typename T>
 int launch_join(const float* part_o, const float2* part_ml, void* out, long long out_stride, int B, int nq, int hd, int S, int P, const int* row_group,
                 const int* slots, const float* sinks, cudaStream_t st) {
-    const int lpg = hd / 4;
-    int groups = 256 / lpg;
-    if (groups > S + P) groups = S + P;
-    if (groups < 1) groups = 1;
-    int threads = groups * lpg;
-    if (threads < 32) threads = 32;
-    groups = threads / lpg;                                   // as the kernel counts them
-    const size_t smem = ((size_t)groups * hd + S + P + 1) * sizeof(float);
-    launch_pdl(attn_shared_join_kernel<T>, dim3((unsigned)(B * nq)), dim3(threads), smem, st, part_o, part_ml, (T*)out, (size_t)out_stride, nq, hd, S, P,
-               row_group, slots, sinks);
+    const int outputs = B * nq, warps = S + P <= 8 ? 1 : JOIN_WARPS, per = JOIN_WARPS / warps;
+    const size_t smem = warps > 1 ? (size_t)JOIN_WARPS * hd * sizeof(float) : 0;
+    const dim3 grid((outputs + per - 1) / per);
+#define QNN_JOIN(PIECES)                                                                                                                         \
+    launch_pdl(attn_shared_join_kernel<T, PIECES>, grid, dim3(JOIN_WARPS * 32), smem, st, part_o, part_ml, (T*)out, (size_t)out_stride, outputs, nq, hd, S, P, \
+               warps, row_group, slots, sinks)
+    if (hd <= 128) QNN_JOIN(1);
+    else if (hd <= 256) QNN_JOIN(2);
+    else QNN_JOIN(8);
+#undef QNN_JOIN
     return (int)cudaGetLastError();
 }
 
@@ -641,28 +748,33 @@ QNN_API int qnn_attn_shared_tile(int dtype, int hd, int queries) {
 // groups: [n_groups][4] (first row, rows, begin, end): positions begin .. end - 1 lie in the same pages in all the group's rows, as far as a row
 // still holds them; row_group: [B], a row's group or -1.  `most_rows`: rows of the largest group.  common_ranges / own_ranges: into how many ranges
 // a group's common keys and a row's own keys are cut.  Scratch: part_o B * nq * (common_ranges + own_ranges) * hd floats, part_ml twice as many
-// without hd; 16-byte aligned.  page_size: a power of two of at least 16; ring: a multiple of it, or 0.  slots, slot_len, page_table, groups and
+// without hd; 16-byte aligned.  pool_pages: pages of
+// the pools; status: as in qnn_gemm_tcgen05 (bit 512: keys or values did not arrive).  page_size: a power of two of at least 16; ring: a multiple of it, or 0.  slots, slot_len, page_table, groups and
 // row_group are read before the kernel waits for the one launched in front of it on the stream: that one must not write them.
 QNN_API int qnn_attn_decode_shared(const void* q, long long q_stride, int dtype, const void* k_pool, const void* v_pool, const int* page_table,
                                    int max_pages, int page_size, int ring, const int* slots, const int* slot_len, int B, const int* groups,
                                    int n_groups, int most_rows, const int* row_group, int nq, int nkv, int hd, float scale, float cap, int window,
                                    int common_ranges, int own_ranges, float* part_o, float* part_ml, void* out, long long out_stride,
-                                   const float* slopes, const float* sinks, cudaStream_t st) {
+                                   const float* slopes, const float* sinks, long long pool_pages, int* status, cudaStream_t st) {
     if (B <= 0) return 0;
-    if (nkv <= 0 || nkv > 65535 || nq <= 0 || nq % nkv || n_groups < 0 || most_rows < 0 || common_ranges < 1 || own_ranges < 1) return QNN_ERR_ARGUMENT;
+    if (nkv <= 0 || nkv > 65535 || nq <= 0 || nq % nkv || n_groups < 0 || most_rows < 0 || common_ranges < 1 || own_ranges < 1 ||
+        common_ranges + own_ranges > MOST_PARTS)
+        return QNN_ERR_ARGUMENT;
     if (page_size < 16 || (page_size & (page_size - 1)) || ring < 0 || ring % page_size) return QNN_ERR_ARGUMENT;
     if (ring > 0 && (window <= 0 || window > ring || ring / page_size > max_pages)) return QNN_ERR_ARGUMENT;   // a ring holds no more
     const int G = nq / nkv, esize = dtype == QNN_DT_BF16 ? 2 : 4;
     const int tile = qnn_attn_shared_tile(dtype, hd, most_rows * G);
     if (tile <= 0) return QNN_ERR_UNSUPPORTED;
     if ((q_stride * esize) % 16 || ((uintptr_t)q & 15) || ((uintptr_t)k_pool & 15) || ((uintptr_t)v_pool & 15) || ((uintptr_t)part_o & 15) ||
-        ((uintptr_t)part_ml & 7) || ((uintptr_t)groups & 15))
+        ((uintptr_t)part_ml & 7) || ((uintptr_t)groups & 15) || ((uintptr_t)out & 15) || (out_stride * esize) % 16)
         return QNN_ERR_ARGUMENT;
     const Cells cells = {page_table, max_pages, 31 - __builtin_clz((unsigned)page_size), ring / page_size, slots, slot_len, window};
     const int common_tiles = (most_rows * G + tile - 1) / tile;
     const Shared sh = {(const int4*)groups, row_group, n_groups, B, common_ranges, own_ranges, common_tiles};
     const long long items = (long long)n_groups * common_tiles * common_ranges + (long long)B * ((G + tile - 1) / tile) * own_ranges;
-    if (items > 0x7fffffff || (long long)B * nq > 0x7fffffff) return QNN_ERR_UNSUPPORTED;
+    const long long pool_rows = pool_pages * nkv * page_size;         // of the pools as matrices of head rows
+    if (items > 0x7fffffff || (long long)B * nq > 0x7fffffff || pool_rows <= 0 || pool_rows > 0x7fffffff) return QNN_ERR_UNSUPPORTED;
+    const Scores sc = {scale, cap, slopes};
     float2* ml = (float2*)part_ml;
     int rc = QNN_ERR_UNSUPPORTED;
     if (on_tensor_cores(dtype, hd)) {
@@ -670,8 +782,8 @@ QNN_API int qnn_attn_decode_shared(const void* q, long long q_stride, int dtype,
 #define QNN_MMA(HDV, NTV)                                                                                                                       \
     if (hd == HDV && nt == NTV)                                                                                                                  \
         rc = slopes != nullptr                                                                                                                   \
-                 ? launch_mma<HDV, NTV, true>(q, q_stride, k_pool, v_pool, cells, sh, (int)items, nq, nkv, scale, cap, part_o, ml, slopes, st)   \
-                 : launch_mma<HDV, NTV, false>(q, q_stride, k_pool, v_pool, cells, sh, (int)items, nq, nkv, scale, cap, part_o, ml, slopes, st);
+                 ? launch_mma<HDV, NTV, true>(q, q_stride, k_pool, v_pool, pool_rows, cells, sh, B, nq, nkv, sc, part_o, ml, status, st)   \
+                 : launch_mma<HDV, NTV, false>(q, q_stride, k_pool, v_pool, pool_rows, cells, sh, B, nq, nkv, sc, part_o, ml, status, st);
         QNN_MMA(64, 1) QNN_MMA(64, 2) QNN_MMA(64, 4) QNN_MMA(128, 1) QNN_MMA(128, 2) QNN_MMA(128, 4) QNN_MMA(256, 1) QNN_MMA(256, 2)
 #undef QNN_MMA
     } else {

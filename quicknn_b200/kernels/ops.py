@@ -329,9 +329,12 @@ def finite_flag(device) -> torch.Tensor:
 def wait_status_message(v: int) -> str:
     """What the status of the tcgen05 kernels says: bits of the waits that ran out (products: 1 loads, 2 tensor-core issue, 4
     epilogue; prompt attention: 2 keys and values, 4 scores, 8 weights, 16 ring, 32 queries, 64 product, 128 the other half of a
-    pair), and 256 for shared memory that does not start where the prompt attention needs it."""
+    pair), 256 for shared memory that does not start where the prompt attention needs it, and 512 for keys and values of rows that share
+    pages."""
     said = []
-    if v & 255 or not v & 256:
+    if v & 512:
+        said.append("gave up waiting for keys and values that rows share (status 512)")
+    if v & 255 or not v & 768:
         said.append(f"gave up waiting (status {v & 255}; products: 1 loads, 2 tensor-core issue, 4 epilogue; prompt attention: 2 keys and "
                     f"values, 4 scores, 8 weights, 16 ring, 32 queries, 64 product, 128 the other half of a pair)")
     if v & 256:
@@ -2375,8 +2378,8 @@ def shared_attention_plan(dtype: torch.dtype, n_rows: int, n_heads: int, n_kv: i
                 best = (t, s, p)
         ranges = best[1:]
     s, p = ranges
-    if s < 1 or p < 1:
-        raise ValueError("shared attention: at least one range of each kind")
+    if s < 1 or p < 1 or s + p > 128:
+        raise ValueError("shared attention: at least one range of each kind, and at most 128 together")
     return SharedPlan(s, p, max(n_rows, 1) * n_heads * (s + p) * (head_dim + 2) * 4)
 
 
@@ -2434,8 +2437,8 @@ def attn_decode_shared(qkv: torch.Tensor, n_heads: int, n_kv: int, head_dim: int
     _lib.check(_lib.load().qnn_attn_decode_shared(
         _p(qkv), ld, dt_code(qkv), _p(k_pool), _p(v_pool), _p(page_table), page_table.shape[1], page_size, ring, _p(slots), _p(slot_len), B,
         _p(shared.groups), shared.groups.shape[0], shared.rows, _p(shared.row_group), n_heads, n_kv, head_dim, float(scale), float(cap or 0.0),
-        int(window or 0), plan.common_ranges, plan.own_ranges, part_o, part_ml, _p(out), out.shape[1], _p(slopes), _p(sinks), _stream()),
-        "attn_decode_shared", 2)
+        int(window or 0), plan.common_ranges, plan.own_ranges, part_o, part_ml, _p(out), out.shape[1], _p(slopes), _p(sinks), k_pool.shape[0],
+        _p(_status_word(qkv.device)), _stream()), "attn_decode_shared", 2)
     return out
 
 
