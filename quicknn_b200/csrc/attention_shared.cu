@@ -15,129 +15,13 @@
 // per kv head; keys are walked in tiles of 16 positions.  An item leaves (m, l, O) in scratch (m in units of log2), and a second kernel joins a row's items in ascending order:
 // results depend on the numbers of ranges, not on what runs when.
 #include "attention_generic.cuh"
+#include "attention_shared.cuh"
 #include "tcgen05.cuh"
 
 using namespace qnn;
+using namespace qnn::shared;
 
 namespace {
-
-constexpr int TILE = 16;                      // positions
-constexpr float LOG2E = 1.4426950408889634f;
-
-__device__ __forceinline__ float exp2_fast(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-
-struct Shared {
-    const int4* groups;                       // first row, rows, first position, position behind the last
-    const int* row_group;                     // of a row: its group, or -1
-    int n_groups, B;
-    int common_ranges, own_ranges;            // S, P: parts 0 .. S - 1 of a row are of C, S .. S + P - 1 its own
-    int common_tiles;                         // tiles of query rows of a group
-};
-
-struct Cells {                                // where keys and values lie
-    const int* page_table;
-    int max_pages, page_shift, ring_pages;    // ring_pages 0: every position kept
-    const int* slots;
-    const int* slot_len;
-    int window;
-};
-
-// What an item works on, the same in all threads of its CTA: tiles t0 .. t1 - 1 of 16 positions each, the first `tiles_a` of the walk from
-// position a0 on, the others from b0 on (both multiples of 16; a row's own keys lie on both sides of C).  Positions outside lo .. hi - 1 that
-// a tile holds do not count.
-struct Item {
-    int row0, rows;                           // its rows of the batch
-    int slot;                                 // whose page table says where the keys are
-    int part;                                 // which part of those rows
-    int query0;                               // first query of the tile: query m is row row0 + m / G, head m % G of the kv head
-    int t0, t1;
-    int tiles_a, a0, b0, lo, hi;
-    __device__ __forceinline__ int position(int t) const { return t < tiles_a ? a0 + t * TILE : b0 + (t - tiles_a) * TILE; }
-};
-
-// The window's start and the length of a row (slot < 0: a row of no sequence, which sees nothing).
-__device__ __forceinline__ int2 sees(const Cells& c, int slot) {
-    if (slot < 0) return make_int2(0, 0);
-    const int n = c.ring_pages > 0 ? c.slot_len[slot] : min(c.slot_len[slot], c.max_pages << c.page_shift);   // no further than its page table
-    return make_int2(c.window > 0 && n > c.window ? n - c.window : 0, n);
-}
-
-// C of a group, by one warp (every lane gets it), and the slot of its first row that belongs to a sequence.  Of what all rows see only
-// whole pages: no tile then holds a cell that nobody has written.
-__device__ int3 common_keys(const Cells& c, int4 g) {
-    int lo = g.z, hi = g.w, slot = -1;
-#pragma unroll 4
-    for (int i = threadIdx.x & 31; i < g.y; i += 32) {
-        const int s = c.slots[g.x + i];
-        if (s < 0) continue;
-        const int2 w = sees(c, s);
-        lo = max(lo, w.x);
-        hi = min(hi, w.y);
-        if (slot < 0) slot = s;
-    }
-    lo = __reduce_max_sync(0xffffffffu, lo);
-    hi = __reduce_min_sync(0xffffffffu, hi);
-    const unsigned have = __ballot_sync(0xffffffffu, slot >= 0);
-    if (have == 0) return make_int3(0, 0, -1);
-    slot = __shfl_sync(0xffffffffu, slot, __ffs(have) - 1);
-    const int mask = (1 << c.page_shift) - 1;
-    lo = (lo + mask) & ~mask;
-    hi &= ~mask;
-    return make_int3(lo, max(lo, hi), slot);
-}
-
-__device__ __forceinline__ void take_range(Item& it, int tiles, int range, int ranges) {
-    const int per = (tiles + ranges - 1) / ranges;
-    it.t0 = min(range * per, tiles);
-    it.t1 = min(it.t0 + per, tiles);
-}
-
-// Range `range` of C of group `group` for the queries from tile `q_tile` on.  Every warp works it out.
-__device__ Item common_item(const Shared& sh, const Cells& c, int group, int q_tile, int range, int tile) {
-    Item it;
-    const int4 g = sh.groups[group];
-    it.row0 = g.x;
-    it.rows = g.y;
-    it.query0 = q_tile * tile;
-    it.part = range;
-    const int3 k = common_keys(c, g);
-    it.slot = k.z;
-    it.tiles_a = 0;
-    it.a0 = it.b0 = it.lo = k.x;
-    it.hi = k.y;
-    take_range(it, (k.y - k.x) / TILE, range, sh.common_ranges);
-    return it;
-}
-
-// Range `range` of row `row`'s own keys.
-__device__ Item own_item(const Shared& sh, const Cells& c, int row, int q_tile, int range, int tile) {
-    Item it;
-    it.row0 = row;
-    it.rows = 1;
-    it.query0 = q_tile * tile;
-    it.part = sh.common_ranges + range;
-    it.slot = c.slots[row];
-    const int g = sh.row_group[row];
-    const int2 w = sees(c, it.slot);
-    it.lo = w.x;
-    it.hi = w.y;
-    it.a0 = w.x & ~(TILE - 1);
-    it.tiles_a = 0;
-    it.b0 = it.a0;
-    if (g >= 0 && it.slot >= 0) {
-        const int3 k = common_keys(c, sh.groups[g]);
-        if (k.y > k.x) {                      // C lies inside what the row sees, and starts and ends with pages
-            it.tiles_a = (k.x - it.a0) / TILE;
-            it.b0 = k.y;
-        }
-    }
-    take_range(it, it.tiles_a + max(0, it.hi - it.b0 + TILE - 1) / TILE, range, sh.own_ranges);
-    return it;
-}
 
 // The page ids of an item's keys, pages from that of its first position on; returns the number of that page.
 __device__ __forceinline__ int load_pages(const Item& it, const Cells& c, int* pages) {
@@ -148,11 +32,6 @@ __device__ __forceinline__ int load_pages(const Item& it, const Cells& c, int* p
         pages[u] = row[c.ring_pages > 0 ? p % c.ring_pages : p];
     }
     return first;
-}
-
-// Where part `part` of query m of an item goes.
-__device__ __forceinline__ size_t part_of(const Item& it, const Shared& sh, int m, int kh, int G, int nq) {
-    return ((size_t)(it.row0 + m / G) * nq + kh * G + m % G) * (sh.common_ranges + sh.own_ranges) + it.part;
 }
 
 // ---- tensor cores, bfloat16 -------------------------------------------------------------------------------------------------
@@ -185,11 +64,6 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-
-struct Scores {
-    float scale, cap;
-    const float* slopes;
-};
 
 // The walk of one item.  smem: the warps' rings, which the merge reuses, then the barriers, then the page ids.
 template <int HD>
@@ -683,15 +557,19 @@ attn_shared_join_kernel(const float* __restrict__ part_o, const float2* __restri
 
 bool on_tensor_cores(int dtype, int hd) { return dtype == QNN_DT_BF16 && (hd == 64 || hd == 128 || hd == 256); }
 
+// Groups of more query rows than an item of the kernel above takes go to the 5th-generation tensor cores, where a CTA takes 128.
+constexpr int MANY_TILE = 128;
+bool many_rows(int dtype, int hd, int queries) { return on_tensor_cores(dtype, hd) && queries > (hd > 128 ? 16 : 32); }
+
 // Column tiles of an item for so many queries: 1, 2 or, up to head size 128, 4.  More do not fit the registers (O and Q of 16 queries of 256
 // elements are 192 registers a thread).
 int column_tiles(int hd, int queries) { return queries <= 8 ? 1 : (queries <= 16 || hd > 128 ? 2 : 4); }
 
 template <int HD, int NT, bool BIAS>
 int launch_mma(const void* q, long long q_stride, const void* k_pool, const void* v_pool, long long pool_rows, const Cells& cells, const Shared& sh,
-               int B, int nq, int nkv, const Scores& sc, float* part_o, float2* part_ml, int* status, cudaStream_t st) {
+               bool with_common, int B, int nq, int nkv, const Scores& sc, float* part_o, float2* part_ml, int* status, cudaStream_t st) {
     const int G = nq / nkv, own_tile = G <= 8 ? 8 : 8 * NT;
-    const long long common = (long long)sh.n_groups * sh.common_tiles * sh.common_ranges, own = (long long)B * ((G + own_tile - 1) / own_tile) * sh.own_ranges;
+    const long long common = with_common ? (long long)sh.n_groups * sh.common_tiles * sh.common_ranges : 0, own = (long long)B * ((G + own_tile - 1) / own_tile) * sh.own_ranges;
     if (common + own > 0x7fffffff) return QNN_ERR_UNSUPPORTED;
     const size_t smem = 1024 + Layout<HD>::ring_bytes(NT) + Layout<HD>::BARRIERS + ((size_t)cells.max_pages + 2) * sizeof(int);
     if (smem > 220 * 1024) return QNN_ERR_UNSUPPORTED;
@@ -742,7 +620,7 @@ int launch_join(const float* part_o, const float2* part_ml, void* out, long long
 QNN_API int qnn_attn_shared_tile(int dtype, int hd, int queries) {
     const int vec = dtype == QNN_DT_BF16 ? 8 : 4;
     if (hd <= 0 || hd % vec || hd > 1024) return -1;
-    return on_tensor_cores(dtype, hd) ? 8 * column_tiles(hd, queries) : GEN_QT;
+    return many_rows(dtype, hd, queries) ? MANY_TILE : (on_tensor_cores(dtype, hd) ? 8 * column_tiles(hd, queries) : GEN_QT);
 }
 
 // groups: [n_groups][4] (first row, rows, begin, end): positions begin .. end - 1 lie in the same pages in all the group's rows, as far as a row
@@ -763,7 +641,8 @@ QNN_API int qnn_attn_decode_shared(const void* q, long long q_stride, int dtype,
     if (page_size < 16 || (page_size & (page_size - 1)) || ring < 0 || ring % page_size) return QNN_ERR_ARGUMENT;
     if (ring > 0 && (window <= 0 || window > ring || ring / page_size > max_pages)) return QNN_ERR_ARGUMENT;   // a ring holds no more
     const int G = nq / nkv, esize = dtype == QNN_DT_BF16 ? 2 : 4;
-    const int tile = qnn_attn_shared_tile(dtype, hd, most_rows * G);
+    const bool many = page_size >= 64 && many_rows(dtype, hd, most_rows * G);
+    const int tile = many ? MANY_TILE : (on_tensor_cores(dtype, hd) ? 8 * column_tiles(hd, most_rows * G) : qnn_attn_shared_tile(dtype, hd, most_rows * G));
     if (tile <= 0) return QNN_ERR_UNSUPPORTED;
     if ((q_stride * esize) % 16 || ((uintptr_t)q & 15) || ((uintptr_t)k_pool & 15) || ((uintptr_t)v_pool & 15) || ((uintptr_t)part_o & 15) ||
         ((uintptr_t)part_ml & 7) || ((uintptr_t)groups & 15) || ((uintptr_t)out & 15) || (out_stride * esize) % 16)
@@ -771,19 +650,24 @@ QNN_API int qnn_attn_decode_shared(const void* q, long long q_stride, int dtype,
     const Cells cells = {page_table, max_pages, 31 - __builtin_clz((unsigned)page_size), ring / page_size, slots, slot_len, window};
     const int common_tiles = (most_rows * G + tile - 1) / tile;
     const Shared sh = {(const int4*)groups, row_group, n_groups, B, common_ranges, own_ranges, common_tiles};
-    const long long items = (long long)n_groups * common_tiles * common_ranges + (long long)B * ((G + tile - 1) / tile) * own_ranges;
+    const int own_tile = on_tensor_cores(dtype, hd) ? 8 : GEN_QT;
+    const long long items = (long long)n_groups * common_tiles * common_ranges + (long long)B * ((G + own_tile - 1) / own_tile) * own_ranges;
     const long long pool_rows = pool_pages * nkv * page_size;         // of the pools as matrices of head rows
     if (items > 0x7fffffff || (long long)B * nq > 0x7fffffff || pool_rows <= 0 || pool_rows > 0x7fffffff) return QNN_ERR_UNSUPPORTED;
     const Scores sc = {scale, cap, slopes};
     float2* ml = (float2*)part_ml;
     int rc = QNN_ERR_UNSUPPORTED;
     if (on_tensor_cores(dtype, hd)) {
-        const int nt = tile / 8;
+        if (many) {
+            const SharedLaunch a = {q, q_stride, k_pool, v_pool, pool_rows, cells, sh, nq, nkv, hd, sc, part_o, ml, status};
+            if (const int err = launch_common_tcgen05(a, st)) return err;
+        }
+        const int nt = many ? column_tiles(hd, G) : tile / 8;
 #define QNN_MMA(HDV, NTV)                                                                                                                       \
     if (hd == HDV && nt == NTV)                                                                                                                  \
         rc = slopes != nullptr                                                                                                                   \
-                 ? launch_mma<HDV, NTV, true>(q, q_stride, k_pool, v_pool, pool_rows, cells, sh, B, nq, nkv, sc, part_o, ml, status, st)   \
-                 : launch_mma<HDV, NTV, false>(q, q_stride, k_pool, v_pool, pool_rows, cells, sh, B, nq, nkv, sc, part_o, ml, status, st);
+                 ? launch_mma<HDV, NTV, true>(q, q_stride, k_pool, v_pool, pool_rows, cells, sh, !many, B, nq, nkv, sc, part_o, ml, status, st)   \
+                 : launch_mma<HDV, NTV, false>(q, q_stride, k_pool, v_pool, pool_rows, cells, sh, !many, B, nq, nkv, sc, part_o, ml, status, st);
         QNN_MMA(64, 1) QNN_MMA(64, 2) QNN_MMA(64, 4) QNN_MMA(128, 1) QNN_MMA(128, 2) QNN_MMA(128, 4) QNN_MMA(256, 1) QNN_MMA(256, 2)
 #undef QNN_MMA
     } else {

@@ -1,0 +1,156 @@
+// What the attention of rows that share pages is made of: which keys a group of rows has in common, the items that the work is cut into,
+// and where their results go.  See attention_shared.cu.
+#pragma once
+#include "common.cuh"
+#include <math_constants.h>
+
+namespace qnn {
+namespace shared {
+
+constexpr int TILE = 16;                      // positions
+constexpr float LOG2E = 1.4426950408889634f;
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+struct Shared {
+    const int4* groups;                       // first row, rows, first position, position behind the last
+    const int* row_group;                     // of a row: its group, or -1
+    int n_groups, B;
+    int common_ranges, own_ranges;            // S, P: parts 0 .. S - 1 of a row are of C, S .. S + P - 1 its own
+    int common_tiles;                         // tiles of query rows of a group
+};
+
+struct Cells {                                // where keys and values lie
+    const int* page_table;
+    int max_pages, page_shift, ring_pages;    // ring_pages 0: every position kept
+    const int* slots;
+    const int* slot_len;
+    int window;
+};
+
+// What an item works on, the same in all threads of its CTA: tiles t0 .. t1 - 1 of 16 positions each, the first `tiles_a` of the walk from
+// position a0 on, the others from b0 on (both multiples of 16; a row's own keys lie on both sides of C).  Positions outside lo .. hi - 1 that
+// a tile holds do not count.
+struct Item {
+    int row0, rows;                           // its rows of the batch
+    int slot;                                 // whose page table says where the keys are
+    int part;                                 // which part of those rows
+    int query0;                               // first query of the tile: query m is row row0 + m / G, head m % G of the kv head
+    int t0, t1;
+    int tiles_a, a0, b0, lo, hi;
+    __device__ __forceinline__ int position(int t) const { return t < tiles_a ? a0 + t * TILE : b0 + (t - tiles_a) * TILE; }
+};
+
+// The window's start and the length of a row (slot < 0: a row of no sequence, which sees nothing).
+__device__ __forceinline__ int2 sees(const Cells& c, int slot) {
+    if (slot < 0) return make_int2(0, 0);
+    const int n = c.ring_pages > 0 ? c.slot_len[slot] : min(c.slot_len[slot], c.max_pages << c.page_shift);   // no further than its page table
+    return make_int2(c.window > 0 && n > c.window ? n - c.window : 0, n);
+}
+
+// C of a group, by one warp (every lane gets it), and the slot of its first row that belongs to a sequence.  Of what all rows see only
+// whole pages: no tile then holds a cell that nobody has written.
+static __device__ int3 common_keys(const Cells& c, int4 g) {
+    int lo = g.z, hi = g.w, slot = -1;
+#pragma unroll 4
+    for (int i = threadIdx.x & 31; i < g.y; i += 32) {
+        const int s = c.slots[g.x + i];
+        if (s < 0) continue;
+        const int2 w = sees(c, s);
+        lo = max(lo, w.x);
+        hi = min(hi, w.y);
+        if (slot < 0) slot = s;
+    }
+    lo = __reduce_max_sync(0xffffffffu, lo);
+    hi = __reduce_min_sync(0xffffffffu, hi);
+    const unsigned have = __ballot_sync(0xffffffffu, slot >= 0);
+    if (have == 0) return make_int3(0, 0, -1);
+    slot = __shfl_sync(0xffffffffu, slot, __ffs(have) - 1);
+    const int mask = (1 << c.page_shift) - 1;
+    lo = (lo + mask) & ~mask;
+    hi &= ~mask;
+    return make_int3(lo, max(lo, hi), slot);
+}
+
+// Range `range` of so many, in whole units of `unit` tiles.
+__device__ __forceinline__ void take_range(Item& it, int tiles, int range, int ranges, int unit = 1) {
+    const int per = ((tiles + unit - 1) / unit + ranges - 1) / ranges * unit;
+    it.t0 = min(range * per, tiles);
+    it.t1 = min(it.t0 + per, tiles);
+}
+
+// Range `range` of C of group `group` for the queries from tile `q_tile` on.  Every warp works it out.
+static __device__ Item common_item(const Shared& sh, const Cells& c, int group, int q_tile, int range, int tile, int unit = 1) {
+    Item it;
+    const int4 g = sh.groups[group];
+    it.row0 = g.x;
+    it.rows = g.y;
+    it.query0 = q_tile * tile;
+    it.part = range;
+    const int3 k = common_keys(c, g);
+    it.slot = k.z;
+    it.tiles_a = 0;
+    it.a0 = it.b0 = it.lo = k.x;
+    it.hi = k.y;
+    take_range(it, (k.y - k.x) / TILE, range, sh.common_ranges, unit);
+    return it;
+}
+
+// Range `range` of row `row`'s own keys.
+static __device__ Item own_item(const Shared& sh, const Cells& c, int row, int q_tile, int range, int tile) {
+    Item it;
+    it.row0 = row;
+    it.rows = 1;
+    it.query0 = q_tile * tile;
+    it.part = sh.common_ranges + range;
+    it.slot = c.slots[row];
+    const int g = sh.row_group[row];
+    const int2 w = sees(c, it.slot);
+    it.lo = w.x;
+    it.hi = w.y;
+    it.a0 = w.x & ~(TILE - 1);
+    it.tiles_a = 0;
+    it.b0 = it.a0;
+    if (g >= 0 && it.slot >= 0) {
+        const int3 k = common_keys(c, sh.groups[g]);
+        if (k.y > k.x) {                      // C lies inside what the row sees, and starts and ends with pages
+            it.tiles_a = (k.x - it.a0) / TILE;
+            it.b0 = k.y;
+        }
+    }
+    take_range(it, it.tiles_a + max(0, it.hi - it.b0 + TILE - 1) / TILE, range, sh.own_ranges);
+    return it;
+}
+
+// Where part `part` of query m of an item goes.
+__device__ __forceinline__ size_t part_of(const Item& it, const Shared& sh, int m, int kh, int G, int nq) {
+    return ((size_t)(it.row0 + m / G) * nq + kh * G + m % G) * (sh.common_ranges + sh.own_ranges) + it.part;
+}
+
+struct Scores {
+    float scale, cap;
+    const float* slopes;
+};
+
+// The items of C on the 5th-generation tensor cores (attention_shared_tcgen05.cu): groups of many rows.
+struct SharedLaunch {
+    const void* q;
+    long long q_stride;
+    const void *k_pool, *v_pool;
+    long long pool_rows;
+    Cells cells;
+    Shared sh;
+    int nq, nkv, hd;
+    Scores sc;
+    float* part_o;
+    float2* part_ml;
+    int* status;
+};
+int launch_common_tcgen05(const SharedLaunch& a, cudaStream_t st);
+
+}  // namespace shared
+}  // namespace qnn

@@ -134,6 +134,46 @@ def test_rows_of_a_group(rows, nq, nkv, hd, dtype):
     b.check(b.run(hd ** -0.5, 30.0), hd ** -0.5, 30.0)
 
 
+@pytest.mark.parametrize("pages", [1, 2, 3, 6, 7])
+@pytest.mark.parametrize("nq,nkv,hd", [(8, 4, 256), (9, 1, 256), (8, 2, 128), (16, 2, 64)])
+@pytest.mark.parametrize("cap", [None, 50.0, 90.0])
+def test_many_rows(cap, nq, nkv, hd, pages):
+    # more query rows than a warp holds: 128 at a time, one or two pages of the pairs there, all divisions of the pages
+    rows = {256: 18, 128: 70, 64: 19}[hd]
+    b = Batch([(0, pages * 64, [pages * 64 + 1 + i % 90 for i in range(rows)]), (64, 192, [200, 222])], nq, nkv, hd, BF, alone=[130], left_out=[3], seed=pages + hd)
+    for ranges in ((1, 1), (2, 1), (3, 2), (9, 1)):
+        b.check(b.run(hd ** -0.5, cap, ranges), hd ** -0.5, cap)
+
+
+@pytest.mark.parametrize("nq,nkv,hd", [(8, 4, 256), (8, 2, 128), (8, 1, 64)])
+def test_many_rows_with_slopes_sinks_and_windows(nq, nkv, hd):
+    g = torch.Generator(device=DEV).manual_seed(hd)
+    slopes = torch.rand(nq, device=DEV, generator=g) * 0.02
+    sinks = 3 * torch.randn(nq, device=DEV, generator=g)
+    lens = [449 + 7 * i % 120 for i in range(34)]
+    b = Batch([(0, 448, lens)], nq, nkv, hd, BF, seed=hd)
+    for sl, si, cap in ((slopes, None, None), (slopes, sinks, 40.0), (None, sinks, 40.0)):
+        b.check(b.run(hd ** -0.5, cap, (2, 2), slopes=sl, sinks=si), hd ** -0.5, cap, sl, si)
+    b = Batch([(0, 448, lens)], nq, nkv, hd, BF, window=300, seed=hd + 1)
+    b.check(b.run(hd ** -0.5, None, (2, 1)), hd ** -0.5)
+    b = Batch([(64 * 20, 64 * 24, [64 * 24 + 1 + i for i in range(60)])], nq, nkv, hd, BF, window=384, ring=384, seed=hd + 2)
+    b.check(b.run(hd ** -0.5, 50.0), hd ** -0.5, 50.0)
+
+
+def test_many_rows_of_large_scores():
+    b = Batch([(0, 704, [705 + i for i in range(40)])], 8, 4, 64, BF, seed=17)
+    pages = torch.from_numpy(b.table[b.slots[0]].astype(np.int64)).to(DEV)
+    pos = torch.arange(704, device=DEV)
+    for sign in (1, -1):
+        ramp = torch.linspace(-1, 1, 704, device=DEV) * sign
+        keys = (b.qkv[0, :64].float() * 3 * ramp[:, None, None]).to(BF).expand(704, 4, 64)
+        for k in b.k_of:
+            k[:704] = keys
+        b.k[pages[pos // 64], :, pos % 64] = keys
+        for ranges in ((1, 1), (2, 1)):
+            b.check(b.run(1.0, None, ranges), 1.0)
+
+
 @pytest.mark.parametrize("ranges", [(1, 1), (1, 3), (5, 1), (7, 4), (64, 40)])
 @pytest.mark.parametrize("nq,nkv,hd,dtype", [(8, 4, 256, BF), (8, 2, 64, BF), (6, 1, 24, FP)])
 def test_numbers_of_ranges(ranges, nq, nkv, hd, dtype):
