@@ -7,7 +7,7 @@
 // Within a beam the order of the scores is that of the logits, so one pass over the logits is enough for everything but a few of them:
 //   1. a warp per segment of a row (SEGMENT logits) leaves the segment's maximum and sum of exp(z - maximum);
 //   2. a block per request joins them to log(sum exp) of every beam, turns the segments' maxima into scores, and takes as a threshold the
-//      `take`-th largest of 256 groups' maxima, so that at least `take` segments reach it.  As each of these holds a score that reaches it, so do the `take` best of all; they lie in the segments
+//      `take`-th largest of 128 groups' maxima, so that at least `take` segments reach it.  As each of these holds a score that reaches it, so do the `take` best of all; they lie in the segments
 //      that reach it, which are read again (a few KB) into a short list, whose best are found by counting.
 // Scores are formed in 64 bits: those of different beams may differ by less than 32 bits resolve after a sum over the vocabulary.
 // A logit that is not finite is no continuation and not in the sum (bit 0 of the error word says so); nor is any of a beam whose score is
@@ -100,6 +100,7 @@ __device__ __forceinline__ unsigned ordered(float f) {
     const unsigned u = __float_as_uint(f);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ float unordered(unsigned u) { return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u); }
 __device__ __forceinline__ bool before(double a, unsigned ia, double b, unsigned ib) { return a > b || (a == b && ia < ib); }
 
 struct Found {
@@ -121,7 +122,7 @@ beam_pick_kernel(const float* __restrict__ logits, int V, int beams, int take, i
     Found* found = reinterpret_cast<Found*>(smem);
     double* base = reinterpret_cast<double*>(found + 1);      // [beams] t_b - log(sum exp)
     unsigned* best = reinterpret_cast<unsigned*>(base + beams);   // [beams * segments] the segments' best scores, ordered
-    constexpr int WARPS = SELECT_THREADS / 32, GROUPS = 256;
+    constexpr int WARPS = SELECT_THREADS / 32, GROUPS = 128, KEPT = 4;
     __shared__ float part_m[WARPS];
     __shared__ double part_s[WARPS];
     __shared__ unsigned group_best[GROUPS], threshold_s;
@@ -134,64 +135,85 @@ beam_pick_kernel(const float* __restrict__ logits, int V, int beams, int take, i
         n_found = n_reached = 0;
         threshold_s = 1u;                     // fewer groups than wanted: all that hold anything
     }
-    // log(sum exp) of every beam, by as many warps as there are for each
+    // log(sum exp) of every beam, by as many warps as there are for each; a lane keeps its segments' numbers where they fit
     const int share = beams >= WARPS ? 1 : WARPS / beams;
     for (int b0 = 0; b0 < beams; b0 += WARPS / share) {
-        const int b = b0 + warp / share, p = warp % share;
+        const int b = b0 + warp / share, p = warp % share, i0 = p * 32 + lane, step = share * 32;
         const bool mine = warp / share < WARPS / share && b < beams;
         const float2* st = stats + (row0 + (mine ? b : 0)) * segments;
+        const double t = mine ? (double)scores[row0 + b] : 0.0;
+        float2 kept[KEPT];
         float m = -CUDART_INF_F;
+#pragma unroll
+        for (int k = 0; k < KEPT; ++k) {
+            kept[k] = mine && i0 + k * step < segments ? st[i0 + k * step] : make_float2(-CUDART_INF_F, 0.f);
+            m = fmaxf(m, kept[k].x);
+        }
         if (mine)
-#pragma unroll 4
-            for (int i = p * 32 + lane; i < segments; i += share * 32) m = fmaxf(m, st[i].x);
+            for (int i = i0 + KEPT * step; i < segments; i += step) m = fmaxf(m, st[i].x);
         m = qnn::warp_max(m);
-        if (lane == 0) part_m[warp] = m;
-        __syncthreads();
-        for (int i = 0; i < share; ++i) m = fmaxf(m, part_m[warp / share * share + i]);
+        if (share > 1) {
+            if (lane == 0) part_m[warp] = m;
+            __syncthreads();
+            if (mine)
+                for (int i = 0; i < share; ++i) m = fmaxf(m, part_m[warp / share * share + i]);
+        }
         double s = 0.0;
-        if (mine && m != -CUDART_INF_F)
-#pragma unroll 4
-            for (int i = p * 32 + lane; i < segments; i += share * 32) s += (double)(st[i].y * expf(st[i].x - m));
+        if (mine && m != -CUDART_INF_F) {
+#pragma unroll
+            for (int k = 0; k < KEPT; ++k) s += (double)(kept[k].y * expf(kept[k].x - m));       // (0 times exp(-inf) where there is none)
+            for (int i = i0 + KEPT * step; i < segments; i += step) s += (double)(st[i].y * expf(st[i].x - m));
+        }
         s = warp_sum(s);
-        if (lane == 0) part_s[warp] = s;
-        __syncthreads();
-        if (mine) {
+        if (share > 1) {
+            if (lane == 0) part_s[warp] = s;
+            __syncthreads();
             s = 0.0;
-            for (int i = 0; i < share; ++i) s += part_s[warp / share * share + i];
-            const double t = (double)scores[row0 + b];
+            if (mine)
+                for (int i = 0; i < share; ++i) s += part_s[warp / share * share + i];
+        }
+        if (mine) {
             const bool alive = m != -CUDART_INF_F && t > -CUDART_INF && t < CUDART_INF;
             const double add = alive ? t - (double)m - log(s) : -CUDART_INF;
             if (p == 0 && lane == 0) base[b] = add;
-            for (int i = p * 32 + lane; i < segments; i += share * 32) {
-                const float z = st[i].x;
-                best[b * segments + i] = alive && z != -CUDART_INF_F ? ordered((float)(add + (double)z)) : 0u;    // 0: none
-            }
+            const auto note = [&](int i, float z) {
+                best[b * segments + i] = alive && z != -CUDART_INF_F ? ordered((float)(add + (double)z)) : 0u;      // 0: none
+            };
+#pragma unroll
+            for (int k = 0; k < KEPT; ++k)
+                if (i0 + k * step < segments) note(i0 + k * step, kept[k].x);
+            for (int i = i0 + KEPT * step; i < segments; i += step) note(i, st[i].x);
         }
-        __syncthreads();
+        if (b0 + WARPS / share < beams) __syncthreads();      // the partial results have been read
     }
-    // The threshold: segments in 256 groups, the `take`-th largest of the groups' maxima (found by counting).
+    // The threshold: segment i is in group i % 128; the `take`-th largest of the groups' maxima (found by counting).
     const int n = beams * segments;
-    unsigned top = 0u;                        // (segment i is in group i % 256)
-    for (int i = (threadIdx.x >> 2) + (threadIdx.x & 3) * GROUPS; i < n; i += SELECT_THREADS) top = max(top, best[i]);
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    if ((threadIdx.x & 3) == 0) group_best[threadIdx.x >> 2] = top;
+    __syncthreads();
+    unsigned most = 0u;                       // eight threads a group
+    for (int i = (threadIdx.x >> 3) + (threadIdx.x & 7) * GROUPS; i < n; i += SELECT_THREADS) most = max(most, best[i]);
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 4));
+    if ((threadIdx.x & 7) == 0) group_best[threadIdx.x >> 3] = most;
     __syncthreads();
     {
-        const int g = threadIdx.x >> 2;       // four threads a group, each counts a quarter
+        const int g = threadIdx.x >> 3;       // each of the eight counts against an eighth
+        const unsigned top = most;
         int rank = 0;
-#pragma unroll 16
-        for (int j = 0; j < GROUPS / 4; ++j) {
-            const int o = j * 4 + (threadIdx.x & 3);
+#pragma unroll
+        for (int j = 0; j < GROUPS / 8; ++j) {
+            const int o = j * 8 + (threadIdx.x & 7);
             const unsigned other = group_best[o];
             rank += other > top || (other == top && o < g);
         }
         rank += __shfl_xor_sync(0xffffffffu, rank, 1);
         rank += __shfl_xor_sync(0xffffffffu, rank, 2);
-        if (rank == take - 1 && (threadIdx.x & 3) == 0 && top > 1u) threshold_s = top;
+        rank += __shfl_xor_sync(0xffffffffu, rank, 4);
+        if (rank == take - 1 && (threadIdx.x & 7) == 0 && top > 1u) threshold_s = top;
     }
     __syncthreads();
     const unsigned threshold = threshold_s;
+    const float threshold_f = unordered(threshold);
     for (int i = threadIdx.x; i < n; i += SELECT_THREADS)
         if (best[i] >= threshold) {
             const int at = atomicAdd(&n_reached, 1);
@@ -206,13 +228,16 @@ beam_pick_kernel(const float* __restrict__ logits, int V, int beams, int take, i
         const int b = i / segments, v0 = (i - b * segments) * SEGMENT;
         const float* row = logits + (row0 + b) * V;
         const double add = base[b];
+        // logits below this are out, whatever the roundings (most of them, and the others are looked at in 64 bits)
+        const double exactly = (double)threshold_f - add;
+        const float limit = threshold > 1u ? (float)(exactly - 1e-5 * (fabs(exactly) + fabs((double)threshold_f))) : -CUDART_INF_F;
         float z[SEGMENT / 32];
 #pragma unroll
         for (int j = 0; j < SEGMENT / 32; ++j) z[j] = row[min(v0 + j * 32 + lane, V - 1)];
 #pragma unroll
         for (int j = 0; j < SEGMENT / 32; ++j) {
             const int v = v0 + j * 32 + lane;
-            if (v >= V || !isfinite(z[j])) continue;
+            if (v >= V || !isfinite(z[j]) || z[j] < limit) continue;
             const double s = add + (double)z[j];
             if (ordered((float)s) < threshold) continue;
             const int at = atomicAdd(&n_found, 1);
