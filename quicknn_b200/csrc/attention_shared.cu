@@ -75,8 +75,7 @@ struct Layout {
 };
 
 template <int HD, int NT, bool BIAS>
-__device__ __forceinline__ void walk(const Item& it, int queries, const CUtensorMap& map_k, const CUtensorMap& map_v, const bf16* __restrict__ q, size_t q_stride,
-                                     const Cells& cells, const Shared& sh, int kh, int nq, int nkv, const Scores& sc, float* __restrict__ part_o,
+__device__ __forceinline__ void walk(const Item& it, int queries, const CUtensorMap& map, KV kv, const bf16* __restrict__ q, size_t q_stride, const Cells& cells, const Shared& sh, int kh, int nq, int nkv, const Scores& sc, float* __restrict__ part_o,
                                      float2* __restrict__ part_ml, int* __restrict__ status, unsigned char* smem, const int* pages, int first_page, unsigned bars) {
     using L = Layout<HD>;
     constexpr int KSTEPS = HD / 16, QT = 8 * NT;
@@ -91,9 +90,9 @@ __device__ __forceinline__ void walk(const Item& it, int queries, const CUtensor
         const unsigned kst = ring + s * 2 * L::TILE_BYTES, bar = bar0 + s * 8;
         tc::mbar_expect_tx(bar, 2 * L::TILE_BYTES);
 #pragma unroll
-        for (int d = 0; d < HD / 64; ++d) tc::tma_load_2d(kst + d * TILE * 128, &map_k, bar, d * 64, y);
+        for (int d = 0; d < HD / 64; ++d) load_rows(kst + d * TILE * 128, &map, bar, d * 64, y, kv.k);
 #pragma unroll
-        for (int d = 0; d < HD / 64; ++d) tc::tma_load_2d(kst + L::TILE_BYTES + d * TILE * 128, &map_v, bar, d * 64, y);
+        for (int d = 0; d < HD / 64; ++d) load_rows(kst + L::TILE_BYTES + d * TILE * 128, &map, bar, d * 64, y, kv.v);
     };
     if (tc::elect_one())
         for (int n = 0; n < STAGES && n < my_tiles; ++n) fetch(n);
@@ -290,7 +289,7 @@ __device__ __forceinline__ void walk(const Item& it, int queries, const CUtensor
 // of an item of C; a row's own heads take one where they fit it.
 template <int HD, int NT, bool BIAS>
 __global__ void __launch_bounds__(WARPS * 32)
-attn_shared_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const bf16* __restrict__ q, size_t q_stride,
+attn_shared_mma_kernel(const __grid_constant__ CUtensorMap map, const KV kv, const bf16* __restrict__ q, size_t q_stride,
                        const Cells cells, const Shared sh, int common_items, int own_tile, int nq, int nkv, const Scores sc, float* __restrict__ part_o,
                        float2* __restrict__ part_ml, int* __restrict__ status) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -325,9 +324,9 @@ attn_shared_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         return;
     }
     if (NT > 1 && own && own_tile == 8)
-        walk<HD, 1, BIAS>(it, queries, map_k, map_v, q, q_stride, cells, sh, kh, nq, nkv, sc, part_o, part_ml, status, smem, pages, first_page, bars);
+        walk<HD, 1, BIAS>(it, queries, map, kv, q, q_stride, cells, sh, kh, nq, nkv, sc, part_o, part_ml, status, smem, pages, first_page, bars);
     else
-        walk<HD, NT, BIAS>(it, queries, map_k, map_v, q, q_stride, cells, sh, kh, nq, nkv, sc, part_o, part_ml, status, smem, pages, first_page, bars);
+        walk<HD, NT, BIAS>(it, queries, map, kv, q, q_stride, cells, sh, kh, nq, nkv, sc, part_o, part_ml, status, smem, pages, first_page, bars);
 }
 
 // ---- any head size, float32 or bfloat16 ----------------------------------------------------------------------------------------
@@ -573,13 +572,13 @@ int launch_mma(const void* q, long long q_stride, const void* k_pool, const void
     if (common + own > 0x7fffffff) return QNN_ERR_UNSUPPORTED;
     const size_t smem = 1024 + Layout<HD>::ring_bytes(NT) + Layout<HD>::BARRIERS + ((size_t)cells.max_pages + 2) * sizeof(int);
     if (smem > 220 * 1024) return QNN_ERR_UNSUPPORTED;
-    CUtensorMap map_k, map_v;
-    if (const int rc = tc::make_map_bf16(&map_k, k_pool, pool_rows, HD, TILE)) return rc;
-    if (const int rc = tc::make_map_bf16(&map_v, v_pool, pool_rows, HD, TILE)) return rc;
+    CUtensorMap map;
+    KV kv;
+    if (const int rc = make_pools_map(&map, &kv, k_pool, v_pool, pool_rows, HD, TILE)) return rc;
     auto kern = attn_shared_mma_kernel<HD, NT, BIAS>;
     static OncePerDevice asked;
     if (const int rc = allow_shared(asked, kern, 220 * 1024)) return rc;
-    launch_pdl(kern, dim3((unsigned)(common + own), nkv), dim3(WARPS * 32), smem, st, map_k, map_v, (const bf16*)q, (size_t)q_stride, cells, sh, (int)common,
+    launch_pdl(kern, dim3((unsigned)(common + own), nkv), dim3(WARPS * 32), smem, st, map, kv, (const bf16*)q, (size_t)q_stride, cells, sh, (int)common,
                own_tile, nq, nkv, sc, part_o, part_ml, status);
     return (int)cudaGetLastError();
 }

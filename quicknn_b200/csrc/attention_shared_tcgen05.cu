@@ -101,7 +101,7 @@ __device__ __forceinline__ bool has_failed(Barriers* b) { return *reinterpret_ca
 
 template <int HD, bool FIXED>
 __global__ void __launch_bounds__(THREADS)
-attn_shared_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const bf16* __restrict__ q, size_t q_stride,
+attn_shared_tcgen05_kernel(const __grid_constant__ CUtensorMap map, const KV kv, const bf16* __restrict__ q, size_t q_stride,
                            const Cells cells, const Shared sh, int nq, int nkv, const Scores sc, float* __restrict__ part_o, float2* __restrict__ part_ml,
                            int* __restrict__ status) {
     constexpr int KS = k_stages(HD), VS = v_stages(HD);
@@ -185,8 +185,8 @@ attn_shared_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
                 const unsigned full = smem_u32(&bars->k_full[s]), dst = smem_u32(sK + s * KP_BYTES);
                 mbar_expect_tx(full, KP_BYTES);
                 for (int d = 0; d < HD / 64; ++d) {
-                    tma_load_2d(dst + d * (2 * BN * 128), &map_k, full, d * 64, lower);
-                    tma_load_2d(dst + d * (2 * BN * 128) + BN * 128, &map_k, full, d * 64, upper);
+                    load_rows(dst + d * (2 * BN * 128), &map, full, d * 64, lower, kv.k);
+                    load_rows(dst + d * (2 * BN * 128) + BN * 128, &map, full, d * 64, upper, kv.k);
                 }
                 lower = tile_row(2 * J + 2);
                 upper = tile_row(2 * J + 3);
@@ -203,7 +203,7 @@ attn_shared_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
                 if (j >= VS && !mbar_wait(smem_u32(&bars->v_empty[s]), ((j / VS) - 1) & 1)) { give_up(16); break; }
                 const unsigned full = smem_u32(&bars->v_full[s]), dst = smem_u32(sV + s * V_BYTES);
                 mbar_expect_tx(full, V_BYTES);
-                for (int d = 0; d < HD / 64; ++d) tma_load_2d(dst + d * (BN * 128), &map_v, full, d * 64, row);
+                for (int d = 0; d < HD / 64; ++d) load_rows(dst + d * (BN * 128), &map, full, d * 64, row, kv.v);
                 row = tile_row(j + 1);
             }
             if (has_failed(bars))
@@ -463,9 +463,9 @@ attn_shared_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
 
 template <int HD, bool FIXED>
 int launch(const SharedLaunch& a, cudaStream_t st) {
-    CUtensorMap map_k, map_v;
-    if (const int rc = make_map_bf16(&map_k, a.k_pool, a.pool_rows, HD, BN)) return rc;
-    if (const int rc = make_map_bf16(&map_v, a.v_pool, a.pool_rows, HD, BN)) return rc;
+    CUtensorMap map;
+    KV kv;
+    if (const int rc = make_pools_map(&map, &kv, a.k_pool, a.v_pool, a.pool_rows, HD, BN)) return rc;
     constexpr size_t layout = (size_t)k_stages(HD) * 2 * BN * HD * 2 + (size_t)v_stages(HD) * BN * HD * 2 + 2 * P_BYTES + sizeof(Barriers);
     static_assert(layout <= 227 * 1024, "a block's shared memory");
     const size_t smem = layout + 1024 < 227 * 1024 ? layout + 1024 : 227 * 1024;
@@ -475,7 +475,7 @@ int launch(const SharedLaunch& a, cudaStream_t st) {
     const long long items = (long long)a.sh.n_groups * a.sh.common_tiles * a.sh.common_ranges;
     if (items <= 0) return 0;
     if (items > 0x7fffffff) return QNN_ERR_UNSUPPORTED;
-    launch_pdl(kern, dim3((unsigned)items, a.nkv), dim3(THREADS), smem, st, map_k, map_v, (const bf16*)a.q, (size_t)a.q_stride, a.cells, a.sh, a.nq, a.nkv, a.sc,
+    launch_pdl(kern, dim3((unsigned)items, a.nkv), dim3(THREADS), smem, st, map, kv, (const bf16*)a.q, (size_t)a.q_stride, a.cells, a.sh, a.nq, a.nkv, a.sc,
                a.part_o, a.part_ml, a.status);
     return (int)cudaGetLastError();
 }

@@ -25,66 +25,103 @@ constexpr int SELECT_THREADS = 1024;
 constexpr int LIST = 2048;                    // places of the short list
 constexpr int MOST_REACHED = 512;             // segments that are looked at again
 
+// Segment `s` of a row starts at its logit s * SEGMENT - shift, shift the row's distance from a 16-byte boundary: segments then start on
+// one, and the row's first and last segments hold a few logits less.
+__device__ __forceinline__ int segment_start(const float* row, int s, int segment) { return s * segment - (int)(((uintptr_t)row >> 2) & 3); }
+
 // One maximum and sum per segment: warp w of the grid takes segments w, w + warps, ... of all rows, and asks for the next one's logits before it
 // works on those it has.  Whether all are finite is read off the maximum, the minimum and the sum; only where they are not does a
-// second look leave the others out.
+// second look leave the others out.  Exponentials are the fast ones of z - m: with the logit's distance d from the maximum they are off by at
+// most |d| 2^-23 + 2^-22, of weight e^d in the sum, which moves the sum's logarithm by less than 2^-20 however the logits lie.
+// Bound by memory, and by how much of it a short kernel keeps in flight: 80 rows of 255,029 (82 MB, 12.5 us at the copy rate), us, by segment and
+// loads: 512, 4 bytes a lane 21.5; 1024, 16 bytes 19.6; the same with the fast exponentials 17.3 (torch's amax alone: 24.7).
 template <int SEGMENT>
-__global__ void __launch_bounds__(256, 4)
+__global__ void __launch_bounds__(256, SEGMENT >= 1024 ? 2 : 4)
 beam_segments_kernel(const float* __restrict__ logits, int V, int segments, int total, float2* __restrict__ stats, int* __restrict__ error_flag) {
-    constexpr int PER = SEGMENT / 32;
+    constexpr int PER = SEGMENT / 128;                        // 16-byte pieces a lane
     pdl_wait();
     const int lane = threadIdx.x & 31, warps = gridDim.x * 8;
-    float ahead[PER];
-    auto ask = [&](int i) {
+    float4 ahead[PER];
+    const auto place = [&](int i, const float*& row) {
+        const int r = i / segments;
+        row = logits + (size_t)r * V;
+        return segment_start(row, i - r * segments, SEGMENT);
+    };
+    const auto ask = [&](int i) {
         if (i >= total) return;
-        const int r = i / segments, v0 = (i - r * segments) * SEGMENT;
-        const float* p = logits + (size_t)r * V + v0 + lane;
-        if (v0 + SEGMENT <= V) {
+        const float* row;
+        const int v0 = place(i, row);
+        if (v0 >= 0 && v0 + SEGMENT <= V) {
+            const float4* p = reinterpret_cast<const float4*>(row + v0) + lane;
 #pragma unroll
             for (int j = 0; j < PER; ++j) ahead[j] = p[j * 32];
-        } else {                                              // behind the row: its last logit again, taken out below
+        } else {                                              // outside the row: its nearest logit, taken out below
 #pragma unroll
-            for (int j = 0; j < PER; ++j) ahead[j] = p[min(j * 32, V - 1 - v0 - lane)];
+            for (int j = 0; j < PER; ++j) {
+                float x[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = row[min(max(v0 + (j * 32 + lane) * 4 + e, 0), V - 1)];
+                ahead[j] = make_float4(x[0], x[1], x[2], x[3]);
+            }
         }
     };
     int i = blockIdx.x * 8 + (threadIdx.x >> 5);
     ask(i);
     for (; i < total; i += warps) {
-        float z[PER];
-#pragma unroll
-        for (int j = 0; j < PER; ++j) z[j] = ahead[j];
-        ask(i + warps);
-        const int left = V - i % segments * SEGMENT;          // logits from the segment's first on
-        float m = -CUDART_INF_F, least = CUDART_INF_F;
+        float z[PER * 4];
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-            m = fmaxf(m, z[j]);
-            least = fminf(least, z[j]);
+            z[j * 4] = ahead[j].x;
+            z[j * 4 + 1] = ahead[j].y;
+            z[j * 4 + 2] = ahead[j].z;
+            z[j * 4 + 3] = ahead[j].w;
         }
-        if (left < SEGMENT) {
+        ask(i + warps);
+        const float* row;
+        const int v0 = place(i, row);
+        float m = -CUDART_INF_F, least = CUDART_INF_F;
+        if (v0 < 0 || v0 + SEGMENT > V) {
 #pragma unroll
-            for (int j = 0; j < PER; ++j)
-                if (j * 32 + lane >= left) z[j] = -CUDART_INF_F;
+            for (int j = 0; j < PER * 4; ++j) {
+                const int v = v0 + (j / 4 * 32 + lane) * 4 + j % 4;
+                if (v >= 0 && v < V) {
+                    m = fmaxf(m, z[j]);
+                    least = fminf(least, z[j]);
+                } else {
+                    z[j] = -CUDART_INF_F;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < PER * 4; ++j) {
+                m = fmaxf(m, z[j]);
+                least = fminf(least, z[j]);
+            }
         }
         m = warp_max(m);
         float s = 0.f;
 #pragma unroll
-        for (int j = 0; j < PER; ++j) s += expf(z[j] - m);
+        for (int j = 0; j < PER * 4; ++j) s += __expf(z[j] - m);
         s = warp_sum(s);
         if (__any_sync(0xffffffffu, least == -CUDART_INF_F) || !(s < CUDART_INF_F)) {      // (NaN, or an infinity in the maximum, make s a NaN)
-            m = -CUDART_INF_F;
+            float finite = -CUDART_INF_F;
+            bool bad = false;
 #pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                if (!isfinite(z[j])) z[j] = -CUDART_INF_F;
-                m = fmaxf(m, z[j]);
+            for (int j = 0; j < PER * 4; ++j) {
+                const int v = v0 + (j / 4 * 32 + lane) * 4 + j % 4;
+                if (!isfinite(z[j])) {
+                    bad = bad || (v >= 0 && v < V);
+                    z[j] = -CUDART_INF_F;
+                }
+                finite = fmaxf(finite, z[j]);
             }
-            m = warp_max(m);
+            m = warp_max(finite);
             s = 0.f;
             if (m != -CUDART_INF_F)
 #pragma unroll
-                for (int j = 0; j < PER; ++j) s += expf(z[j] - m);
+                for (int j = 0; j < PER * 4; ++j) s += __expf(z[j] - m);
             s = warp_sum(s);
-            if (lane == 0 && error_flag != nullptr) atomicOr(error_flag, 1);
+            if (__any_sync(0xffffffffu, bad) && lane == 0 && error_flag != nullptr) atomicOr(error_flag, 1);
         }
         if (lane == 0) stats[i] = make_float2(m, s);
     }
@@ -225,19 +262,20 @@ beam_pick_kernel(const float* __restrict__ logits, int V, int beams, int take, i
     for (int l = warp; l < n_look; l += WARPS) {
         const int i = n_reached <= MOST_REACHED ? reached[l] : l;
         if (best[i] < threshold) continue;
-        const int b = i / segments, v0 = (i - b * segments) * SEGMENT;
+        const int b = i / segments;
         const float* row = logits + (row0 + b) * V;
+        const int v0 = segment_start(row, i - b * segments, SEGMENT);
         const double add = base[b];
         // logits below this are out, whatever the roundings (most of them, and the others are looked at in 64 bits)
         const double exactly = (double)threshold_f - add;
         const float limit = threshold > 1u ? (float)(exactly - 1e-5 * (fabs(exactly) + fabs((double)threshold_f))) : -CUDART_INF_F;
         float z[SEGMENT / 32];
 #pragma unroll
-        for (int j = 0; j < SEGMENT / 32; ++j) z[j] = row[min(v0 + j * 32 + lane, V - 1)];
+        for (int j = 0; j < SEGMENT / 32; ++j) z[j] = row[min(max(v0 + j * 32 + lane, 0), V - 1)];
 #pragma unroll
         for (int j = 0; j < SEGMENT / 32; ++j) {
             const int v = v0 + j * 32 + lane;
-            if (v >= V || !isfinite(z[j]) || z[j] < limit) continue;
+            if (v < 0 || v >= V || !isfinite(z[j]) || z[j] < limit) continue;
             const double s = add + (double)z[j];
             if (ordered((float)s) < threshold) continue;
             const int at = atomicAdd(&n_found, 1);
@@ -278,11 +316,12 @@ beam_pick_kernel(const float* __restrict__ logits, int V, int beams, int take, i
         unsigned a_best = 0xffffffffu;
         for (int i = warp; i < n; i += SELECT_THREADS / 32) {
             if (best[i] < threshold) continue;
-            const int b = i / segments, v0 = (i - b * segments) * SEGMENT;
+            const int b = i / segments;
             const float* row = logits + (row0 + b) * V;
+            const int v0 = segment_start(row, i - b * segments, SEGMENT);
             for (int j = 0; j < SEGMENT / 32; ++j) {
                 const int v = v0 + j * 32 + lane;
-                if (v >= V) continue;
+                if (v < 0 || v >= V) continue;
                 const float z = row[v];
                 if (!isfinite(z)) continue;
                 const double s = base[b] + (double)z;
@@ -324,37 +363,39 @@ beam_pick_kernel(const float* __restrict__ logits, int V, int beams, int take, i
     }
 }
 
-// Logits per segment: small vocabularies get short ones, so that the threshold, the `take`-th best segment, stays near the best.
-int segment_of(int V) { return V >= 16384 ? 512 : 128; }
+// Logits per segment.  Small vocabularies get short ones, so that the threshold, the `take`-th best of 128 groups, stays near the best.
+// Where 512 would give every warp of the device several, 1024 keep more in flight.
+int least_segment(int V) { return V < 16384 ? 128 : 512; }
+int segment_of(int rows, int V) { return least_segment(V) == 512 && (long long)rows * V > 148LL * 32 * 512 ? 1024 : least_segment(V); }
+int segments_of(int V, int segment) { return (V + 3 + segment - 1) / segment; }
 
 }  // namespace
 
-QNN_API int qnn_beam_select_segments(int V) { return V <= 0 ? 0 : (V + segment_of(V) - 1) / segment_of(V); }
+// the most segments that a row is cut into, however many rows there are
+QNN_API int qnn_beam_select_segments(int V) { return V <= 0 ? 0 : segments_of(V, least_segment(V)); }
 
 // logits: [requests * beams, V] float32; scores: [requests * beams]; the outputs [requests, take].  Scratch: requests * beams *
 // qnn_beam_select_segments(V) float2.  take <= 64; beams * V < 2^32.
 QNN_API int qnn_beam_select(const float* logits, const float* scores, int requests, int beams, int V, int take, void* scratch, float* out_scores,
                             int* out_beams, int* out_tokens, const int* status_in, int* error_flag, cudaStream_t st) {
     if (requests <= 0) return 0;
-    if (beams < 1 || V < 1 || take < 1 || take > SELECT_MOST) return QNN_ERR_ARGUMENT;
+    if (beams < 1 || V < 1 || take < 1 || take > SELECT_MOST || ((uintptr_t)logits & 3)) return QNN_ERR_ARGUMENT;
     if ((long long)requests * beams > 65535 || (long long)beams * V >= 0xffffffffLL) return QNN_ERR_UNSUPPORTED;
-    const int segments = qnn_beam_select_segments(V);
+    const int rows = requests * beams, segment = segment_of(rows, V), segments = segments_of(V, segment);
     const size_t smem = sizeof(Found) + (size_t)beams * sizeof(double) + (size_t)beams * segments * sizeof(unsigned);
-    if (smem > 200 * 1024) return QNN_ERR_UNSUPPORTED;
-    const long long total = (long long)requests * beams * segments;
-    if (total > 0x7fffffff) return QNN_ERR_UNSUPPORTED;
-    const int wave = device_sms() * 4;        // blocks of the first kernel at a time
-    const int blocks = (int)((total + 7) / 8 < wave ? (total + 7) / 8 : wave);
+    if (smem > 200 * 1024 || (long long)rows * segments > 0x7fffffff) return QNN_ERR_UNSUPPORTED;
+    const int total = rows * segments, wave = device_sms() * (segment >= 1024 ? 2 : 4);       // blocks of the first kernel at a time
+    const int blocks = (total + 7) / 8 < wave ? (total + 7) / 8 : wave;
     float2* stats = (float2*)scratch;
 #define QNN_SELECT(SEG)                                                                                                                        \
     {                                                                                                                                          \
         static OncePerDevice asked;                                                                                                            \
         if (const int rc = allow_shared(asked, beam_pick_kernel<SEG>, 200 * 1024)) return rc;                                                  \
-        launch_pdl(beam_segments_kernel<SEG>, dim3(blocks), dim3(256), 0, st, logits, V, segments, (int)total, stats, error_flag);                                 \
+        launch_pdl(beam_segments_kernel<SEG>, dim3(blocks), dim3(256), 0, st, logits, V, segments, total, stats, error_flag);                  \
         launch_pdl(beam_pick_kernel<SEG>, dim3(requests), dim3(SELECT_THREADS), smem, st, logits, V, beams, take, segments, scores,             \
                    (const float2*)stats, out_scores, out_beams, out_tokens, status_in, error_flag);                                            \
     }
-    if (segment_of(V) == 512) QNN_SELECT(512) else QNN_SELECT(128)
+    if (segment == 1024) QNN_SELECT(1024) else if (segment == 512) QNN_SELECT(512) else QNN_SELECT(128)
 #undef QNN_SELECT
     QNN_LAUNCH_CHECK();
 }

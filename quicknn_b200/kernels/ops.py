@@ -2360,23 +2360,31 @@ def shared_attention_plan(dtype: torch.dtype, n_rows: int, n_heads: int, n_kv: i
         keys, own = max(shared.keys, 1), max(shared.own, 1)
         if window:
             keys, own = min(keys, window), min(own, window)
-        resident = _sm_count("cuda") * max(1, min(8, 512 // head_dim))       # CTAs at a time
-        common = shared.n_groups * (-(-shared.rows * heads // tile)) * n_kv         # walks over common keys
+        sms = _sm_count("cuda")
+        resident = sms * max(1, min(8, 512 // head_dim))                                   # CTAs at a time
+        common = shared.n_groups * (-(-shared.rows * heads // tile)) * n_kv                # walks over common keys
         alone = n_rows * (-(-heads // tile)) * n_kv                                        # walks over own keys
-        best = None
-        for c in _SHARED_CHUNKS:
-            s, p = -(-keys // c), -(-own // c)
-            if s > 64 or p > 64:
-                continue
-            items = common * s + alone * p
-            longest = max(-(-keys // s) if common else 0, -(-own // p))
-            t = longest + SHARED_ITEM_COST
-            if items > resident:
-                t = max(t, (common * (keys + s * SHARED_ITEM_COST) + alone * (own + p * SHARED_ITEM_COST)) / resident + longest / 2)
-            t += 2.0 * n_rows * n_heads * (s + p) / resident                               # the parts, written and read as float32
-            if best is None or t < best[0] * 0.999:
-                best = (t, s, p)
-        ranges = best[1:]
+        # the times below are in keys of a walk; the parts are written and read as float32
+        parts = 2.0 * n_rows * n_heads / resident
+        if tile >= 128:
+            # two kernels: common keys by CTAs that have an SM each and start as late as 800 keys, own keys by small ones
+            s = min(range(1, 65), key=lambda n: -(-common * n // sms) * (-(-keys // n) + 800.0) + parts * n)
+            p = min(range(1, 65), key=lambda n: _spread(alone * n, resident, own / n) + parts * n)
+            ranges = (min(s, -(-keys // 64)), p)
+        else:
+            best = None
+            for c in _SHARED_CHUNKS:
+                s, p = -(-keys // c), -(-own // c)
+                if s > 64 or p > 64:
+                    continue
+                longest = max(-(-keys // s) if common else 0, -(-own // p))
+                t = longest + SHARED_ITEM_COST
+                if common * s + alone * p > resident:
+                    t = max(t, (common * (keys + s * SHARED_ITEM_COST) + alone * (own + p * SHARED_ITEM_COST)) / resident + longest / 2)
+                t += parts * (s + p)
+                if best is None or t < best[0] * 0.999:
+                    best = (t, s, p)
+            ranges = best[1:]
     s, p = ranges
     if s < 1 or p < 1 or s + p > 128:
         raise ValueError("shared attention: at least one range of each kind, and at most 128 together")
@@ -2391,6 +2399,12 @@ def shared_attention_pays(dtype: torch.dtype, n_heads: int, n_kv: int, head_dim:
 _SHARED_CHUNKS = tuple(sorted({16 * int(round(2 ** (i / 2))) for i in range(4, 28)}))       # 64 keys .. 128 K
 
 
+def _spread(items: int, resident: int, keys: float) -> float:
+    """Time of so many CTAs of so many keys at most each, in keys: at once, or filling the device evenly with half a CTA at the end."""
+    t = keys + SHARED_ITEM_COST
+    return t if items <= resident else max(t, items * t / resident + keys / 2)
+
+
 def _on_current_device(*ts: torch.Tensor) -> None:
     here = torch.cuda.current_device()
     for t in ts:
@@ -2398,15 +2412,10 @@ def _on_current_device(*ts: torch.Tensor) -> None:
             raise ValueError(f"a tensor is on {t.device}, the current device is cuda:{here}")
 
 
-def attn_decode_shared(qkv: torch.Tensor, n_heads: int, n_kv: int, head_dim: int, k_pool: torch.Tensor, v_pool: torch.Tensor,
-                       page_table: torch.Tensor, page_size: int, ring: int, slots: torch.Tensor, slot_len: torch.Tensor,
-                       shared: SharedKeys, scale: float, cap: Optional[float], window: Optional[int], plan: SharedPlan,
-                       scratch: torch.Tensor, slopes: Optional[torch.Tensor] = None, sinks: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """``attn_decode`` for rows that share pages: the same results up to rounding, with the keys that a group's rows hold in the same
-    pages (and all see) read once for the group.  ``plan`` comes from ``shared_attention_plan``; ``scratch`` (uint8 or float32, 16-byte
-    aligned) holds ``plan.scratch_bytes`` and is overwritten.  ``slots``, ``slot_len``, ``page_table`` and what ``shared`` holds must be
-    complete before the kernel that runs just before this one on the stream starts, as for ``attn_decode``."""
-    ld = _rows(qkv, "qkv")
+def _check_shared(qkv, n_heads, n_kv, head_dim, k_pool, v_pool, page_table, page_size, ring, slots, slot_len, shared, window, plan, scratch,
+                  slopes, sinks) -> None:
+    """The checks of ``attn_decode_shared`` one by one, each with its message."""
+    _rows(qkv, "qkv")
     _check_per_head(slopes, sinks, n_heads)
     B = qkv.shape[0]
     _req(k_pool, "k_pool", qkv.dtype, 4)
@@ -2431,9 +2440,34 @@ def attn_decode_shared(qkv: torch.Tensor, n_heads: int, n_kv: int, head_dim: int
     if scratch.numel() * scratch.element_size() < plan.scratch_bytes or plan.scratch_bytes < B * n_heads * (plan.common_ranges + plan.own_ranges) * (head_dim + 2) * 4:
         raise ValueError("shared attention: scratch is too small for the plan, or the plan for the batch")
     _on_current_device(qkv, k_pool, v_pool, page_table, slots, slot_len, shared.groups, shared.row_group, scratch)
-    out = torch.empty((B, n_heads * head_dim), dtype=qkv.dtype, device=qkv.device)
+
+
+def attn_decode_shared(qkv: torch.Tensor, n_heads: int, n_kv: int, head_dim: int, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                       page_table: torch.Tensor, page_size: int, ring: int, slots: torch.Tensor, slot_len: torch.Tensor,
+                       shared: SharedKeys, scale: float, cap: Optional[float], window: Optional[int], plan: SharedPlan,
+                       scratch: torch.Tensor, slopes: Optional[torch.Tensor] = None, sinks: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``attn_decode`` for rows that share pages: the same results up to rounding, with the keys that a group's rows hold in the same
+    pages (and all see) read once for the group.  ``plan`` comes from ``shared_attention_plan``; ``scratch`` (uint8 or float32, 16-byte
+    aligned) holds ``plan.scratch_bytes`` and is overwritten.  ``slots``, ``slot_len``, ``page_table`` and what ``shared`` holds must be
+    complete before the kernel that runs just before this one on the stream starts, as for ``attn_decode``."""
+    B, width = qkv.shape if qkv.dim() == 2 else (0, 0)
+    parts = B * n_heads * (plan.common_ranges + plan.own_ranges)
+    dt, here, i32, pools, table = qkv.dtype, _raw_device(), torch.int32, k_pool.shape, page_table.shape
+    ok = (slopes is None and sinks is None and not ring and window is None and n_kv > 0 and n_heads % n_kv == 0 and pools == v_pool.shape
+          and pools[1:] == (n_kv, page_size, head_dim) and k_pool.dtype is dt and v_pool.dtype is dt and width >= n_heads * head_dim
+          and qkv.stride(1) == 1 and qkv.stride(0) >= width and slots.numel() == B == shared.row_group.numel() and slot_len.numel() == table[0]
+          and len(table) == 2 and scratch.numel() * scratch.element_size() >= plan.scratch_bytes >= parts * (head_dim + 2) * 4
+          and page_table.dtype is i32 and slots.dtype is i32 and slot_len.dtype is i32)
+    if ok:
+        for t in (k_pool, v_pool, page_table, slots, slot_len, scratch, shared.groups, shared.row_group):
+            ok = ok and t.get_device() == here and t.is_contiguous()
+    if not ok or qkv.get_device() != here:                   # what is not so plain is looked at one by one
+        _check_shared(qkv, n_heads, n_kv, head_dim, k_pool, v_pool, page_table, page_size, ring, slots, slot_len, shared, window, plan, scratch, slopes,
+                      sinks)
+    ld = qkv.stride(0) if B > 1 else max(qkv.stride(0), width)
+    out = qkv.new_empty((B, n_heads * head_dim))
     part_o = scratch.data_ptr()
-    part_ml = part_o + B * n_heads * (plan.common_ranges + plan.own_ranges) * head_dim * 4
+    part_ml = part_o + parts * head_dim * 4
     _lib.check(_lib.load().qnn_attn_decode_shared(
         _p(qkv), ld, dt_code(qkv), _p(k_pool), _p(v_pool), _p(page_table), page_table.shape[1], page_size, ring, _p(slots), _p(slot_len), B,
         _p(shared.groups), shared.groups.shape[0], shared.rows, _p(shared.row_group), n_heads, n_kv, head_dim, float(scale), float(cap or 0.0),
@@ -2446,7 +2480,7 @@ BEAM_MOST = 64                   # continuations per request that beam_select re
 
 
 def beam_select_scratch_bytes(rows: int, vocab: int, take: int) -> int:
-    """Scratch of ``beam_select`` for so many rows (requests x beams)."""
+    """Scratch of ``beam_select`` for so many rows (requests x beams) or fewer."""
     if not 1 <= take <= BEAM_MOST:
         raise ValueError(f"beam selection returns 1..{BEAM_MOST} continuations per request, not {take}")
     return 8 * rows * int(_lib.load().qnn_beam_select_segments(vocab))

@@ -57,6 +57,25 @@ def test_against_a_sort(Q, W, V, take):
     check(*data(Q, W, V, Q + W + V), W, take)
 
 
+def test_scratch_of_many_rows_serves_fewer():
+    V, most = 65537, 64
+    scratch = torch.empty(ops.beam_select_scratch_bytes(most, V, 8), dtype=torch.uint8, device=DEV)
+    for Q in (16, 9, 8, 4, 1):
+        logits, scores = data(Q, 4, V, Q)
+        got, want = ops.beam_select(logits, scores, 4, 8, scratch), wanted(logits, scores, 4, 8)
+        assert np.array_equal(got[1].cpu().numpy(), want[1]) and np.array_equal(got[2].cpu().numpy(), want[2])
+
+
+def test_rows_off_sixteen_bytes():
+    for V in (257, 16387, 255029):
+        flat = torch.randn(4 * V + 5, device=DEV, generator=torch.Generator(device=DEV).manual_seed(V))
+        for off in range(4):
+            x = flat[off:off + 4 * V].view(4, V)
+            x[:, 0] += 9 * (off % 2)                                # the first and the last of a row among the best
+            x[:, V - 1] += 9
+            check(x, torch.tensor([-1.0, -1.5, -1.2, -3.0], device=DEV), 2, 6)
+
+
 def test_equal_scores_go_to_the_lowest_beam_and_token():
     logits, scores = data(2, 4, 3000, 1)
     logits = logits.round()                                         # many equal ones
