@@ -259,29 +259,39 @@ __device__ __forceinline__ void walk(const Item& it, int queries, const CUtensor
         }
     }
     __syncthreads();
-    for (int m = warp; m < queries; m += WARPS) {             // a warp per query
-        float mm = -CUDART_INF_F, coef[WARPS], ll = 0.f;
+    // lane m has query m's weights and place; then a warp per query, several on their way
+    float coef[WARPS];
+    size_t at = 0;
+    if (lane < queries) {
+        float mm = -CUDART_INF_F, ll = 0.f;
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) mm = fmaxf(mm, ms[((size_t)w * QT + m) * ROW + HD]);
+        for (int w = 0; w < WARPS; ++w) mm = fmaxf(mm, ms[((size_t)w * QT + lane) * ROW + HD]);
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
-            const float mw = ms[((size_t)w * QT + m) * ROW + HD], lw = ms[((size_t)w * QT + m) * ROW + HD + 1];
+            const float mw = ms[((size_t)w * QT + lane) * ROW + HD], lw = ms[((size_t)w * QT + lane) * ROW + HD + 1];
             coef[w] = mw == -CUDART_INF_F ? (lw != lw ? lw : 0.f) : exp2_fast(mw - mm);
             ll += coef[w] * lw;
         }
-        const size_t at = part_of(it, sh, it.query0 + m, kh, G, nq);
+        at = part_of(it, sh, it.query0 + lane, kh, G, nq);
+        if (warp == 0) part_ml[at] = make_float2(mm, ll);
+    }
+#pragma unroll 4
+    for (int m = warp; m < queries; m += WARPS) {
+        float c[WARPS];
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) c[w] = __shfl_sync(0xffffffffu, coef[w], m);
+        float* dst = part_o + __shfl_sync(0xffffffffu, (unsigned long long)at, m) * HD;
 #pragma unroll
         for (int d = lane * 2; d < HD; d += 64) {
             float2 acc = make_float2(0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) {
                 const float2 v = *reinterpret_cast<const float2*>(ms + ((size_t)w * QT + m) * ROW + d);
-                acc.x += coef[w] * v.x;
-                acc.y += coef[w] * v.y;
+                acc.x += c[w] * v.x;
+                acc.y += c[w] * v.y;
             }
-            *reinterpret_cast<float2*>(part_o + at * HD + d) = acc;
+            *reinterpret_cast<float2*>(dst + d) = acc;
         }
-        if (lane == 0) part_ml[at] = make_float2(mm, ll);
     }
 }
 
@@ -472,7 +482,7 @@ attn_shared_join_kernel(const float* __restrict__ part_o, const float2* __restri
         const int p = k * 32 + lane;
         ml[k] = p >= from && p < parts ? part_ml[at + p] : make_float2(-CUDART_INF_F, 0.f);
     }
-    constexpr int AHEAD = 4;
+    constexpr int AHEAD = PIECES <= 2 ? 8 : 4;
     float4 v[AHEAD][PIECES];
     const auto ask = [&](int p0) {
 #pragma unroll
