@@ -297,11 +297,14 @@ __device__ __forceinline__ void walk(const Item& it, int queries, const CUtensor
 
 // Items: those of C first (group, tile of queries, range; the range fastest), then the rows' own (row, tile of heads, range).  NT: column tiles
 // of an item of C; a row's own heads take one where they fit it.
-template <int HD, int NT, bool BIAS>
+// BESIDE: the kernel in front is that of the groups' common keys (attention_shared_tcgen05.cu), which nothing here depends on.  Its CTAs have
+// all waited for what is in front of them before this kernel can start, so the queries are there and the scratch is free.  One CTA waits
+// for it at its end, so that this kernel is over only when that one is.
+template <int HD, int NT, bool BIAS, bool BESIDE>
 __global__ void __launch_bounds__(WARPS * 32)
 attn_shared_mma_kernel(const __grid_constant__ CUtensorMap map, const KV kv, const bf16* __restrict__ q, size_t q_stride,
-                       const Cells cells, const Shared sh, int common_items, int own_tile, int nq, int nkv, const Scores sc, float* __restrict__ part_o,
-                       float2* __restrict__ part_ml, int* __restrict__ status) {
+                       const Cells cells, const Shared sh, int common_items, int own_tile, int nq, int nkv, const Scores sc,
+                       float* __restrict__ part_o, float2* __restrict__ part_ml, int* __restrict__ status) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     const unsigned bars = tc::smem_u32(smem) + Layout<HD>::ring_bytes(NT);
@@ -327,16 +330,22 @@ attn_shared_mma_kernel(const __grid_constant__ CUtensorMap map, const KV kv, con
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncthreads();
-    pdl_wait();
-    if (queries <= 0) return;
+    if (!BESIDE) pdl_wait();
+    const bool last = BESIDE && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1;
+    if (queries <= 0) {
+        if (last) pdl_wait();
+        return;
+    }
     if (it.t0 >= it.t1) {                                     // a range without keys
         for (int m = threadIdx.x; m < queries; m += blockDim.x) part_ml[part_of(it, sh, it.query0 + m, kh, G, nq)] = make_float2(-CUDART_INF_F, 0.f);
+        if (last) pdl_wait();
         return;
     }
     if (NT > 1 && own && own_tile == 8)
         walk<HD, 1, BIAS>(it, queries, map, kv, q, q_stride, cells, sh, kh, nq, nkv, sc, part_o, part_ml, status, smem, pages, first_page, bars);
     else
         walk<HD, NT, BIAS>(it, queries, map, kv, q, q_stride, cells, sh, kh, nq, nkv, sc, part_o, part_ml, status, smem, pages, first_page, bars);
+    if (last) pdl_wait();
 }
 
 // ---- any head size, float32 or bfloat16 ----------------------------------------------------------------------------------------
@@ -574,23 +583,34 @@ bool many_rows(int dtype, int hd, int queries) { return on_tensor_cores(dtype, h
 // elements are 192 registers a thread).
 int column_tiles(int hd, int queries) { return queries <= 8 ? 1 : (queries <= 16 || hd > 128 ? 2 : 4); }
 
-template <int HD, int NT, bool BIAS>
+template <int HD, int NT, bool BIAS, bool BESIDE>
 int launch_mma(const void* q, long long q_stride, const void* k_pool, const void* v_pool, long long pool_rows, const Cells& cells, const Shared& sh,
-               bool with_common, int B, int nq, int nkv, const Scores& sc, float* part_o, float2* part_ml, int* status, cudaStream_t st) {
+               int B, int nq, int nkv, const Scores& sc, float* part_o, float2* part_ml, int* status, cudaStream_t st) {
     const int G = nq / nkv, own_tile = G <= 8 ? 8 : 8 * NT;
-    const long long common = with_common ? (long long)sh.n_groups * sh.common_tiles * sh.common_ranges : 0, own = (long long)B * ((G + own_tile - 1) / own_tile) * sh.own_ranges;
+    const long long common = BESIDE ? 0 : (long long)sh.n_groups * sh.common_tiles * sh.common_ranges, own = (long long)B * ((G + own_tile - 1) / own_tile) * sh.own_ranges;
     if (common + own > 0x7fffffff) return QNN_ERR_UNSUPPORTED;
     const size_t smem = 1024 + Layout<HD>::ring_bytes(NT) + Layout<HD>::BARRIERS + ((size_t)cells.max_pages + 2) * sizeof(int);
     if (smem > 220 * 1024) return QNN_ERR_UNSUPPORTED;
     CUtensorMap map;
     KV kv;
     if (const int rc = make_pools_map(&map, &kv, k_pool, v_pool, pool_rows, HD, TILE)) return rc;
-    auto kern = attn_shared_mma_kernel<HD, NT, BIAS>;
+    auto kern = attn_shared_mma_kernel<HD, NT, BIAS, BESIDE>;
     static OncePerDevice asked;
     if (const int rc = allow_shared(asked, kern, 220 * 1024)) return rc;
-    launch_pdl(kern, dim3((unsigned)(common + own), nkv), dim3(WARPS * 32), smem, st, map, kv, (const bf16*)q, (size_t)q_stride, cells, sh, (int)common,
-               own_tile, nq, nkv, sc, part_o, part_ml, status);
-    return (int)cudaGetLastError();
+    // (beside the kernel of the common keys also where the grid is larger than others are launched early with)
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(common + own), nkv);
+    cfg.blockDim = dim3(WARPS * 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = (BESIDE && pdl_enabled()) || (pdl_enabled() && (common + own) * nkv <= pdl_max_grid()) ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, map, kv, (const bf16*)q, (size_t)q_stride, cells, sh, (int)common, own_tile, nq, nkv, sc,
+                                             part_o, part_ml, status);
+    return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
 
 template <typename T, int DPL>
@@ -650,7 +670,7 @@ QNN_API int qnn_attn_decode_shared(const void* q, long long q_stride, int dtype,
     if (page_size < 16 || (page_size & (page_size - 1)) || ring < 0 || ring % page_size) return QNN_ERR_ARGUMENT;
     if (ring > 0 && (window <= 0 || window > ring || ring / page_size > max_pages)) return QNN_ERR_ARGUMENT;   // a ring holds no more
     const int G = nq / nkv, esize = dtype == QNN_DT_BF16 ? 2 : 4;
-    const bool many = page_size >= 64 && many_rows(dtype, hd, most_rows * G);
+    const bool many = n_groups > 0 && page_size >= 64 && many_rows(dtype, hd, most_rows * G);
     const int tile = many ? MANY_TILE : (on_tensor_cores(dtype, hd) ? 8 * column_tiles(hd, most_rows * G) : qnn_attn_shared_tile(dtype, hd, most_rows * G));
     if (tile <= 0) return QNN_ERR_UNSUPPORTED;
     if ((q_stride * esize) % 16 || ((uintptr_t)q & 15) || ((uintptr_t)k_pool & 15) || ((uintptr_t)v_pool & 15) || ((uintptr_t)part_o & 15) ||
@@ -672,13 +692,14 @@ QNN_API int qnn_attn_decode_shared(const void* q, long long q_stride, int dtype,
             if (const int err = launch_common_tcgen05(a, st)) return err;
         }
         const int nt = many ? column_tiles(hd, G) : tile / 8;
+#define QNN_MMA_AS(HDV, NTV, BIAS, BESIDE) launch_mma<HDV, NTV, BIAS, BESIDE>(q, q_stride, k_pool, v_pool, pool_rows, cells, sh, B, nq, nkv, sc, part_o, ml, status, st)
 #define QNN_MMA(HDV, NTV)                                                                                                                       \
     if (hd == HDV && nt == NTV)                                                                                                                  \
-        rc = slopes != nullptr                                                                                                                   \
-                 ? launch_mma<HDV, NTV, true>(q, q_stride, k_pool, v_pool, pool_rows, cells, sh, !many, B, nq, nkv, sc, part_o, ml, status, st)   \
-                 : launch_mma<HDV, NTV, false>(q, q_stride, k_pool, v_pool, pool_rows, cells, sh, !many, B, nq, nkv, sc, part_o, ml, status, st);
+        rc = slopes != nullptr ? (many ? QNN_MMA_AS(HDV, NTV, true, true) : QNN_MMA_AS(HDV, NTV, true, false))                                   \
+                               : (many ? QNN_MMA_AS(HDV, NTV, false, true) : QNN_MMA_AS(HDV, NTV, false, false));
         QNN_MMA(64, 1) QNN_MMA(64, 2) QNN_MMA(64, 4) QNN_MMA(128, 1) QNN_MMA(128, 2) QNN_MMA(128, 4) QNN_MMA(256, 1) QNN_MMA(256, 2)
 #undef QNN_MMA
+#undef QNN_MMA_AS
     } else {
 #define QNN_GENERIC(T, DPLV) \
     launch_generic<T, DPLV>(q, q_stride, k_pool, v_pool, cells, sh, (int)items, nq, nkv, hd, scale, cap, part_o, ml, slopes, st)

@@ -27,8 +27,9 @@ constexpr int P_BYTES = BM * BN * 2;
 constexpr int S_COL = 0, O_COL = 128;         // tensor-memory columns of S (two halves of 64) and of O; Q follows O
 constexpr float STEP = 8.f;                   // how far (in e) a maximum may rise before O is rescaled
 constexpr int POLY = 4;                       // of every 8 exponentials, those taken on the FMA pipe (with a softcap)
-__host__ __device__ constexpr int k_stages(int hd) { return hd >= 256 ? 2 : (hd >= 128 ? 3 : 4); }       // pairs of pages
-__host__ __device__ constexpr int v_stages(int hd) { return hd >= 256 ? 2 : (hd >= 128 ? 4 : 6); }       // pages
+// Depth of the rings.  Up to head size 128 they leave room for a CTA of the rows' own keys on the same SM.
+__host__ __device__ constexpr int k_stages(int hd) { return hd >= 128 ? 2 : 4; }                        // pairs of pages
+__host__ __device__ constexpr int v_stages(int hd) { return hd >= 256 ? 2 : (hd >= 128 ? 3 : 6); }       // pages
 
 // D[tmem] (+)= A[tmem] B[smem]
 __device__ __forceinline__ void umma_a_tmem(unsigned tmem_d, unsigned tmem_a, uint64_t bdesc, unsigned idesc, unsigned accumulate) {
@@ -108,6 +109,8 @@ attn_shared_tcgen05_kernel(const __grid_constant__ CUtensorMap map, const KV kv,
     constexpr int KP_BYTES = 2 * BN * HD * 2, V_BYTES = BN * HD * 2;
     constexpr int Q_COL = O_COL + HD;                                // HD / 2 columns, two bfloat16 each
     constexpr int TMEM_COLS = HD > 64 ? 512 : 256;
+    constexpr int BLOCKS = HD / 64, Q_GROUPS = BLOCKS > 1 ? 2 : 1;    // both softmax groups bring queries, alternate blocks of 64 elements
+    static_assert(BM * HD * 4 <= KS * KP_BYTES, "the results are staged in the K ring");
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     unsigned char* sK = smem;
@@ -132,7 +135,7 @@ attn_shared_tcgen05_kernel(const __grid_constant__ CUtensorMap map, const KV kv,
         return;
     }
     if (threadIdx.x == 0) {
-        mbar_init(smem_u32(&bars->q_tmem), 4);
+        mbar_init(smem_u32(&bars->q_tmem), 4 * Q_GROUPS);
         for (int s = 0; s < KS; ++s) {
             mbar_init(smem_u32(&bars->k_full[s]), 1);
             mbar_init(smem_u32(&bars->k_empty[s]), 1);
@@ -255,17 +258,22 @@ attn_shared_tcgen05_kernel(const __grid_constant__ CUtensorMap map, const KV kv,
         bool alive = true;
         const int m = it.query0 + rloc, row = it.row0 + m / G, head = kh * G + m % G;
         const bool have = rloc < queries;
-        if (group == 0) {
+        if (group < Q_GROUPS) {
+            constexpr int MINE = BLOCKS / Q_GROUPS;
             const uint4* src = reinterpret_cast<const uint4*>(q + (have ? (size_t)row * q_stride + (size_t)head * HD : 0));
-#pragma unroll 1
-            for (int d = 0; d < HD / 64; ++d) {
+            uint4 w[MINE][8];
+#pragma unroll
+            for (int i = 0; i < MINE; ++i)
+#pragma unroll
+                for (int c = 0; c < 8; ++c) w[i][c] = have ? src[(i * Q_GROUPS + group) * 8 + c] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+            for (int i = 0; i < MINE; ++i) {
                 uint32_t v[32];
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
-                    const uint4 w = have ? src[d * 8 + c] : make_uint4(0u, 0u, 0u, 0u);
-                    v[c * 4 + 0] = w.x; v[c * 4 + 1] = w.y; v[c * 4 + 2] = w.z; v[c * 4 + 3] = w.w;
+                    v[c * 4 + 0] = w[i][c].x; v[c * 4 + 1] = w[i][c].y; v[c * 4 + 2] = w[i][c].z; v[c * 4 + 3] = w[i][c].w;
                 }
-                tmem_st32(lane_base + Q_COL + d * 32, v);
+                tmem_st32(lane_base + Q_COL + (i * Q_GROUPS + group) * 32, v);
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
@@ -441,16 +449,32 @@ attn_shared_tcgen05_kernel(const __grid_constant__ CUtensorMap map, const KV kv,
                 if (!FIXED && nt > 1) l_other *= exp2_fast((m_second[rloc] - m_used) * k2);
                 part_ml[at] = make_float2(FIXED ? 0.f : m_used * k2, l_sum + l_other);
             }
-            // the groups write half of the head each
+            // Half of the head by each group, through the K ring (16-byte pieces XOR-ed with the row), so that whole rows are written.
             constexpr int HALF = HD / 2;
+            unsigned char* const mine = sK + rloc * (HD * 4);
 #pragma unroll 1
             for (int c0 = group * HALF; c0 < (group + 1) * HALF; c0 += 32) {
                 uint32_t v[32];
                 tmem_ld32_sync(lane_base + O_COL + c0, v);
-                if (have)
 #pragma unroll
-                    for (int c = 0; c < 32; c += 4)
-                        *reinterpret_cast<uint4*>(part_o + at * HD + c0 + c) = make_uint4(v[c], v[c + 1], v[c + 2], v[c + 3]);
+                for (int c = 0; c < 32; c += 4)
+                    *reinterpret_cast<uint4*>(mine + (((c0 + c) / 4 ^ (rloc & 7)) << 4)) = make_uint4(v[c], v[c + 1], v[c + 2], v[c + 3]);
+            }
+        }
+        asm volatile("bar.sync 2, 256;" ::: "memory");
+        if (alive) {
+            constexpr int CPR = HD / 4, RPI = CPR < 32 ? 32 / CPR : 1, PPR = CPR < 32 ? 1 : CPR / 32;       // pieces of a row; rows, pieces per lane at a time
+            const int first_row = (warp - 2) * 16;                   // each of the eight warps writes sixteen rows
+#pragma unroll 4
+            for (int rr = 0; rr < 16; rr += RPI) {
+                const int r = first_row + rr + (CPR < 32 ? lane / CPR : 0);
+                if (r >= queries) continue;
+                float* dst = part_o + part_of(it, sh, it.query0 + r, kh, G, nq) * HD;
+#pragma unroll
+                for (int i = 0; i < PPR; ++i) {
+                    const int c = i * 32 + lane % (CPR < 32 ? CPR : 32);
+                    *reinterpret_cast<uint4*>(dst + c * 4) = *reinterpret_cast<const uint4*>(sK + r * (HD * 4) + ((c ^ (r & 7)) << 4));
+                }
             }
         }
     }

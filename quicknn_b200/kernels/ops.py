@@ -2367,9 +2367,13 @@ def shared_attention_plan(dtype: torch.dtype, n_rows: int, n_heads: int, n_kv: i
         # the times below are in keys of a walk; the parts are written and read as float32
         parts = 2.0 * n_rows * n_heads / resident
         if tile >= 128:
-            # two kernels: common keys by CTAs that have an SM each and start as late as 800 keys, own keys by small ones
-            s = min(range(1, 65), key=lambda n: -(-common * n // sms) * (-(-keys // n) + 800.0) + parts * n)
+            # Two kernels side by side: common keys by CTAs that take most of an SM (a quarter of a walk's time per key, from 200 on), own keys
+            # by small ones on what is left, bound by memory.  As few of the former as are done in time; where own keys are few, as many
+            # as make them short.
             p = min(range(1, 65), key=lambda n: _spread(alone * n, resident, own / n) + parts * n)
+            time = _spread(alone * p, resident, own / p)
+            walk = lambda n: -(-common * n // sms) * (0.25 * (-(-keys // n)) + 200.0)  # noqa: E731
+            s = next((n for n in range(1, 9) if walk(n) <= 0.6 * time), 0) or min(range(1, 65), key=lambda n: walk(n) + parts * n)
             ranges = (min(s, -(-keys // 64)), p)
         else:
             best = None
