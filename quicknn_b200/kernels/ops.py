@@ -43,6 +43,7 @@ def _p(t: Optional[torch.Tensor]):
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _raw_device = getattr(torch._C, "_cuda_getDevice", None)
+_here = _raw_device or torch.cuda.current_device        # the current device's number
 
 
 def _stream():
@@ -2319,7 +2320,7 @@ class SharedKeys:
     a row's group, or -1.  ``rows``, ``keys`` and ``own`` bound the rows of a group, the positions of a group and the keys that a row has
     beside them: host numbers, from which the work is divided (``rows`` must hold; the others are a matter of speed)."""
 
-    __slots__ = ("groups", "row_group", "rows", "keys", "own")
+    __slots__ = ("groups", "row_group", "n_groups", "rows", "keys", "own")
 
     def __init__(self, groups: torch.Tensor, row_group: torch.Tensor, *, rows: int, keys: int, own: int):
         _req(groups, "groups", torch.int32, 2)
@@ -2329,10 +2330,7 @@ class SharedKeys:
         if rows < 0 or keys < 0 or own < 0 or (groups.shape[0] and rows < 1):
             raise ValueError("shared keys: bounds of rows and keys cannot be negative, and a group has a row")
         self.groups, self.row_group, self.rows, self.keys, self.own = groups, row_group, int(rows), int(keys), int(own)
-
-    @property
-    def n_groups(self) -> int:
-        return self.groups.shape[0]
+        self.n_groups = groups.shape[0]
 
 
 class SharedPlan(NamedTuple):
@@ -2341,6 +2339,7 @@ class SharedPlan(NamedTuple):
     common_ranges: int
     own_ranges: int
     scratch_bytes: int
+    kernels: int = 2             # launches of a call
 
 
 SHARED_ITEM_COST = 64.0          # what a CTA of that attention costs beside its keys, in keys
@@ -2392,7 +2391,7 @@ def shared_attention_plan(dtype: torch.dtype, n_rows: int, n_heads: int, n_kv: i
     s, p = ranges
     if s < 1 or p < 1 or s + p > 128:
         raise ValueError("shared attention: at least one range of each kind, and at most 128 together")
-    return SharedPlan(s, p, max(n_rows, 1) * n_heads * (s + p) * (head_dim + 2) * 4)
+    return SharedPlan(s, p, max(n_rows, 1) * n_heads * (s + p) * (head_dim + 2) * 4, 3 if tile >= 128 else 2)
 
 
 def shared_attention_pays(dtype: torch.dtype, n_heads: int, n_kv: int, head_dim: int, shared, window: Optional[int] = None) -> bool:
@@ -2456,11 +2455,11 @@ def attn_decode_shared(qkv: torch.Tensor, n_heads: int, n_kv: int, head_dim: int
     complete before the kernel that runs just before this one on the stream starts, as for ``attn_decode``."""
     B, width = qkv.shape if qkv.dim() == 2 else (0, 0)
     parts = B * n_heads * (plan.common_ranges + plan.own_ranges)
-    dt, here, i32, pools, table = qkv.dtype, _raw_device(), torch.int32, k_pool.shape, page_table.shape
-    ok = (slopes is None and sinks is None and not ring and window is None and n_kv > 0 and n_heads % n_kv == 0 and pools == v_pool.shape
+    dt, here, i32, pools, table = qkv.dtype, _here(), torch.int32, k_pool.shape, page_table.shape
+    ok = (slopes is None and sinks is None and (not ring or 0 < (window or 0) <= ring <= table[1] * page_size) and n_kv > 0 and n_heads % n_kv == 0 and pools == v_pool.shape
           and pools[1:] == (n_kv, page_size, head_dim) and k_pool.dtype is dt and v_pool.dtype is dt and width >= n_heads * head_dim
           and qkv.stride(1) == 1 and qkv.stride(0) >= width and slots.numel() == B == shared.row_group.numel() and slot_len.numel() == table[0]
-          and len(table) == 2 and scratch.numel() * scratch.element_size() >= plan.scratch_bytes >= parts * (head_dim + 2) * 4
+          and (window or 0) >= 0 and len(table) == 2 and scratch.numel() * scratch.element_size() >= plan.scratch_bytes >= parts * (head_dim + 2) * 4
           and page_table.dtype is i32 and slots.dtype is i32 and slot_len.dtype is i32)
     if ok:
         for t in (k_pool, v_pool, page_table, slots, slot_len, scratch, shared.groups, shared.row_group):
@@ -2473,10 +2472,10 @@ def attn_decode_shared(qkv: torch.Tensor, n_heads: int, n_kv: int, head_dim: int
     part_o = scratch.data_ptr()
     part_ml = part_o + parts * head_dim * 4
     _lib.check(_lib.load().qnn_attn_decode_shared(
-        _p(qkv), ld, dt_code(qkv), _p(k_pool), _p(v_pool), _p(page_table), page_table.shape[1], page_size, ring, _p(slots), _p(slot_len), B,
-        _p(shared.groups), shared.groups.shape[0], shared.rows, _p(shared.row_group), n_heads, n_kv, head_dim, float(scale), float(cap or 0.0),
-        int(window or 0), plan.common_ranges, plan.own_ranges, part_o, part_ml, _p(out), out.shape[1], _p(slopes), _p(sinks), k_pool.shape[0],
-        _p(_status_word(qkv.device)), _stream()), "attn_decode_shared", 2)
+        qkv.data_ptr(), ld, dt_code(qkv), k_pool.data_ptr(), v_pool.data_ptr(), page_table.data_ptr(), table[1], page_size, ring, slots.data_ptr(),
+        slot_len.data_ptr(), B, shared.groups.data_ptr(), shared.n_groups, shared.rows, shared.row_group.data_ptr(), n_heads, n_kv, head_dim, scale,
+        cap or 0.0, window or 0, plan.common_ranges, plan.own_ranges, part_o, part_ml, out.data_ptr(), n_heads * head_dim, _p(slopes), _p(sinks),
+        pools[0], _status_word(qkv.device).data_ptr(), _stream()), "attn_decode_shared", plan.kernels)
     return out
 
 
@@ -2500,27 +2499,31 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, take: in
     (formed in 64 bits, rounded once), its beam within the request and its token; equal scores in the order of (beam, token).  Places that
     nothing is left for hold -inf, -1, -1.  A logit that is not finite is never chosen and sets bit 0 of ``error_flag``; ``status`` joins the
     error word as in ``sample``."""
-    _req(logits, "logits", torch.float32, 2)
-    _req(scores, "scores", torch.float32, 1)
+    here, f32, i32 = _here(), torch.float32, torch.int32
+    _req(logits, "logits", f32, 2)
+    _req(scores, "scores", f32, 1)
+    _req(scratch, "scratch")
     R, V = logits.shape
     if beams < 1 or R % beams or scores.numel() != R:
         raise ValueError(f"beam selection: {R} rows and {scores.numel()} scores are not requests of {beams} beams")
+    L = _lib.load()
     if not 1 <= take <= BEAM_MOST:
         raise ValueError(f"beam selection returns 1..{BEAM_MOST} continuations per request, not {take}")
-    if scratch.numel() * scratch.element_size() < beam_select_scratch_bytes(R, V, take):
+    if scratch.numel() * scratch.element_size() < 8 * R * L.qnn_beam_select_segments(V):
         raise ValueError("beam selection: scratch is too small")
-    _req(scratch, "scratch")
     Q = R // beams
     if out is None:
-        out = (torch.empty((Q, take), dtype=torch.float32, device=logits.device),
-               torch.empty((Q, take), dtype=torch.int32, device=logits.device), torch.empty((Q, take), dtype=torch.int32, device=logits.device))
-    for t, dt, what in zip(out, (torch.float32, torch.int32, torch.int32), ("scores", "beams", "tokens")):
-        _req(t, f"out {what}", dt, 2)
-        if tuple(t.shape) != (Q, take):
-            raise ValueError(f"beam selection: the output {what} are {tuple(t.shape)}, not {(Q, take)}")
-    _on_current_device(logits, scores, scratch, *out)
-    _lib.check(_lib.load().qnn_beam_select(_p(logits), _p(scores), Q, beams, V, take, _p(scratch), _p(out[0]), _p(out[1]), _p(out[2]), _p(status),
-                                           _p(error_flag), _stream()), "beam_select", 2)
+        tokens = logits.new_empty((Q, take), dtype=i32)
+        out = (logits.new_empty((Q, take)), torch.empty_like(tokens), tokens)
+    else:
+        for t, dt, what in zip(out, (f32, i32, i32), ("scores", "beams", "tokens")):
+            _req(t, f"out {what}", dt, 2)
+            if tuple(t.shape) != (Q, take):
+                raise ValueError(f"beam selection: the output {what} are {tuple(t.shape)}, not {(Q, take)}")
+    if not here == logits.get_device() == scores.get_device() == scratch.get_device() == out[0].get_device():
+        _on_current_device(logits, scores, scratch, *out)
+    _lib.check(L.qnn_beam_select(logits.data_ptr(), scores.data_ptr(), Q, beams, V, take, scratch.data_ptr(), out[0].data_ptr(), out[1].data_ptr(),
+                                 out[2].data_ptr(), _p(status), _p(error_flag), _stream()), "beam_select", 2)
     return out
 
 
@@ -2543,16 +2546,19 @@ def copy_slots(tensors: Sequence[torch.Tensor], src: Sequence[int], dst: Sequenc
     if not tensors:
         _check_moves(src, dst, 0, 1 << 31, "copy_slots")
         return
-    _check_moves(src, dst, 0, min(t.shape[0] if t.dim() else 0 for t in tensors), "copy_slots")
-    for t in tensors:
-        _req(t, "a tensor of copy_slots")
-    _on_current_device(*tensors)
-    n, p = len(tensors), len(src)
-    launched = ctypes.c_int(0)
-    base = (ctypes.c_void_p * n)(*[t.data_ptr() for t in tensors])
-    size = (ctypes.c_longlong * n)(*[t.numel() // t.shape[0] * t.element_size() for t in tensors])
-    code = _lib.load().qnn_copy_slots(base, size, n, (ctypes.c_int * p)(*src), (ctypes.c_int * p)(*dst), p, ctypes.byref(launched), _stream())
-    _lib.check(code, "copy_slots", launched.value)
+    _check_moves(src, dst, 0, min([t.shape[0] if t.dim() else 0 for t in tensors]), "copy_slots")
+    here, base, size = _here(), [], []
+    for t in tensors:                        # (two rows at least: source and destination)
+        if t.get_device() != here or not t.is_contiguous():
+            _req(t, "a tensor of copy_slots")
+            _on_current_device(t)
+        base.append(t.data_ptr())
+        size.append(t.stride(0) * t.element_size() if t.numel() else 0)
+    n, p, launched = len(tensors), len(src), ctypes.c_int(0)
+    ints = ctypes.c_int * p
+    _lib.check(_lib.load().qnn_copy_slots((ctypes.c_void_p * n)(*base), (ctypes.c_longlong * n)(*size), n, ints(*src), ints(*dst), p,
+                                          ctypes.byref(launched), _stream()), "copy_slots", 0)
+    _lib.launches += launched.value
 
 
 def copy_pages(k: torch.Tensor, v: torch.Tensor, src: Sequence[int], dst: Sequence[int], used: Sequence[int]) -> None:
@@ -2564,16 +2570,18 @@ def copy_pages(k: torch.Tensor, v: torch.Tensor, src: Sequence[int], dst: Sequen
     if not len(src) and not len(dst):
         return
     _req(k, "k", None, 5)
-    _req(v, "v", k.dtype, 5)
-    if k.shape != v.shape:
-        raise ValueError(f"copy_pages: pools of different shapes, {tuple(k.shape)} and {tuple(v.shape)}")
+    if v is not k:
+        _req(v, "v", k.dtype, 5)
+        if k.shape != v.shape:
+            raise ValueError(f"copy_pages: pools of different shapes, {tuple(k.shape)} and {tuple(v.shape)}")
     lines, pages, heads, page, dim = k.shape
     _check_moves(src, dst, 1, pages, "copy_pages")
     if min(used) < 0 or max(used) > page:
         raise ValueError(f"copy_pages: a page holds {page} positions")
-    _on_current_device(k, v)
-    p = len(src)
-    launched = ctypes.c_int(0)
-    code = _lib.load().qnn_copy_pages(_p(k), _p(v), lines, pages, heads, page, dim, k.element_size(), (ctypes.c_int * p)(*src), (ctypes.c_int * p)(*dst),
-                                      (ctypes.c_int * p)(*used), p, ctypes.byref(launched), _stream())
-    _lib.check(code, "copy_pages", launched.value)
+    if not k.get_device() == v.get_device() == _here():
+        _on_current_device(k, v)
+    p, launched = len(src), ctypes.c_int(0)
+    ints = ctypes.c_int * p
+    _lib.check(_lib.load().qnn_copy_pages(k.data_ptr(), v.data_ptr(), lines, pages, heads, page, dim, k.element_size(), ints(*src), ints(*dst),
+                                          ints(*used), p, ctypes.byref(launched), _stream()), "copy_pages", 0)
+    _lib.launches += launched.value
