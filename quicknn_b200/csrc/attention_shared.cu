@@ -349,8 +349,9 @@ attn_shared_mma_kernel(const __grid_constant__ CUtensorMap map, const KV kv, con
 }
 
 // ---- any head size, float32 or bfloat16 ----------------------------------------------------------------------------------------
-// Tiles of 32 keys as float32 in shared memory (rows an odd number of floats apart); a lane forms the scores of one key, then the lanes
-// take the head's elements.  A warp keeps GEN_Q queries; exact exponentials and tanh in float32.
+// Tiles of 32 keys as float32 in shared memory (rows an odd number of floats apart).  A warp keeps GEN_Q queries: a lane forms their scores with one
+// key, the weights go to shared memory, and then the lanes take the head's elements, so that what is read of K and V serves all
+// the warp's queries.  Exact exponentials and tanh in float32.
 constexpr int GEN_WARPS = 4, GEN_Q = 4, GEN_QT = GEN_WARPS * GEN_Q;
 
 template <typename T, int DPL>                                // elements of a head per lane, at most
@@ -377,10 +378,12 @@ attn_shared_generic_kernel(const T* __restrict__ q, size_t q_stride, const T* __
     const int pitch = hd + 1;
     float* sk = sm;
     float* sv = sk + tile_keys * pitch;
-    float* sq = sv + tile_keys * pitch;                       // [GEN_QT][hd], times the scale
-    for (int i = threadIdx.x; i < queries * hd; i += blockDim.x) {
+    float* sq = sv + tile_keys * pitch;                       // [GEN_QT][hd], times the scale; zeros for queries that are not there
+    float4* sw = reinterpret_cast<float4*>(sq + GEN_QT * hd) + warp * 32;      // the warp's weights: key, then query
+    static_assert(GEN_Q == 4, "a float4 of weights");
+    for (int i = threadIdx.x; i < GEN_QT * hd; i += blockDim.x) {
         const int m = it.query0 + i / hd, d = i % hd;
-        sq[i] = to_f(q[(size_t)(it.row0 + m / G) * q_stride + (size_t)(kh * G + m % G) * hd + d]) * scale;
+        sq[i] = i / hd < queries ? to_f(q[(size_t)(it.row0 + m / G) * q_stride + (size_t)(kh * G + m % G) * hd + d]) * scale : 0.f;
     }
     float mx[GEN_Q], l[GEN_Q], o[GEN_Q][DPL], slope[GEN_Q];
     int newest[GEN_Q];
@@ -428,31 +431,47 @@ attn_shared_generic_kernel(const T* __restrict__ q, size_t q_stride, const T* __
         __syncthreads();
         const int pos = lane < n ? it.position(t + lane / TILE) + lane % TILE : 0;
         const bool valid = lane < n && pos >= it.lo && pos < it.hi;
+        if (warp * GEN_Q >= queries) continue;                // (the warp still brings keys)
+        float s[GEN_Q] = {0.f, 0.f, 0.f, 0.f}, w[GEN_Q];
+        {
+            const float* kr = sk + (valid ? lane : 0) * pitch;
+            const float* qr = sq + warp * GEN_Q * hd;
+#pragma unroll 4
+            for (int d = 0; d < hd; d += 4) {
+                const float k0 = kr[d], k1 = kr[d + 1], k2 = kr[d + 2], k3 = kr[d + 3];
+#pragma unroll
+                for (int i = 0; i < GEN_Q; ++i) {
+                    const float4 x = *reinterpret_cast<const float4*>(qr + i * hd + d);
+                    s[i] = fmaf(x.w, k3, fmaf(x.z, k2, fmaf(x.y, k1, fmaf(x.x, k0, s[i]))));
+                }
+            }
+        }
 #pragma unroll
         for (int i = 0; i < GEN_Q; ++i) {
-            const int m = warp * GEN_Q + i;
-            if (m >= queries) break;
-            float s = 0.f;
-            if (valid) {
-                const float* kr = sk + lane * pitch;
-                const float* qr = sq + m * hd;
-                for (int d = 0; d < hd; ++d) s = fmaf(qr[d], kr[d], s);
-                s = softcap_t<T>(s, cap) - slope[i] * (float)(newest[i] - pos);
-            }
-            const float top = fmaxf(mx[i], warp_max(valid ? s : -CUDART_INF_F));
+            s[i] = softcap_t<T>(s[i], cap) - slope[i] * (float)(newest[i] - pos);
+            const float top = fmaxf(mx[i], warp_max(valid ? s[i] : -CUDART_INF_F));
             const float keep = mx[i] == -CUDART_INF_F ? 0.f : fexp<T>(mx[i] - top);
-            const float w = valid && (top != -CUDART_INF_F || s != s) ? fexp<T>(s - top) : 0.f;
-            l[i] = l[i] * keep + warp_sum(w);
+            w[i] = valid && (top != -CUDART_INF_F || s[i] != s[i]) ? fexp<T>(s[i] - top) : 0.f;
+            l[i] = l[i] * keep + warp_sum(w[i]);
             mx[i] = top;
 #pragma unroll
             for (int d = 0; d < DPL; ++d) o[i][d] *= keep;
-            for (int j = 0; j < n; ++j) {
-                const float wj = __shfl_sync(0xffffffffu, w, j);
+        }
+        sw[lane] = make_float4(w[0], w[1], w[2], w[3]);
+        __syncwarp();
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) {
+            const float4 wj = sw[j];
 #pragma unroll
-                for (int d = 0; d < DPL; ++d)
-                    if (lane + d * 32 < hd) o[i][d] = fmaf(wj, sv[j * pitch + lane + d * 32], o[i][d]);
+            for (int d = 0; d < DPL; ++d) {
+                const float v = lane + d * 32 < hd ? sv[j * pitch + lane + d * 32] : 0.f;
+                o[0][d] = fmaf(wj.x, v, o[0][d]);
+                o[1][d] = fmaf(wj.y, v, o[1][d]);
+                o[2][d] = fmaf(wj.z, v, o[2][d]);
+                o[3][d] = fmaf(wj.w, v, o[3][d]);
             }
         }
+        __syncwarp();                                         // before the weights are written again
     }
 #pragma unroll
     for (int i = 0; i < GEN_Q; ++i) {
@@ -617,7 +636,7 @@ template <typename T, int DPL>
 int launch_generic(const void* q, long long q_stride, const void* k_pool, const void* v_pool, const Cells& cells, const Shared& sh, int items, int nq,
                    int nkv, int hd, float scale, float cap, float* part_o, float2* part_ml, const float* slopes, cudaStream_t st) {
     const int keys = hd <= 512 ? 32 : 16;
-    const size_t smem = ((size_t)2 * keys * (hd + 1) + (size_t)GEN_QT * hd) * sizeof(float);
+    const size_t smem = ((size_t)2 * keys * (hd + 1) + (size_t)GEN_QT * hd + GEN_WARPS * 32 * 4) * sizeof(float);
     auto kern = attn_shared_generic_kernel<T, DPL>;
     static OncePerDevice asked;
     if (const int rc = allow_shared(asked, kern, 220 * 1024)) return rc;

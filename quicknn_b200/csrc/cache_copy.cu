@@ -76,20 +76,18 @@ __global__ void __launch_bounds__(COPY_THREADS) copy_pages_kernel(char* __restri
 
 }  // namespace
 
-// tensor i: `slots` rows of bytes[i] bytes at base[i]; row dst[p] = row src[p] for every pair and tensor.  base, bytes, src and dst are host arrays,
-// read before the call returns.
-QNN_API int qnn_copy_slots(void* const* base, const long long* bytes, int n_tensors, const int* src, const int* dst, int n_pairs, int* launched,
-                           cudaStream_t st) {
-    *launched = 0;
+// tensors: n_tensors x (address, bytes of a row); row dst[p] = row src[p] of every tensor, for every pair.  pairs: n_pairs sources, then as many
+// destinations.  Both are host arrays, read before the call returns.
+QNN_API int qnn_copy_slots(const long long* tensors, int n_tensors, const int* pairs_of, int n_pairs, cudaStream_t st) {
     for (int t0 = 0; t0 < n_tensors; t0 += MOST_TENSORS) {
         Tensors t;
         const int nt = n_tensors - t0 < MOST_TENSORS ? n_tensors - t0 : MOST_TENSORS;
         long long blocks = 0;
         for (int i = 0; i < nt; ++i) {
-            t.base[i] = (char*)base[t0 + i];
-            t.bytes[i] = bytes[t0 + i];
+            t.base[i] = (char*)tensors[2 * (t0 + i)];
+            t.bytes[i] = tensors[2 * (t0 + i) + 1];
             t.blocks[i] = (int)blocks;
-            blocks += (bytes[t0 + i] + COPY_BYTES - 1) / COPY_BYTES;
+            blocks += (t.bytes[i] + COPY_BYTES - 1) / COPY_BYTES;
             if (blocks > 0x7fffffff) return QNN_ERR_UNSUPPORTED;
         }
         t.blocks[nt] = (int)blocks;
@@ -98,25 +96,25 @@ QNN_API int qnn_copy_slots(void* const* base, const long long* bytes, int n_tens
             Pairs pairs;
             const int np = n_pairs - p0 < MOST_PAIRS ? n_pairs - p0 : MOST_PAIRS;
             for (int i = 0; i < np; ++i) {
-                pairs.src[i] = src[p0 + i];
-                pairs.dst[i] = dst[p0 + i];
+                pairs.src[i] = pairs_of[p0 + i];
+                pairs.dst[i] = pairs_of[n_pairs + p0 + i];
             }
             launch_pdl(copy_slots_kernel, dim3((unsigned)blocks, np), dim3(COPY_THREADS), 0, st, t, pairs, nt);
-            ++*launched;
             if (const cudaError_t e = cudaGetLastError()) return (int)e;
         }
     }
     return 0;
 }
 
-// Pools [lines][pages][heads][page_size][head_dim] of esize-byte elements (v == k: one pool): the first used[p] positions of page src[p] go to page
-// dst[p], in every line and head.  src, dst and used are host arrays, read before the call returns.
-QNN_API int qnn_copy_pages(void* k, void* v, int lines, long long pages, int heads, int page_size, int head_dim, int esize, const int* src,
-                           const int* dst, const int* used, int n_pairs, int* launched, cudaStream_t st) {
-    *launched = 0;
+// Pools [lines][pages][heads][page_size][head_dim] of esize-byte elements (v == k: one pool): the first used positions of page src go to page
+// dst, in every line and head, for every pair.  moves: n_pairs sources, as many destinations, as many numbers of positions: a host array, read
+// before the call returns.
+QNN_API int qnn_copy_pages(void* k, void* v, int lines, long long pages, int heads, int page_size, int head_dim, int esize, const int* moves,
+                           int n_pairs, cudaStream_t st) {
     if (lines <= 0 || n_pairs <= 0) return 0;
     const long long page_bytes = (long long)page_size * head_dim * esize;
     if (page_bytes > 0x7fffffff) return QNN_ERR_UNSUPPORTED;
+    const int *src = moves, *dst = moves + n_pairs, *used = moves + 2 * n_pairs;
     for (int p0 = 0; p0 < n_pairs; p0 += MOST_PAIRS) {
         PagePairs pairs;
         const int np = n_pairs - p0 < MOST_PAIRS ? n_pairs - p0 : MOST_PAIRS;
@@ -133,7 +131,6 @@ QNN_API int qnn_copy_pages(void* k, void* v, int lines, long long pages, int hea
         if (runs > 0x7fffffff) return QNN_ERR_UNSUPPORTED;
         launch_pdl(copy_pages_kernel, dim3((unsigned)runs, np, v != k ? 2 : 1), dim3(COPY_THREADS), 0, st, (char*)k, (char*)v, pairs, pages, heads,
                    (int)page_bytes, head_dim * esize, pieces);
-        ++*launched;
         if (const cudaError_t e = cudaGetLastError()) return (int)e;
     }
     return 0;

@@ -2342,7 +2342,7 @@ class SharedPlan(NamedTuple):
     kernels: int = 2             # launches of a call
 
 
-SHARED_ITEM_COST = 64.0          # what a CTA of that attention costs beside its keys, in keys
+SHARED_ITEM_COST = 64.0          # what a CTA of that attention costs beside its keys, in keys; of the kernel for any head size a quarter
 
 
 def shared_attention_plan(dtype: torch.dtype, n_rows: int, n_heads: int, n_kv: int, head_dim: int, shared: SharedKeys,
@@ -2375,15 +2375,15 @@ def shared_attention_plan(dtype: torch.dtype, n_rows: int, n_heads: int, n_kv: i
             s = next((n for n in range(1, 9) if walk(n) <= 0.6 * time), 0) or min(range(1, 65), key=lambda n: walk(n) + parts * n)
             ranges = (min(s, -(-keys // 64)), p)
         else:
-            best = None
+            best, cost = None, SHARED_ITEM_COST / (1 if dtype == torch.bfloat16 and head_dim in (64, 128, 256) else 4)
             for c in _SHARED_CHUNKS:
                 s, p = -(-keys // c), -(-own // c)
                 if s > 64 or p > 64:
                     continue
                 longest = max(-(-keys // s) if common else 0, -(-own // p))
-                t = longest + SHARED_ITEM_COST
+                t = longest + cost
                 if common * s + alone * p > resident:
-                    t = max(t, (common * (keys + s * SHARED_ITEM_COST) + alone * (own + p * SHARED_ITEM_COST)) / resident + longest / 2)
+                    t = max(t, (common * (keys + s * cost) + alone * (own + p * cost)) / resident + longest / 2)
                 t += parts * (s + p)
                 if best is None or t < best[0] * 0.999:
                     best = (t, s, p)
@@ -2399,7 +2399,7 @@ def shared_attention_pays(dtype: torch.dtype, n_heads: int, n_kv: int, head_dim:
     return min(shared.keys, window or shared.keys) >= 256
 
 
-_SHARED_CHUNKS = tuple(sorted({16 * int(round(2 ** (i / 2))) for i in range(4, 28)}))       # 64 keys .. 128 K
+_SHARED_CHUNKS = tuple(sorted({16 * int(round(2 ** (i / 2))) for i in range(2, 28)}))       # 32 keys .. 128 K
 
 
 def _spread(items: int, resident: int, keys: float) -> float:
@@ -2546,19 +2546,20 @@ def copy_slots(tensors: Sequence[torch.Tensor], src: Sequence[int], dst: Sequenc
     if not tensors:
         _check_moves(src, dst, 0, 1 << 31, "copy_slots")
         return
-    _check_moves(src, dst, 0, min([t.shape[0] if t.dim() else 0 for t in tensors]), "copy_slots")
-    here, base, size = _here(), [], []
+    rows, where, flat = 1 << 31, set(), []
     for t in tensors:                        # (two rows at least: source and destination)
-        if t.get_device() != here or not t.is_contiguous():
+        if not t.is_cuda or not t.dim() or not t.is_contiguous():
+            _check_moves(src, dst, 0, min([t.shape[0] if t.dim() else 0 for t in tensors]), "copy_slots")
             _req(t, "a tensor of copy_slots")
-            _on_current_device(t)
-        base.append(t.data_ptr())
-        size.append(t.stride(0) * t.element_size() if t.numel() else 0)
-    n, p, launched = len(tensors), len(src), ctypes.c_int(0)
-    ints = ctypes.c_int * p
-    _lib.check(_lib.load().qnn_copy_slots((ctypes.c_void_p * n)(*base), (ctypes.c_longlong * n)(*size), n, ints(*src), ints(*dst), p,
-                                          ctypes.byref(launched), _stream()), "copy_slots", 0)
-    _lib.launches += launched.value
+        rows = min(rows, t.shape[0])
+        where.add(t.get_device())
+        flat += (t.data_ptr(), t.stride(0) * t.element_size() if t.numel() else 0)
+    _check_moves(src, dst, 0, rows, "copy_slots")
+    if where != {_here()}:
+        _on_current_device(*tensors)
+    n, p = len(tensors), len(src)
+    _lib.check(_lib.load().qnn_copy_slots((ctypes.c_longlong * (2 * n))(*flat), n, (ctypes.c_int * (2 * p))(*src, *dst), p, _stream()), "copy_slots",
+               -(-n // 64) * -(-p // 128))
 
 
 def copy_pages(k: torch.Tensor, v: torch.Tensor, src: Sequence[int], dst: Sequence[int], used: Sequence[int]) -> None:
@@ -2580,8 +2581,6 @@ def copy_pages(k: torch.Tensor, v: torch.Tensor, src: Sequence[int], dst: Sequen
         raise ValueError(f"copy_pages: a page holds {page} positions")
     if not k.get_device() == v.get_device() == _here():
         _on_current_device(k, v)
-    p, launched = len(src), ctypes.c_int(0)
-    ints = ctypes.c_int * p
-    _lib.check(_lib.load().qnn_copy_pages(k.data_ptr(), v.data_ptr(), lines, pages, heads, page, dim, k.element_size(), ints(*src), ints(*dst),
-                                          ints(*used), p, ctypes.byref(launched), _stream()), "copy_pages", 0)
-    _lib.launches += launched.value
+    p = len(src)
+    _lib.check(_lib.load().qnn_copy_pages(k.data_ptr(), v.data_ptr(), lines, pages, heads, page, dim, k.element_size(),
+                                          (ctypes.c_int * (3 * p))(*src, *dst, *used), p, _stream()), "copy_pages", -(-p // 128))
