@@ -594,13 +594,21 @@ attn_shared_join_kernel(const float* __restrict__ part_o, const float2* __restri
 
 bool on_tensor_cores(int dtype, int hd) { return dtype == QNN_DT_BF16 && (hd == 64 || hd == 128 || hd == 256); }
 
-// Groups of more query rows than an item of the kernel above takes go to the 5th-generation tensor cores, where a CTA takes 128.
-constexpr int MANY_TILE = 128;
-bool many_rows(int dtype, int hd, int queries) { return on_tensor_cores(dtype, hd) && queries > (hd > 128 ? 16 : 32); }
-
 // Column tiles of an item for so many queries: 1, 2 or, up to head size 128, 4.  More do not fit the registers (O and Q of 16 queries of 256
 // elements are 192 registers a thread).
 int column_tiles(int hd, int queries) { return queries <= 8 ? 1 : (queries <= 16 || hd > 128 ? 2 : 4); }
+
+// Groups of more query rows than an item of the mma.sync kernel takes go to the 5th-generation tensor cores, where a CTA takes 128, if the work is
+// enough for what a kernel of its own costs (3 to 4 us): `walks` walks (groups x kv heads) over `keys` keys, times the items beside one another
+// that the queries would take here.  Where both take the same time, in items x walks x keys: head size 256 from 22,000 (128 queries) to 90,000 (576);
+// 128 and 64 from 4000 to 10,000.  us there and here, 4 kv heads of 256: 64 queries on 1024 keys 14.5 / 12.8, on 4096 17.3 / 25.2; 18 queries on
+// 4096 16.6 / 12.5; 16 kv heads of 128: 128 queries on 512 18.1 / 24.7, on 8192 42 / 85.
+constexpr int MANY_TILE = 128;
+bool many_rows(int dtype, int hd, int queries, long long walks, int keys) {
+    if (!on_tensor_cores(dtype, hd)) return false;
+    const int tile = 8 * column_tiles(hd, queries);
+    return queries > tile && (queries + tile - 1) / tile * walks * keys >= (hd == 256 ? 50000 : 6000);
+}
 
 template <int HD, int NT, bool BIAS, bool BESIDE>
 int launch_mma(const void* q, long long q_stride, const void* k_pool, const void* v_pool, long long pool_rows, const Cells& cells, const Shared& sh,
@@ -664,33 +672,34 @@ int launch_join(const float* part_o, const float2* part_ml, void* out, long long
 }  // namespace
 
 // Queries that one item takes (what the number of items, and with it the choice of ranges, goes by), or a negative number for a head
-// size that is not taken.  `queries`: rows x query heads per kv head of the largest group.
-QNN_API int qnn_attn_shared_tile(int dtype, int hd, int queries) {
+// size that is not taken.  queries: rows x query heads per kv head of the largest group; walks: groups x kv heads; keys: of a group, at most.
+QNN_API int qnn_attn_shared_tile(int dtype, int hd, int queries, int walks, int keys) {
     const int vec = dtype == QNN_DT_BF16 ? 8 : 4;
     if (hd <= 0 || hd % vec || hd > 1024) return -1;
-    return many_rows(dtype, hd, queries) ? MANY_TILE : (on_tensor_cores(dtype, hd) ? 8 * column_tiles(hd, queries) : GEN_QT);
+    return many_rows(dtype, hd, queries, walks, keys) ? MANY_TILE : (on_tensor_cores(dtype, hd) ? 8 * column_tiles(hd, queries) : GEN_QT);
 }
 
 // groups: [n_groups][4] (first row, rows, begin, end): positions begin .. end - 1 lie in the same pages in all the group's rows, as far as a row
-// still holds them; row_group: [B], a row's group or -1.  `most_rows`: rows of the largest group.  common_ranges / own_ranges: into how many ranges
+// still holds them; row_group: [B], a row's group or -1.  `most_rows`: rows of the largest group; `most_keys`: positions of the
+// longest (a matter of speed).  common_ranges / own_ranges: into how many ranges
 // a group's common keys and a row's own keys are cut.  Scratch: part_o B * nq * (common_ranges + own_ranges) * hd floats, part_ml twice as many
 // without hd; 16-byte aligned.  pool_pages: pages of
 // the pools; status: as in qnn_gemm_tcgen05 (bit 512: keys or values did not arrive).  page_size: a power of two of at least 16; ring: a multiple of it, or 0.  slots, slot_len, page_table, groups and
 // row_group are read before the kernel waits for the one launched in front of it on the stream: that one must not write them.
 QNN_API int qnn_attn_decode_shared(const void* q, long long q_stride, int dtype, const void* k_pool, const void* v_pool, const int* page_table,
                                    int max_pages, int page_size, int ring, const int* slots, const int* slot_len, int B, const int* groups,
-                                   int n_groups, int most_rows, const int* row_group, int nq, int nkv, int hd, float scale, float cap, int window,
+                                   int n_groups, int most_rows, int most_keys, const int* row_group, int nq, int nkv, int hd, float scale, float cap, int window,
                                    int common_ranges, int own_ranges, float* part_o, float* part_ml, void* out, long long out_stride,
                                    const float* slopes, const float* sinks, long long pool_pages, int* status, cudaStream_t st) {
     if (B <= 0) return 0;
-    if (nkv <= 0 || nkv > 65535 || nq <= 0 || nq % nkv || n_groups < 0 || most_rows < 0 || common_ranges < 1 || own_ranges < 1 ||
+    if (nkv <= 0 || nkv > 65535 || nq <= 0 || nq % nkv || n_groups < 0 || most_rows < 0 || most_keys < 0 || common_ranges < 1 || own_ranges < 1 ||
         common_ranges + own_ranges > MOST_PARTS)
         return QNN_ERR_ARGUMENT;
     if (page_size < 16 || (page_size & (page_size - 1)) || ring < 0 || ring % page_size) return QNN_ERR_ARGUMENT;
     if (ring > 0 && (window <= 0 || window > ring || ring / page_size > max_pages)) return QNN_ERR_ARGUMENT;   // a ring holds no more
     const int G = nq / nkv, esize = dtype == QNN_DT_BF16 ? 2 : 4;
-    const bool many = n_groups > 0 && page_size >= 64 && many_rows(dtype, hd, most_rows * G);
-    const int tile = many ? MANY_TILE : (on_tensor_cores(dtype, hd) ? 8 * column_tiles(hd, most_rows * G) : qnn_attn_shared_tile(dtype, hd, most_rows * G));
+    const bool many = n_groups > 0 && page_size >= 64 && many_rows(dtype, hd, most_rows * G, (long long)n_groups * nkv, most_keys);
+    const int tile = many ? MANY_TILE : (on_tensor_cores(dtype, hd) ? 8 * column_tiles(hd, most_rows * G) : qnn_attn_shared_tile(dtype, hd, most_rows * G, 0, 0));
     if (tile <= 0) return QNN_ERR_UNSUPPORTED;
     if ((q_stride * esize) % 16 || ((uintptr_t)q & 15) || ((uintptr_t)k_pool & 15) || ((uintptr_t)v_pool & 15) || ((uintptr_t)part_o & 15) ||
         ((uintptr_t)part_ml & 7) || ((uintptr_t)groups & 15) || ((uintptr_t)out & 15) || (out_stride * esize) % 16)

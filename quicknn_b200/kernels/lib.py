@@ -154,8 +154,8 @@ _SIGNATURES: Dict[str, list] = {
     "qnn_map_difference": [c_vp, c_ll, c_int, c_vp, c_ll, c_int, c_int, c_int, c_float, c_float, c_float, c_int, c_vp],
     "qnn_head_norm_gate": [c_vp, c_ll, c_int, c_vp, c_ll, c_vp, c_int, c_int, c_float, c_vp, c_ll, c_int, c_vp, c_ll,
                            c_int, c_int, c_int, c_int, c_vp],
-    "qnn_attn_shared_tile": [c_int, c_int, c_int],
-    "qnn_attn_decode_shared": [c_vp, c_ll, c_int, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_vp, c_vp, c_int, c_vp, c_int, c_int, c_vp, c_int,
+    "qnn_attn_shared_tile": [c_int, c_int, c_int, c_int, c_int],
+    "qnn_attn_decode_shared": [c_vp, c_ll, c_int, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_vp, c_vp, c_int, c_vp, c_int, c_int, c_int, c_vp, c_int,
                                c_int, c_int, c_float, c_float, c_int, c_int, c_int, c_vp, c_vp, c_vp, c_ll, c_vp, c_vp, c_ll, c_vp, c_vp],
     "qnn_beam_select_segments": [c_int],
     "qnn_beam_select": [c_vp, c_vp, c_int, c_int, c_int, c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp],

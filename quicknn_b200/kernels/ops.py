@@ -2352,7 +2352,8 @@ def shared_attention_plan(dtype: torch.dtype, n_rows: int, n_heads: int, n_kv: i
     if n_kv < 1 or n_heads % n_kv or n_rows < 0:
         raise ValueError(f"shared attention: {n_kv} kv heads do not divide {n_heads} heads")
     heads = n_heads // n_kv
-    tile = _lib.load().qnn_attn_shared_tile(BF16 if dtype == torch.bfloat16 else F32, head_dim, max(shared.rows, 1) * heads)
+    tile = _lib.load().qnn_attn_shared_tile(BF16 if dtype == torch.bfloat16 else F32, head_dim, max(shared.rows, 1) * heads, shared.n_groups * n_kv,
+                                            shared.keys)
     if dtype not in (torch.bfloat16, torch.float32) or tile <= 0:
         raise ValueError(f"shared attention does not take head size {head_dim} in {dtype}")
     if ranges is None:
@@ -2395,8 +2396,16 @@ def shared_attention_plan(dtype: torch.dtype, n_rows: int, n_heads: int, n_kv: i
 
 
 def shared_attention_pays(dtype: torch.dtype, n_heads: int, n_kv: int, head_dim: int, shared, window: Optional[int] = None) -> bool:
-    """Whether a decode step should read common keys once (``attn_decode_shared``) rather than once per row (``attn_decode``)."""
-    return min(shared.keys, window or shared.keys) >= 256
+    """Whether a decode step should read common keys once (``attn_decode_shared``) rather than once per row (``attn_decode``): from so many
+    common keys on.  Measured, us, once / per row, rows with up to 100 keys of their own: 2 rows, 4 kv heads of 256, two query heads each: 64 keys
+    5.5 / 5.9, 512 5.7 / 8.2, 4096 8.5 / 17.6; 8 rows: 64 7.5 / 6.5, 256 8.1 / 8.4, 512 8.8 / 10.3; 8 rows, 16 kv heads of 128: 256 9.4 / 7.6, 512
+    10.0 / 9.7, 1024 10.9 / 13.8; 32 rows, 4 kv heads of 64: 512 9.9 / 8.0, 1024 11.6 / 10.8, 2048 13.4 / 15.9.  The kernel for any head size:
+    6 heads of 24 on one, float32, 4 rows: 128 7.9 / 8.0, 1024 8.4 / 13.8; at head size 256 it keeps too little in flight: 8 rows 1024 29 / 27, 2048
+    39 / 44, eight groups of 4 rows never."""
+    keys, heads = min(shared.keys, window or shared.keys), n_heads // n_kv
+    if dtype == torch.bfloat16 and head_dim in (64, 128, 256):
+        return keys >= (1024 if head_dim == 64 else 512)
+    return keys >= 256 if head_dim <= 64 else keys >= 2048 and shared.rows * heads >= 16 and shared.n_groups == 1
 
 
 _SHARED_CHUNKS = tuple(sorted({16 * int(round(2 ** (i / 2))) for i in range(2, 28)}))       # 32 keys .. 128 K
@@ -2473,7 +2482,7 @@ def attn_decode_shared(qkv: torch.Tensor, n_heads: int, n_kv: int, head_dim: int
     part_ml = part_o + parts * head_dim * 4
     _lib.check(_lib.load().qnn_attn_decode_shared(
         qkv.data_ptr(), ld, dt_code(qkv), k_pool.data_ptr(), v_pool.data_ptr(), page_table.data_ptr(), table[1], page_size, ring, slots.data_ptr(),
-        slot_len.data_ptr(), B, shared.groups.data_ptr(), shared.n_groups, shared.rows, shared.row_group.data_ptr(), n_heads, n_kv, head_dim, scale,
+        slot_len.data_ptr(), B, shared.groups.data_ptr(), shared.n_groups, shared.rows, shared.keys, shared.row_group.data_ptr(), n_heads, n_kv, head_dim, scale,
         cap or 0.0, window or 0, plan.common_ranges, plan.own_ranges, part_o, part_ml, out.data_ptr(), n_heads * head_dim, _p(slopes), _p(sinks),
         pools[0], _status_word(qkv.device).data_ptr(), _stream()), "attn_decode_shared", plan.kernels)
     return out

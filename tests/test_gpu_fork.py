@@ -63,7 +63,9 @@ def shared_calls(monkeypatch):
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 @pytest.mark.parametrize("name", sorted(CONFIGS))
 @pytest.mark.parametrize("prefix", [40, 330])
-def test_steps_after_a_fork(name, dtype, prefix, shared_calls):
+def test_steps_after_a_fork(name, dtype, prefix, shared_calls, monkeypatch):
+    if prefix == 330:                                                      # common keys read once, however few they are
+        monkeypatch.setattr(ops, "shared_attention_pays", lambda *a: True)
     llm = load(name, dtype)
     eng, V = llm.engine, llm.model.spec.embedding.vocab_size
     rng = np.random.default_rng(prefix)
@@ -95,7 +97,7 @@ def test_steps_after_a_fork(name, dtype, prefix, shared_calls):
     decode(1)
     decode(4)
     if prefix == 330:
-        assert bool(shared_calls) == (name not in ("gunirax", "fuposun"))  # (their attention has a window below 256)
+        assert bool(shared_calls) == (name != "gunirax")                   # (whose attention is of another kind)
     out = eng.step([(a, tails[1][:3]), (base, tails[0][5:6])], "last")     # portions onto sequences that share pages
     said[1] += tails[1][:3]
     said[0] += tails[0][5:6]

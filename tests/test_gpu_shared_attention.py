@@ -68,13 +68,14 @@ class Batch:
     def i32(self, a):
         return torch.from_numpy(np.ascontiguousarray(a, dtype=np.int32)).to(DEV)
 
-    def shared(self):
+    def shared(self, keys=None):
         g = self.i32(np.asarray(self.group_list, dtype=np.int32).reshape(-1, 4))
-        keys = max([e - a for _, _, a, e in self.group_list] or [0])
+        keys = keys or max([e - a for _, _, a, e in self.group_list] or [0])
         return ops.SharedKeys(g, self.i32(self.row_group), rows=max([r for _, r, _, _ in self.group_list] or [0]), keys=keys, own=max(self.lens))
 
-    def run(self, scale, cap=None, ranges=None, slopes=None, sinks=None):
-        sh = self.shared()
+    def run(self, scale, cap=None, ranges=None, slopes=None, sinks=None, keys=None):
+        """``keys``: the bound of a group's keys that the call is told (it may take groups of many rows to another kernel)"""
+        sh = self.shared(keys)
         plan = ops.shared_attention_plan(self.dtype, self.B, self.nq, self.nkv, self.hd, sh, self.window or None, ranges=ranges)
         scratch = torch.full((plan.scratch_bytes // 4,), float("nan"), device=DEV)
         return ops.attn_decode_shared(self.qkv, self.nq, self.nkv, self.hd, self.k, self.v, self.i32(self.table), PAGE, self.ring, self.i32(self.slots),
@@ -142,7 +143,8 @@ def test_many_rows(cap, nq, nkv, hd, pages):
     rows = {256: 18, 128: 70, 64: 19}[hd]
     b = Batch([(0, pages * 64, [pages * 64 + 1 + i % 90 for i in range(rows)]), (64, 192, [200, 222])], nq, nkv, hd, BF, alone=[130], left_out=[3], seed=pages + hd)
     for ranges in ((1, 1), (2, 1), (3, 2), (9, 1)):
-        b.check(b.run(hd ** -0.5, cap, ranges), hd ** -0.5, cap)
+        for keys in (1, 1 << 20):                                    # by either kernel
+            b.check(b.run(hd ** -0.5, cap, ranges, keys=keys), hd ** -0.5, cap)
 
 
 @pytest.mark.parametrize("nq,nkv,hd", [(8, 4, 256), (8, 2, 128), (8, 1, 64)])
@@ -153,11 +155,11 @@ def test_many_rows_with_slopes_sinks_and_windows(nq, nkv, hd):
     lens = [449 + 7 * i % 120 for i in range(34)]
     b = Batch([(0, 448, lens)], nq, nkv, hd, BF, seed=hd)
     for sl, si, cap in ((slopes, None, None), (slopes, sinks, 40.0), (None, sinks, 40.0)):
-        b.check(b.run(hd ** -0.5, cap, (2, 2), slopes=sl, sinks=si), hd ** -0.5, cap, sl, si)
+        b.check(b.run(hd ** -0.5, cap, (2, 2), slopes=sl, sinks=si, keys=1 << 20), hd ** -0.5, cap, sl, si)
     b = Batch([(0, 448, lens)], nq, nkv, hd, BF, window=300, seed=hd + 1)
-    b.check(b.run(hd ** -0.5, None, (2, 1)), hd ** -0.5)
+    b.check(b.run(hd ** -0.5, None, (2, 1), keys=1 << 20), hd ** -0.5)
     b = Batch([(64 * 20, 64 * 24, [64 * 24 + 1 + i for i in range(60)])], nq, nkv, hd, BF, window=384, ring=384, seed=hd + 2)
-    b.check(b.run(hd ** -0.5, 50.0), hd ** -0.5, 50.0)
+    b.check(b.run(hd ** -0.5, 50.0, keys=1 << 20), hd ** -0.5, 50.0)
 
 
 def test_many_rows_of_large_scores():
@@ -171,7 +173,7 @@ def test_many_rows_of_large_scores():
             k[:704] = keys
         b.k[pages[pos // 64], :, pos % 64] = keys
         for ranges in ((1, 1), (2, 1)):
-            b.check(b.run(1.0, None, ranges), 1.0)
+            b.check(b.run(1.0, None, ranges, keys=1 << 20), 1.0)
 
 
 @pytest.mark.parametrize("ranges", [(1, 1), (1, 3), (5, 1), (7, 4), (64, 40)])
