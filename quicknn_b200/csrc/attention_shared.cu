@@ -594,20 +594,19 @@ attn_shared_join_kernel(const float* __restrict__ part_o, const float2* __restri
 
 bool on_tensor_cores(int dtype, int hd) { return dtype == QNN_DT_BF16 && (hd == 64 || hd == 128 || hd == 256); }
 
-// Column tiles of an item for so many queries: 1, 2 or, up to head size 128, 4.  More do not fit the registers (O and Q of 16 queries of 256
-// elements are 192 registers a thread).
-int column_tiles(int hd, int queries) { return queries <= 8 ? 1 : (queries <= 16 || hd > 128 ? 2 : 4); }
+// Column tiles of an item for so many queries: 1 or 2.  (4, up to head size 128, were slower wherever they would have been taken: 18 queries, 8 kv
+// heads of 128, 2048 keys 12.7 us against 9.9.)
+int column_tiles(int queries) { return queries <= 8 ? 1 : 2; }
 
 // Groups of more query rows than an item of the mma.sync kernel takes go to the 5th-generation tensor cores, where a CTA takes 128, if the work is
 // enough for what a kernel of its own costs (3 to 4 us): `walks` walks (groups x kv heads) over `keys` keys, times the items beside one another
-// that the queries would take here.  Where both take the same time, in items x walks x keys: head size 256 from 22,000 (128 queries) to 90,000 (576);
-// 128 and 64 from 4000 to 10,000.  us there and here, 4 kv heads of 256: 64 queries on 1024 keys 14.5 / 12.8, on 4096 17.3 / 25.2; 18 queries on
-// 4096 16.6 / 12.5; 16 kv heads of 128: 128 queries on 512 18.1 / 24.7, on 8192 42 / 85.
+// that the queries would take here.  Both take the same time at 22,000 (128 queries of 256) to 100,000 (18 queries of 128).  us there and here,
+// 4 kv heads of 256: 64 queries on 1024 keys 14.5 / 12.8, on 4096 17.3 / 25.2; 18 queries on 4096 16.6 / 12.5; 2 kv heads of 128: 64 queries on
+// 2048 11.5 / 9.3; four groups of 24 queries, 8 kv heads of 128, 8192 keys 35 / 48.
 constexpr int MANY_TILE = 128;
+constexpr long long MANY_WORK = 50000;
 bool many_rows(int dtype, int hd, int queries, long long walks, int keys) {
-    if (!on_tensor_cores(dtype, hd)) return false;
-    const int tile = 8 * column_tiles(hd, queries);
-    return queries > tile && (queries + tile - 1) / tile * walks * keys >= (hd == 256 ? 50000 : 6000);
+    return on_tensor_cores(dtype, hd) && queries > 16 && (queries + 15) / 16 * walks * keys >= MANY_WORK;
 }
 
 template <int HD, int NT, bool BIAS, bool BESIDE>
@@ -676,7 +675,7 @@ int launch_join(const float* part_o, const float2* part_ml, void* out, long long
 QNN_API int qnn_attn_shared_tile(int dtype, int hd, int queries, int walks, int keys) {
     const int vec = dtype == QNN_DT_BF16 ? 8 : 4;
     if (hd <= 0 || hd % vec || hd > 1024) return -1;
-    return many_rows(dtype, hd, queries, walks, keys) ? MANY_TILE : (on_tensor_cores(dtype, hd) ? 8 * column_tiles(hd, queries) : GEN_QT);
+    return many_rows(dtype, hd, queries, walks, keys) ? MANY_TILE : (on_tensor_cores(dtype, hd) ? 8 * column_tiles(queries) : GEN_QT);
 }
 
 // groups: [n_groups][4] (first row, rows, begin, end): positions begin .. end - 1 lie in the same pages in all the group's rows, as far as a row
@@ -699,7 +698,7 @@ QNN_API int qnn_attn_decode_shared(const void* q, long long q_stride, int dtype,
     if (ring > 0 && (window <= 0 || window > ring || ring / page_size > max_pages)) return QNN_ERR_ARGUMENT;   // a ring holds no more
     const int G = nq / nkv, esize = dtype == QNN_DT_BF16 ? 2 : 4;
     const bool many = n_groups > 0 && page_size >= 64 && many_rows(dtype, hd, most_rows * G, (long long)n_groups * nkv, most_keys);
-    const int tile = many ? MANY_TILE : (on_tensor_cores(dtype, hd) ? 8 * column_tiles(hd, most_rows * G) : qnn_attn_shared_tile(dtype, hd, most_rows * G, 0, 0));
+    const int tile = many ? MANY_TILE : (on_tensor_cores(dtype, hd) ? 8 * column_tiles(most_rows * G) : qnn_attn_shared_tile(dtype, hd, most_rows * G, 0, 0));
     if (tile <= 0) return QNN_ERR_UNSUPPORTED;
     if ((q_stride * esize) % 16 || ((uintptr_t)q & 15) || ((uintptr_t)k_pool & 15) || ((uintptr_t)v_pool & 15) || ((uintptr_t)part_o & 15) ||
         ((uintptr_t)part_ml & 7) || ((uintptr_t)groups & 15) || ((uintptr_t)out & 15) || (out_stride * esize) % 16)
@@ -719,13 +718,13 @@ QNN_API int qnn_attn_decode_shared(const void* q, long long q_stride, int dtype,
             const SharedLaunch a = {q, q_stride, k_pool, v_pool, pool_rows, cells, sh, nq, nkv, hd, sc, part_o, ml, status};
             if (const int err = launch_common_tcgen05(a, st)) return err;
         }
-        const int nt = many ? column_tiles(hd, G) : tile / 8;
+        const int nt = many ? column_tiles(G) : tile / 8;
 #define QNN_MMA_AS(HDV, NTV, BIAS, BESIDE) launch_mma<HDV, NTV, BIAS, BESIDE>(q, q_stride, k_pool, v_pool, pool_rows, cells, sh, B, nq, nkv, sc, part_o, ml, status, st)
 #define QNN_MMA(HDV, NTV)                                                                                                                       \
     if (hd == HDV && nt == NTV)                                                                                                                  \
         rc = slopes != nullptr ? (many ? QNN_MMA_AS(HDV, NTV, true, true) : QNN_MMA_AS(HDV, NTV, true, false))                                   \
                                : (many ? QNN_MMA_AS(HDV, NTV, false, true) : QNN_MMA_AS(HDV, NTV, false, false));
-        QNN_MMA(64, 1) QNN_MMA(64, 2) QNN_MMA(64, 4) QNN_MMA(128, 1) QNN_MMA(128, 2) QNN_MMA(128, 4) QNN_MMA(256, 1) QNN_MMA(256, 2)
+        QNN_MMA(64, 1) QNN_MMA(64, 2) QNN_MMA(128, 1) QNN_MMA(128, 2) QNN_MMA(256, 1) QNN_MMA(256, 2)
 #undef QNN_MMA
 #undef QNN_MMA_AS
     } else {

@@ -2385,7 +2385,7 @@ def shared_attention_plan(dtype: torch.dtype, n_rows: int, n_heads: int, n_kv: i
                 t = longest + cost
                 if common * s + alone * p > resident:
                     t = max(t, (common * (keys + s * cost) + alone * (own + p * cost)) / resident + longest / 2)
-                t += parts * (s + p)
+                t += parts * (s + p) + 33.0 * min(common * s + alone * p, resident) / sms      # (an SM starts its CTAs one after another)
                 if best is None or t < best[0] * 0.999:
                     best = (t, s, p)
             ranges = best[1:]
