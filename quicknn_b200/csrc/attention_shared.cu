@@ -39,7 +39,8 @@ __device__ __forceinline__ int load_pages(const Item& it, const Cells& c, int* p
 //     S^T[16 keys x 8 q] = K Q^T,    O^T[hd x 8 q] += V^T P^T,
 // here with NT column tiles (8 NT queries) for every fragment of K and V that ldmatrix brings.  A warp walks its own tiles of 16 keys: one
 // lane asks the copy engine for them (a tile lies within a page; boxes of 64 elements x 16 positions, 128-byte swizzle, so that ldmatrix does
-// not conflict), STAGES deep, an mbarrier each.  Nothing but the last merge is shared between the warps of a CTA.  P^T is the transpose
+// not conflict), STAGES deep, an mbarrier each.  (Rows copied one by one to padded rows, without a tensor map: 16 x 4 rows under a window of
+// 4096 126 us instead of 93; cp.async by every lane 114.)  Nothing but the last merge is shared between the warps of a CTA.  P^T is the transpose
 // of S^T's accumulator, eight by eight (movmatrix).  The exponentials are taken against a reference that is raised only when a score
 // exceeds it by more than 8 (in log2): the stale reference cancels in the division, P stays below 2^8.
 constexpr float REFERENCE_STEP = 8.f;

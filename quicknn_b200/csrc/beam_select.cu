@@ -36,26 +36,26 @@ __device__ __forceinline__ int segment_start(const float* row, int s, int segmen
 // Bound by memory, and by how much of it a short kernel keeps in flight: 80 rows of 255,029 (82 MB, 12.5 us at the copy rate), us, by segment and
 // loads: 512, 4 bytes a lane 21.5; 1024, 16 bytes 19.6; the same with the fast exponentials 17.3 (torch's amax alone: 24.7).
 template <int SEGMENT>
-__global__ void __launch_bounds__(256, SEGMENT >= 1024 ? 2 : 4)
-beam_segments_kernel(const float* __restrict__ logits, int V, int segments, int total, float2* __restrict__ stats, int* __restrict__ error_flag) {
-    constexpr int PER = SEGMENT / 128;                        // 16-byte pieces a lane
-    pdl_wait();
-    const int lane = threadIdx.x & 31, warps = gridDim.x * 8;
+struct Segment {
+    static constexpr int PER = SEGMENT / 128;                 // 16-byte pieces a lane
     float4 ahead[PER];
-    const auto place = [&](int i, const float*& row) {
+
+    __device__ __forceinline__ static int place(const float* logits, int V, int segments, int i, const float*& row) {
         const int r = i / segments;
         row = logits + (size_t)r * V;
         return segment_start(row, i - r * segments, SEGMENT);
-    };
-    const auto ask = [&](int i) {
+    }
+    // asks for segment i's logits
+    __device__ __forceinline__ void ask(const float* __restrict__ logits, int V, int segments, int total, int i) {
         if (i >= total) return;
+        const int lane = threadIdx.x & 31;
         const float* row;
-        const int v0 = place(i, row);
+        const int v0 = place(logits, V, segments, i, row);
         if (v0 >= 0 && v0 + SEGMENT <= V) {
             const float4* p = reinterpret_cast<const float4*>(row + v0) + lane;
 #pragma unroll
             for (int j = 0; j < PER; ++j) ahead[j] = p[j * 32];
-        } else {                                              // outside the row: its nearest logit, taken out below
+        } else {                                              // outside the row: its nearest logit, taken out later
 #pragma unroll
             for (int j = 0; j < PER; ++j) {
                 float x[4];
@@ -64,10 +64,10 @@ beam_segments_kernel(const float* __restrict__ logits, int V, int segments, int 
                 ahead[j] = make_float4(x[0], x[1], x[2], x[3]);
             }
         }
-    };
-    int i = blockIdx.x * 8 + (threadIdx.x >> 5);
-    ask(i);
-    for (; i < total; i += warps) {
+    }
+    // the maximum and sum of segment i, whose logits are here, and asks for those of segment `next`
+    __device__ __forceinline__ float2 stats(const float* __restrict__ logits, int V, int segments, int total, int i, int next, int* __restrict__ error_flag) {
+        const int lane = threadIdx.x & 31;
         float z[PER * 4];
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
@@ -76,9 +76,9 @@ beam_segments_kernel(const float* __restrict__ logits, int V, int segments, int 
             z[j * 4 + 2] = ahead[j].z;
             z[j * 4 + 3] = ahead[j].w;
         }
-        ask(i + warps);
+        ask(logits, V, segments, total, next);
         const float* row;
-        const int v0 = place(i, row);
+        const int v0 = place(logits, V, segments, i, row);
         float m = -CUDART_INF_F, least = CUDART_INF_F;
         if (v0 < 0 || v0 + SEGMENT > V) {
 #pragma unroll
@@ -123,7 +123,21 @@ beam_segments_kernel(const float* __restrict__ logits, int V, int segments, int 
             s = warp_sum(s);
             if (__any_sync(0xffffffffu, bad) && lane == 0 && error_flag != nullptr) atomicOr(error_flag, 1);
         }
-        if (lane == 0) stats[i] = make_float2(m, s);
+        return make_float2(m, s);
+    }
+};
+
+template <int SEGMENT>
+__global__ void __launch_bounds__(256, SEGMENT >= 1024 ? 2 : 4)
+beam_segments_kernel(const float* __restrict__ logits, int V, int segments, int total, float2* __restrict__ stats, int* __restrict__ error_flag) {
+    pdl_wait();
+    const int warps = gridDim.x * 8;
+    Segment<SEGMENT> seg;
+    int i = blockIdx.x * 8 + (threadIdx.x >> 5);
+    seg.ask(logits, V, segments, total, i);
+    for (; i < total; i += warps) {
+        const float2 ms = seg.stats(logits, V, segments, total, i, i + warps, error_flag);
+        if ((threadIdx.x & 31) == 0) stats[i] = ms;
     }
 }
 
@@ -145,7 +159,8 @@ struct Found {
     unsigned at[LIST];                        // beam * V + token
 };
 
-template <int SEGMENT>
+// ALONE: a request's logits are few enough for this block to do the first pass as well (`stats` is not used then).
+template <int SEGMENT, bool ALONE>
 __global__ void __launch_bounds__(SELECT_THREADS)
 beam_pick_kernel(const float* __restrict__ logits, int V, int beams, int take, int segments, const float* __restrict__ scores,
                  const float2* __restrict__ stats, float* __restrict__ out_scores, int* __restrict__ out_beams, int* __restrict__ out_tokens,
@@ -168,16 +183,29 @@ beam_pick_kernel(const float* __restrict__ logits, int V, int beams, int take, i
     __shared__ unsigned last_at;
     const int q = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const size_t row0 = (size_t)q * beams;
+    const float2* mine_stats = stats + row0 * segments;       // of this request's beams
+    if (ALONE) {
+        float2* here = reinterpret_cast<float2*>(best + (beams * segments + 1) / 2 * 2);
+        Segment<SEGMENT> seg;
+        const int total = beams * segments;
+        seg.ask(logits + row0 * V, V, segments, total, warp);
+        for (int i = warp; i < total; i += WARPS) {
+            const float2 ms = seg.stats(logits + row0 * V, V, segments, total, i, i + WARPS, error_flag);
+            if (lane == 0) here[i] = ms;
+        }
+        mine_stats = here;
+    }
     if (threadIdx.x == 0) {
         n_found = n_reached = 0;
         threshold_s = 1u;                     // fewer groups than wanted: all that hold anything
     }
+    if (ALONE) __syncthreads();
     // log(sum exp) of every beam, by as many warps as there are for each; a lane keeps its segments' numbers where they fit
     const int share = beams >= WARPS ? 1 : WARPS / beams;
     for (int b0 = 0; b0 < beams; b0 += WARPS / share) {
         const int b = b0 + warp / share, p = warp % share, i0 = p * 32 + lane, step = share * 32;
         const bool mine = warp / share < WARPS / share && b < beams;
-        const float2* st = stats + (row0 + (mine ? b : 0)) * segments;
+        const float2* st = mine_stats + (size_t)(mine ? b : 0) * segments;
         const double t = mine ? (double)scores[row0 + b] : 0.0;
         float2 kept[KEPT];
         float m = -CUDART_INF_F;
@@ -382,20 +410,31 @@ QNN_API int qnn_beam_select(const float* logits, const float* scores, int reques
     if (beams < 1 || V < 1 || take < 1 || take > SELECT_MOST || ((uintptr_t)logits & 3)) return QNN_ERR_ARGUMENT;
     if ((long long)requests * beams > 65535 || (long long)beams * V >= 0xffffffffLL) return QNN_ERR_UNSUPPORTED;
     const int rows = requests * beams, segment = segment_of(rows, V), segments = segments_of(V, segment);
-    const size_t smem = sizeof(Found) + (size_t)beams * sizeof(double) + (size_t)beams * segments * sizeof(unsigned);
+    // A block of 32 warps does it all up to 64 segments, two a warp: a launch less (4 beams x 1000 words: host 15.7 -> 13.5 us a call, device 8.0 -> 7.7)
+    const bool alone = segment == 128 && beams * segments <= 64;
+    const size_t smem = sizeof(Found) + (size_t)beams * sizeof(double) + (size_t)(beams * segments + 1) / 2 * 2 * sizeof(unsigned) +
+                        (alone ? (size_t)beams * segments * sizeof(float2) : 0);
     if (smem > 200 * 1024 || (long long)rows * segments > 0x7fffffff) return QNN_ERR_UNSUPPORTED;
     const int total = rows * segments, wave = device_sms() * (segment >= 1024 ? 2 : 4);       // blocks of the first kernel at a time
     const int blocks = (total + 7) / 8 < wave ? (total + 7) / 8 : wave;
     float2* stats = (float2*)scratch;
-#define QNN_SELECT(SEG)                                                                                                                        \
+#define QNN_PICK(SEG, ALONE)                                                                                                                   \
     {                                                                                                                                          \
         static OncePerDevice asked;                                                                                                            \
-        if (const int rc = allow_shared(asked, beam_pick_kernel<SEG>, 200 * 1024)) return rc;                                                  \
-        launch_pdl(beam_segments_kernel<SEG>, dim3(blocks), dim3(256), 0, st, logits, V, segments, total, stats, error_flag);                  \
-        launch_pdl(beam_pick_kernel<SEG>, dim3(requests), dim3(SELECT_THREADS), smem, st, logits, V, beams, take, segments, scores,             \
+        if (const int rc = allow_shared(asked, beam_pick_kernel<SEG, ALONE>, 200 * 1024)) return rc;                                           \
+        launch_pdl(beam_pick_kernel<SEG, ALONE>, dim3(requests), dim3(SELECT_THREADS), smem, st, logits, V, beams, take, segments, scores,      \
                    (const float2*)stats, out_scores, out_beams, out_tokens, status_in, error_flag);                                            \
     }
-    if (segment == 1024) QNN_SELECT(1024) else if (segment == 512) QNN_SELECT(512) else QNN_SELECT(128)
+#define QNN_SELECT(SEG)                                                                                                                        \
+    {                                                                                                                                          \
+        launch_pdl(beam_segments_kernel<SEG>, dim3(blocks), dim3(256), 0, st, logits, V, segments, total, stats, error_flag);                  \
+        QNN_PICK(SEG, false)                                                                                                                   \
+    }
+    if (alone) QNN_PICK(128, true)
+    else if (segment == 1024) QNN_SELECT(1024)
+    else if (segment == 512) QNN_SELECT(512)
+    else QNN_SELECT(128)
+#undef QNN_PICK
 #undef QNN_SELECT
     QNN_LAUNCH_CHECK();
 }
