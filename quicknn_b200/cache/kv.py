@@ -207,13 +207,17 @@ class KVCache:
             self.longest_host[slot] = self.longest_host[s]
             self._join(slot, self._family[s])
         self._lengths_dirty = True
-        states = self._all_states()
-        if states and made:
-            if states[0].is_cuda:
+        try:
+            states = self._all_states()
+            if states and made and states[0].is_cuda:
                 kernel_ops.copy_slots(states, list(sources), made)
-            else:
+            elif made:
                 for t in states:
                     t[made] = t[list(sources)]
+        except Exception:
+            for slot in made:
+                self.free(slot)
+            raise
         return made
 
     def free(self, slot: int) -> None:
@@ -274,6 +278,7 @@ class KVCache:
         for gi, g in enumerate(self.groups):
             if split[gi]:
                 self._split(g, split[gi])
+        for gi, g in enumerate(self.groups):
             for slot, extra in want[gi]:
                 start = len(g.held[slot])
                 pages = g.pool.take(extra)
@@ -307,14 +312,16 @@ class KVCache:
         new = g.pool.take(len(pages))
         old = [g.held[slot][i] for slot, i, _ in pages]
         moves = [(s, d, u) for s, d, (_, _, u) in zip(old, new, pages) if u]
-        if moves:
-            src, dst, used = (list(x) for x in zip(*moves))
-            if g.k.is_cuda:
-                kernel_ops.copy_pages(g.k, g.v, src, dst, used)
+        try:
+            if moves and g.k.is_cuda:
+                kernel_ops.copy_pages(g.k, g.v, *(list(x) for x in zip(*moves)))
             else:
-                for pool in (g.k, g.v) if g.need.values else (g.k,):
-                    for s, d, u in moves:
+                for s, d, u in moves:
+                    for pool in (g.k, g.v) if g.need.values else (g.k,):
                         pool[:, d, :, :u] = pool[:, s, :, :u]
+        except Exception:
+            g.pool.give_back(new)
+            raise
         # only now, with every copy queued, do the old pages lose a holder
         for (slot, i, _), o, n in zip(pages, old, new):
             g.held[slot][i] = n

@@ -496,13 +496,13 @@ constexpr int JOIN_WARPS = 8, MOST_PARTS = 128;
 template <typename T, int PIECES>                             // pieces of 128 elements that a head has, at most
 __global__ void __launch_bounds__(JOIN_WARPS * 32)
 attn_shared_join_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml, T* __restrict__ out, size_t out_stride, int outputs, int nq,
-                        int hd, int S, int P, int warps, const int* __restrict__ row_group, const int* __restrict__ slots, const float* __restrict__ sinks) {
+                        int hd, const Shared sh, int warps, const int* __restrict__ slots, const float* __restrict__ sinks) {
     extern __shared__ __align__(16) float js[];               // [warps][hd] where several warps share an output
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, parts = S + P;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, S = sh.common_ranges, parts = S + sh.own_ranges;
     const int i = blockIdx.x * (JOIN_WARPS / warps) + warp / warps, wi = warp % warps;
     const bool mine = i < outputs;
     const int row = mine ? i / nq : 0, h = mine ? i % nq : 0;
-    const int from = row_group[row] >= 0 && slots[row] >= 0 ? 0 : S;      // a row of no group or no sequence has no part in C
+    const int from = sh.group_of(row).y > 0 && slots[row] >= 0 ? 0 : S;      // a row of no group or no sequence has no part in C
     pdl_wait();
     const size_t at = (size_t)(mine ? i : 0) * parts;
     float2 ml[MOST_PARTS / 32];
@@ -654,14 +654,14 @@ int launch_generic(const void* q, long long q_stride, const void* k_pool, const 
 }
 
 template <typename T>
-int launch_join(const float* part_o, const float2* part_ml, void* out, long long out_stride, int B, int nq, int hd, int S, int P, const int* row_group,
-                const int* slots, const float* sinks, cudaStream_t st) {
-    const int outputs = B * nq, warps = S + P <= 8 ? 1 : JOIN_WARPS, per = JOIN_WARPS / warps;
+int launch_join(const float* part_o, const float2* part_ml, void* out, long long out_stride, int nq, int hd, const Shared& sh, const int* slots,
+                const float* sinks, cudaStream_t st) {
+    const int outputs = sh.B * nq, warps = sh.common_ranges + sh.own_ranges <= 8 ? 1 : JOIN_WARPS, per = JOIN_WARPS / warps;
     const size_t smem = warps > 1 ? (size_t)JOIN_WARPS * hd * sizeof(float) : 0;
     const dim3 grid((outputs + per - 1) / per);
 #define QNN_JOIN(PIECES)                                                                                                                         \
-    launch_pdl(attn_shared_join_kernel<T, PIECES>, grid, dim3(JOIN_WARPS * 32), smem, st, part_o, part_ml, (T*)out, (size_t)out_stride, outputs, nq, hd, S, P, \
-               warps, row_group, slots, sinks)
+    launch_pdl(attn_shared_join_kernel<T, PIECES>, grid, dim3(JOIN_WARPS * 32), smem, st, part_o, part_ml, (T*)out, (size_t)out_stride, outputs, nq, hd, sh, \
+               warps, slots, sinks)
     if (hd <= 128) QNN_JOIN(1);
     else if (hd <= 256) QNN_JOIN(2);
     else QNN_JOIN(8);
@@ -695,6 +695,7 @@ QNN_API int qnn_attn_decode_shared(const void* q, long long q_stride, int dtype,
     if (nkv <= 0 || nkv > 65535 || nq <= 0 || nq % nkv || n_groups < 0 || most_rows < 0 || most_keys < 0 || common_ranges < 1 || own_ranges < 1 ||
         common_ranges + own_ranges > MOST_PARTS)
         return QNN_ERR_ARGUMENT;
+    if (n_groups > 0 && most_rows < 1) return QNN_ERR_ARGUMENT;
     if (page_size < 16 || (page_size & (page_size - 1)) || ring < 0 || ring % page_size) return QNN_ERR_ARGUMENT;
     if (ring > 0 && (window <= 0 || window > ring || ring / page_size > max_pages)) return QNN_ERR_ARGUMENT;   // a ring holds no more
     const int G = nq / nkv, esize = dtype == QNN_DT_BF16 ? 2 : 4;
@@ -706,7 +707,7 @@ QNN_API int qnn_attn_decode_shared(const void* q, long long q_stride, int dtype,
         return QNN_ERR_ARGUMENT;
     const Cells cells = {page_table, max_pages, 31 - __builtin_clz((unsigned)page_size), ring / page_size, slots, slot_len, window};
     const int common_tiles = (most_rows * G + tile - 1) / tile;
-    const Shared sh = {(const int4*)groups, row_group, n_groups, B, common_ranges, own_ranges, common_tiles};
+    const Shared sh = {(const int4*)groups, row_group, n_groups, B, common_ranges, own_ranges, common_tiles, most_rows};
     const int own_tile = on_tensor_cores(dtype, hd) ? 8 : GEN_QT;
     const long long items = (long long)n_groups * common_tiles * common_ranges + (long long)B * ((G + own_tile - 1) / own_tile) * own_ranges;
     const long long pool_rows = pool_pages * nkv * page_size;         // of the pools as matrices of head rows
@@ -736,6 +737,6 @@ QNN_API int qnn_attn_decode_shared(const void* q, long long q_stride, int dtype,
 #undef QNN_GENERIC
     }
     if (rc) return rc;
-    return dtype == QNN_DT_BF16 ? launch_join<bf16>(part_o, ml, out, out_stride, B, nq, hd, common_ranges, own_ranges, row_group, slots, sinks, st)
-                                : launch_join<float>(part_o, ml, out, out_stride, B, nq, hd, common_ranges, own_ranges, row_group, slots, sinks, st);
+    return dtype == QNN_DT_BF16 ? launch_join<bf16>(part_o, ml, out, out_stride, nq, hd, sh, slots, sinks, st)
+                                : launch_join<float>(part_o, ml, out, out_stride, nq, hd, sh, slots, sinks, st);
 }

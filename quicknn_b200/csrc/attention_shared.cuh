@@ -23,6 +23,21 @@ struct Shared {
     int n_groups, B;
     int common_ranges, own_ranges;            // S, P: parts 0 .. S - 1 of a row are of C, S .. S + P - 1 its own
     int common_tiles;                         // tiles of query rows of a group
+    int most_rows;
+    // Group g with the rows that the batch and the launch have room for.
+    __device__ __forceinline__ int4 group(int g) const {
+        int4 v = groups[g];
+        v.y = v.x < 0 || v.x >= B ? 0 : min(min(v.y, most_rows), B - v.x);
+        return v;
+    }
+    // The group of a row that holds it, or one without rows.
+    __device__ __forceinline__ int4 group_of(int row) const {
+        const int g = row_group[row];
+        if (g < 0 || g >= n_groups) return make_int4(0, 0, 0, 0);
+        int4 v = group(g);
+        if (row < v.x || row - v.x >= v.y) v.y = 0;
+        return v;
+    }
 };
 
 struct Cells {                                // where keys and values lie
@@ -120,7 +135,7 @@ __device__ __forceinline__ void take_range(Item& it, int tiles, int range, int r
 static __device__ Item common_item(const Shared& sh, const Cells& c, int group, int q_tile, int range, int tile, int unit = 1) {
     Item it;
     Seen all;
-    const int4 g = sh.groups[group];
+    const int4 g = sh.group(group);
     ask_slots(sh, c, all);
     ask_lengths(c, all);
     it.row0 = g.x;
@@ -146,8 +161,7 @@ static __device__ Item own_item(const Shared& sh, const Cells& c, int row, int q
     it.query0 = q_tile * tile;
     it.part = sh.common_ranges + range;
     it.slot = c.slots[row];
-    const int g = sh.row_group[row];
-    const int4 group = g >= 0 ? sh.groups[g] : make_int4(0, 0, 0, 0);
+    const int4 group = sh.group_of(row);
     ask_lengths(c, all);
     const int2 w = sees(c, it.slot);
     it.lo = w.x;
@@ -155,7 +169,7 @@ static __device__ Item own_item(const Shared& sh, const Cells& c, int row, int q
     it.a0 = w.x & ~(TILE - 1);
     it.tiles_a = 0;
     it.b0 = it.a0;
-    if (g >= 0 && it.slot >= 0) {
+    if (group.y > 0 && it.slot >= 0) {
         const int3 k = common_keys(sh, c, all, group);
         if (k.y > k.x) {                      // C lies inside what the row sees, and starts and ends with pages
             it.tiles_a = (k.x - it.a0) / TILE;

@@ -135,6 +135,31 @@ def test_rows_of_a_group(rows, nq, nkv, hd, dtype):
     b.check(b.run(hd ** -0.5, 30.0), hd ** -0.5, 30.0)
 
 
+@pytest.mark.parametrize("nq,nkv,hd,dtype", [(4, 2, 64, BF), (6, 1, 24, FP)])
+def test_batches_of_more_rows_than_are_asked_for_at_once(nq, nkv, hd, dtype):
+    groups = [(0, 192, [193 + (i * 13) % 70 for i in range(n)]) for n in (140, 3, 20)]
+    b = Batch(groups, nq, nkv, hd, dtype, alone=[50, 129], left_out=[0, 141, 163], seed=41)
+    for keys in (None, 1 << 20):
+        b.check(b.run(hd ** -0.5, 50.0, keys=keys), hd ** -0.5, 50.0)
+
+
+@pytest.mark.parametrize("nq,nkv,hd,dtype", [(8, 2, 128, BF), (4, 4, 256, BF), (6, 1, 24, FP)])
+@pytest.mark.parametrize("keys", [None, 1 << 20])
+def test_groups_that_say_too_much(nq, nkv, hd, dtype, keys):
+    # rows that the batch does not have, more rows than the launch was told of, a row whose group does not hold it, a group that is not there:
+    # such rows read their keys themselves
+    b = Batch([(0, 256, [300, 260, 270, 299, 301])], nq, nkv, hd, dtype, alone=[90], seed=43)
+    want = b.run(hd ** -0.5)
+    for groups, row_group, rows in (([(0, 99, 0, 256)], [0] * 5 + [-1], 8), ([(0, 5, 0, 256)], [0] * 5 + [-1], 3), ([(1, 3, 0, 256)], [0] * 6, 4),
+                                    ([(-2, 4, 0, 256), (6, 2, 0, 256), (0, 2, 0, 256)], [2, 2, 0, 1, 7, -5], 4)):
+        sh = ops.SharedKeys(b.i32(groups), b.i32(row_group), rows=rows, keys=keys or 256, own=301)
+        plan = ops.shared_attention_plan(dtype, b.B, nq, nkv, hd, sh)
+        scratch = torch.full((plan.scratch_bytes // 4,), float("nan"), device=DEV)
+        got = ops.attn_decode_shared(b.qkv, nq, nkv, hd, b.k, b.v, b.i32(b.table), PAGE, 0, b.i32(b.slots), b.i32(b.slot_len), sh, hd ** -0.5, None, None, plan, scratch)
+        b.check(got, hd ** -0.5)
+    b.check(want, hd ** -0.5)
+
+
 @pytest.mark.parametrize("pages", [1, 2, 3, 6, 7])
 @pytest.mark.parametrize("nq,nkv,hd", [(8, 4, 256), (9, 1, 256), (8, 2, 128), (16, 2, 64)])
 @pytest.mark.parametrize("cap", [None, 50.0, 90.0])
