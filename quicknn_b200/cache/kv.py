@@ -295,14 +295,14 @@ class KVCache:
         length = int(self.lengths_host[slot])
         if new_len <= length:
             return
+        first, last = length // PAGE, (new_len - 1) // PAGE
         for gi, g in enumerate(self.groups):
-            held = g.held[slot]
-            first, last = length // PAGE, (new_len - 1) // PAGE
+            held, mine = g.held[slot], len(split[gi])
             for n in range(first, min(last, first + g.pages_per_seq) + 1):
                 i = n % g.pages_per_seq if g.ring else n
                 if i >= len(held):               # a page that is taken anew (in a ring older ones may follow)
                     continue
-                if g.pool.holders(held[i]) > 1 and not any(s == slot and j == i for s, j, _ in split[gi]):
+                if g.pool.holders(held[i]) > 1 and not any(j == i for _, j, _ in split[gi][mine:]):
                     # in a later lap of a ring the cells behind the new tokens still hold the lap before
                     again = g.ring and n >= g.pages_per_seq
                     split[gi].append((slot, i, PAGE if again else max(0, length - n * PAGE)))
@@ -397,36 +397,36 @@ class KVCache:
                 start = r
         return out
 
-    def shared_positions(self, slots: Sequence[int], runs: Sequence[Tuple[int, int]]) -> List[np.ndarray]:
-        """For every group of the cache and every run (first row, rows) of rows: the positions begin .. end - 1 that lie in the same
-        pages in all of the run's sequences, as int32 [runs, 2]; the last such stretch where a ring leaves several.  Whole pages:
-        ``end`` may lie behind what some row holds."""
-        first = np.asarray([r for r, _ in runs])
-        rows = np.concatenate([np.arange(r, r + n) for r, n in runs])
-        of = np.repeat(np.arange(len(runs)), [n for _, n in runs])
-        starts = np.concatenate([[0], np.cumsum([n for _, n in runs])[:-1]])
-        slot = np.asarray(slots)[rows]
-        shortest = np.minimum.reduceat(self.lengths_host[slot], starts)
+    def shared_positions(self, slots: Sequence[int], runs: Sequence[Tuple[int, int]]) -> List[List[Tuple[int, int]]]:
+        """For every group of the cache and every run (first row, rows) of rows: the positions (begin, end) that lie in the same pages in
+        all of the run's sequences.  Whole pages: ``end`` may lie behind what some row holds.
+
+        Sequences part where one of them first writes beside the others, and behind that place every page is somebody's own; in a
+        ring the pages in front of what the longest still holds are overwritten.  So the common pages of two sequences are a stretch
+        that begins where the longest's do, and its end is found by halving."""
+        lengths = self.lengths_host[list(slots)].tolist()
         out = []
         for g in self.groups:
-            lead = g.table_host[np.asarray(slots)[first]]                       # [runs, pages per sequence]
-            same = np.logical_and.reduceat(g.table_host[slot] == lead[of], starts) & (lead != 0)
-            n = g.pages_per_seq
-            # page numbers in the order of positions; in a ring the newest `n` of the shortest row
-            base = np.maximum((shortest - 1) // PAGE - n + 1, 0) if g.ring else np.zeros(len(runs), dtype=np.int64)
-            if g.ring:
-                same = np.take_along_axis(same, (base[:, None] + np.arange(n)) % n, axis=1)
-                last = n - 1 - np.argmax(same[:, ::-1], axis=1)                 # the last shared page, and the one behind the hole before it
-                hole = np.where((np.arange(n) < last[:, None]) & ~same, np.arange(n), -1).max(axis=1)
-                begin, end = hole + 1, last + 1
-                none = ~same.any(axis=1)
-            else:
-                begin = np.zeros(len(runs), dtype=np.int64)
-                end = np.where(same.all(axis=1), n, np.argmin(same, axis=1))
-                none = end == 0
-            both = np.stack([(base + begin) * PAGE, (base + end) * PAGE], axis=1)
-            both[none] = 0
-            out.append(both.astype(np.int32))
+            n, found = g.pages_per_seq, []
+            for first, rows in runs:
+                mine = lengths[first:first + rows]
+                start = max(0, (max(mine) - 1) // PAGE - n + 1) if g.ring else 0
+                end = (min(mine) - 1) // PAGE + 1
+                lead = g.held[slots[first]]
+                for r in range(first + 1, first + rows):
+                    held = g.held[slots[r]]
+                    if end <= start or held[(end - 1) % n] == lead[(end - 1) % n]:
+                        continue
+                    lo, hi = start, end - 1                     # page hi is not common; pages below lo are
+                    while lo < hi:
+                        mid = (lo + hi) // 2
+                        if held[mid % n] == lead[mid % n]:
+                            lo = mid + 1
+                        else:
+                            hi = mid
+                    end = lo
+                found.append((start * PAGE, end * PAGE) if end > start else (0, 0))
+            out.append(found)
         return out
 
     # ---- views ------------------------------------------------------------------------

@@ -264,32 +264,29 @@ class Engine:
         return bound, (1.0 if ratio < 1.1 else (1.25 if ratio < 1.4 else (1.6 if ratio < 1.9 else 2.2)))
 
     def _sharing(self, slots, lengths):
-        """What the rows of a decode step hold together: (bounds as ``StepSharing``, what the kernels read of it as one int32 array per
-        group of the cache, a row's group) or None.  The numbers of groups and rows are rounded up to powers of two, as the other bounds
+        """What the rows of a decode step hold together: (bounds as ``StepSharing``, what the kernels read of it for the groups of the cache
+        one after another, a row's group; int32 arrays) or None.  The numbers of groups and rows are rounded up to powers of two, as the other bounds
         are, so that a graph serves many steps."""
         runs = self.cache.families(slots)
         if not runs:
             return None
-        ranges = self.cache.shared_positions(slots, runs)
         up = lambda n: 1 << max(int(n) - 1, 0).bit_length()  # noqa: E731
         n_groups, most = up(len(runs)), up(max(n for _, n in runs))
-        row_group = np.full(len(slots), -1, np.int32)
-        tables, keys, own = [], 0, 1
-        lens = np.asarray(lengths)
+        row_group = [-1] * len(slots)
         for i, (r, n) in enumerate(runs):
-            row_group[r:r + n] = i
-        for g, ab in zip(self.cache.groups, ranges):
-            table = np.zeros((n_groups, 4), np.int32)
-            table[:len(runs), :2] = runs
-            table[:len(runs), 2:] = ab
-            tables.append(table)
-            together = np.where(row_group >= 0, (ab[:, 1] - ab[:, 0])[row_group], 0)
-            keys = max(keys, int(together.max()))
-            held = np.minimum(lens, g.need.window) if g.ring else lens
-            own = max(own, int((held - np.minimum(together, held)).max()))
-        if not tables or not keys:
+            row_group[r:r + n] = [i] * n
+        tables, keys, own = [], 0, 64
+        for g, ranges in zip(self.cache.groups, self.cache.shared_positions(slots, runs)):
+            for (r, n), (begin, end) in zip(runs, ranges):
+                tables += (r, n, begin, end)
+                keys = max(keys, end - begin)
+            tables += (0,) * (4 * (n_groups - len(runs)))
+            for length, i in zip(lengths, row_group):
+                held = min(length, g.need.window) if g.ring else length
+                own = max(own, held - (ranges[i][1] - ranges[i][0] if i >= 0 else 0))
+        if not keys:
             return None
-        return StepSharing(n_groups, most, up(keys), up(max(own, 64))), tables, row_group
+        return StepSharing(n_groups, most, up(keys), up(own)), np.asarray(tables, np.int32), np.asarray(row_group, np.int32)
 
     def _decode(self, slots, starts, tokens_dev, use_graph, tail, rows):
         n_seqs, B = len(slots), rows                 # B rows, of which the last B - n_seqs belong to no sequence
@@ -333,7 +330,7 @@ class Engine:
         pad_rows = B - n_seqs
         parts = [np.asarray(list(starts) + [0] * pad_rows, np.int32), np.asarray(list(slots) + [-1] * pad_rows, np.int32)]
         if shared is not None:
-            parts = [t.reshape(-1) for t in shared[1]] + parts + [shared[2], np.full(pad_rows, -1, np.int32)]
+            parts = [shared[1]] + parts + [shared[2], np.full(pad_rows, -1, np.int32)]
         self.cache.uploader.send(st["meta"], np.concatenate(parts))
         st["step"].tokens[:n_seqs].copy_(tokens_dev.reshape(-1))
         self.steps_run += 1

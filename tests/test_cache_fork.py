@@ -207,7 +207,24 @@ def test_random_walk(window, seed):
         except CacheFull:
             pass
         t.c.audit()
+        live = list(t.said)
+        rnd.shuffle(live)
+        live.sort(key=lambda s: t.c._family[s])
+        live = [s for s in live if t.said[s]]
+        runs = t.c.families(live)
+        for g, found in zip(t.c.groups, t.c.shared_positions(live, runs)):
+            for run, (begin, end) in zip(runs, found):
+                assert rows_hold(t.c, live, run, g, begin, end) and (end == 0 or longest_common(t.c, live, run, g) <= (end - begin) // PAGE)
     t.check()
+
+
+def longest_common(c, slots, run, g):
+    """Pages that all rows of a run hold together and that no row's ring has lost."""
+    rows = slots[run[0]:run[0] + run[1]]
+    n = g.pages_per_seq
+    first = max(0, (max(c.length(s) for s in rows) - 1) // PAGE - n + 1) if g.ring else 0
+    last = (min(c.length(s) for s in rows) - 1) // PAGE
+    return sum(len({int(g.table_host[s, p % n]) for s in rows}) == 1 for p in range(first, last + 1))
 
 
 def rows_hold(c, slots, run, g, begin, end):
@@ -238,13 +255,13 @@ def test_what_rows_share(window):
         runs = t.c.families(slots)
         got = t.c.shared_positions(slots, runs)
         for g, ab in zip(t.c.groups, got):
-            for run, (begin, end) in zip(runs, ab.tolist()):
+            for run, (begin, end) in zip(runs, ab):
                 assert begin % PAGE == 0 and end % PAGE == 0 and 0 <= begin <= end
                 assert rows_hold(t.c, slots, run, g, begin, end)
             if not g.ring:
-                assert ab.tolist() == [[0, 256], [0, 0]]                # the whole pages of what was common
+                assert ab == [(0, 256), (0, 0)]                # the whole pages of what was common
             elif round_ == 0 and window == 192:
-                assert ab[0].tolist() == [128, 256]                     # the ring's newest page is everyone's own
+                assert ab[0] == (128, 256)                     # the ring's newest page is everyone's own
     t.drop(b)
     t.drop(c)
     assert t.c.families([a, z, y]) == [(1, 2)]
@@ -257,5 +274,5 @@ def test_tables_of_rows_that_just_forked():
     a = c.allocate()
     c.extend([(a, 130)])
     b, = c.fork([a])
-    assert [x.tolist() for x in c.shared_positions([a, b], [(0, 2)])] == [[[0, 192]]] * len(c.groups)      # the partly filled page too, as yet
+    assert c.shared_positions([a, b], [(0, 2)]) == [[(0, 192)]] * len(c.groups)      # the partly filled page too, as yet
     assert np.array_equal(c.groups[0].table_host[a], c.groups[0].table_host[b])
