@@ -488,23 +488,20 @@ attn_shared_generic_kernel(const T* __restrict__ q, size_t q_stride, const T* __
 }
 
 // ---- the parts of a row joined ---------------------------------------------------------------------------------------------------
-// A warp per (row, head), or JOIN_WARPS of them where a row has many parts: warp i adds parts i, i + warps, ...; the warps' sums in ascending
-// order.  Weights are in the lanes' registers (part p: lane p % 32), the first parts are asked for before the weights are known.  Of parts
+// JOIN_WARPS warps per (row, head): warp i adds parts i, i + JOIN_WARPS, ...; then the warps' sums in ascending order.  Weights are in the lanes' registers (part p: lane p % 32), the first parts are asked for before the weights are known.  Of parts
 // without keys (l = 0) nothing counts.
 constexpr int JOIN_WARPS = 8, MOST_PARTS = 128;
 
 template <typename T, int PIECES>                             // pieces of 128 elements that a head has, at most
 __global__ void __launch_bounds__(JOIN_WARPS * 32)
-attn_shared_join_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml, T* __restrict__ out, size_t out_stride, int outputs, int nq,
-                        int hd, const Shared sh, int warps, const int* __restrict__ slots, const float* __restrict__ sinks) {
-    extern __shared__ __align__(16) float js[];               // [warps][hd] where several warps share an output
+attn_shared_join_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml, T* __restrict__ out, size_t out_stride, int nq, int hd,
+                        const Shared sh, const int* __restrict__ slots, const float* __restrict__ sinks) {
+    extern __shared__ __align__(16) float js[];               // [JOIN_WARPS][hd]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, S = sh.common_ranges, parts = S + sh.own_ranges;
-    const int i = blockIdx.x * (JOIN_WARPS / warps) + warp / warps, wi = warp % warps;
-    const bool mine = i < outputs;
-    const int row = mine ? i / nq : 0, h = mine ? i % nq : 0;
+    const int i = blockIdx.x, row = i / nq, h = i % nq;
     const int from = sh.group_of(row).y > 0 && slots[row] >= 0 ? 0 : S;      // a row of no group or no sequence has no part in C
     pdl_wait();
-    const size_t at = (size_t)(mine ? i : 0) * parts;
+    const size_t at = (size_t)i * parts;
     float2 ml[MOST_PARTS / 32];
 #pragma unroll
     for (int k = 0; k < MOST_PARTS / 32; ++k) {
@@ -516,7 +513,7 @@ attn_shared_join_kernel(const float* __restrict__ part_o, const float2* __restri
     const auto ask = [&](int p0) {
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {
-            const int p = p0 + j * warps;
+            const int p = p0 + j * JOIN_WARPS;
 #pragma unroll
             for (int k = 0; k < PIECES; ++k) {
                 const int c = k * 128 + lane * 4;
@@ -524,7 +521,7 @@ attn_shared_join_kernel(const float* __restrict__ part_o, const float2* __restri
             }
         }
     };
-    ask(from + wi);
+    ask(from + warp);
     float M = -CUDART_INF_F, sum = 0.f, w[MOST_PARTS / 32];
 #pragma unroll
     for (int k = 0; k < MOST_PARTS / 32; ++k)
@@ -541,10 +538,10 @@ attn_shared_join_kernel(const float* __restrict__ part_o, const float2* __restri
     float4 acc[PIECES];
 #pragma unroll
     for (int k = 0; k < PIECES; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int p0 = from + wi; p0 < parts; p0 += AHEAD * warps) {
+    for (int p0 = from + warp; p0 < parts; p0 += AHEAD * JOIN_WARPS) {
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {
-            const int p = p0 + j * warps;
+            const int p = p0 + j * JOIN_WARPS;
             float mine_w = 0.f;
 #pragma unroll
             for (int k = 0; k < MOST_PARTS / 32; ++k) {
@@ -560,36 +557,72 @@ attn_shared_join_kernel(const float* __restrict__ part_o, const float2* __restri
                     acc[k].w += mine_w * v[j][k].w;
                 }
         }
-        if (p0 + AHEAD * warps < parts) ask(p0 + AHEAD * warps);
+        if (p0 + AHEAD * JOIN_WARPS < parts) ask(p0 + AHEAD * JOIN_WARPS);
     }
-    if (warps > 1) {
-        float* mine_s = js + (size_t)warp * hd;
-#pragma unroll
-        for (int k = 0; k < PIECES; ++k) {
-            const int c = k * 128 + lane * 4;
-            if (c < hd) *reinterpret_cast<float4*>(mine_s + c) = acc[k];
-        }
-        __syncthreads();
-        if (mine)
-            for (int d = wi * 32 + lane; d < hd; d += warps * 32) {
-                float a = 0.f;
-                for (int x = 0; x < warps; ++x) a += js[(size_t)(warp / warps * warps + x) * hd + d];
-                out[(size_t)row * out_stride + (size_t)h * hd + d] = from_f<T>(a * inverse);
-            }
-        return;
-    }
-    if (!mine) return;
 #pragma unroll
     for (int k = 0; k < PIECES; ++k) {
         const int c = k * 128 + lane * 4;
-        if (c >= hd) continue;
-        T* dst = out + (size_t)row * out_stride + (size_t)h * hd + c;
-        const float r[4] = {acc[k].x * inverse, acc[k].y * inverse, acc[k].z * inverse, acc[k].w * inverse};
-        if constexpr (sizeof(T) == 2) {
-            *reinterpret_cast<uint2*>(dst) = make_uint2(tc::pack_bf16(r[0], r[1]), tc::pack_bf16(r[2], r[3]));
-        } else {
-            *reinterpret_cast<float4*>(dst) = make_float4(r[0], r[1], r[2], r[3]);
-        }
+        if (c < hd) *reinterpret_cast<float4*>(js + (size_t)warp * hd + c) = acc[k];
+    }
+    __syncthreads();
+    for (int d = threadIdx.x; d < hd; d += blockDim.x) {
+        float a = 0.f;
+#pragma unroll
+        for (int x = 0; x < JOIN_WARPS; ++x) a += js[(size_t)x * hd + d];
+        out[(size_t)row * out_stride + (size_t)h * hd + d] = from_f<T>(a * inverse);
+    }
+}
+
+// The same where a row has few parts: a thread per four elements of an output, which asks for all of them at once (a part that nobody has written is
+// read all the same and does not count).  59,520 outputs of 64 from two parts: 46 us with a
+// warp each, 13 so.
+constexpr int FEW_PARTS = 8;
+
+template <typename T, int PARTS>                              // at most
+__global__ void __launch_bounds__(JOIN_WARPS * 32)
+attn_shared_join_few_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml, T* __restrict__ out, size_t out_stride, long long pieces, int nq,
+                            int hd, const Shared sh, const int* __restrict__ slots, const float* __restrict__ sinks) {
+    const long long x = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+    const int chunks = hd / 4, S = sh.common_ranges, parts = S + sh.own_ranges;
+    const bool mine = x < pieces;
+    const long long i = mine ? x / chunks : 0;
+    const int c = mine ? (int)(x - i * chunks) * 4 : 0, row = (int)(i / nq), h = (int)(i - (long long)row * nq);
+    const int from = sh.group_of(row).y > 0 && slots[row] >= 0 ? 0 : S;      // a row of no group or no sequence has no part in C
+    const float sink = sinks != nullptr ? sinks[h] * LOG2E : -CUDART_INF_F;
+    pdl_wait();
+    if (!mine) return;
+    const size_t at = (size_t)i * parts;
+    float2 ml[PARTS];
+    float4 v[PARTS];
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+        ml[p] = p < parts ? part_ml[at + p] : make_float2(-CUDART_INF_F, 0.f);
+        v[p] = p < parts ? *reinterpret_cast<const float4*>(part_o + (at + p) * hd + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    float M = -CUDART_INF_F, sum = 0.f;
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+        if (p < from) ml[p] = make_float2(-CUDART_INF_F, 0.f);
+        if (ml[p].y != 0.f) M = fmaxf(M, ml[p].x);
+    }
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+        const float w = ml[p].y != ml[p].y ? ml[p].y : (ml[p].y != 0.f ? exp2f(ml[p].x - M) : 0.f);   // a NaN among the scores has to come out
+        if (w == 0.f) continue;
+        sum += w * ml[p].y;
+        acc.x += w * v[p].x;
+        acc.y += w * v[p].y;
+        acc.z += w * v[p].z;
+        acc.w += w * v[p].w;
+    }
+    const float inverse = sum != 0.f ? 1.f / (sum + exp2f(sink - M)) : 0.f;
+    T* dst = out + (size_t)row * out_stride + (size_t)h * hd + c;
+    const float r[4] = {acc.x * inverse, acc.y * inverse, acc.z * inverse, acc.w * inverse};
+    if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<uint2*>(dst) = make_uint2(tc::pack_bf16(r[0], r[1]), tc::pack_bf16(r[2], r[3]));
+    } else {
+        *reinterpret_cast<float4*>(dst) = make_float4(r[0], r[1], r[2], r[3]);
     }
 }
 
@@ -656,12 +689,23 @@ int launch_generic(const void* q, long long q_stride, const void* k_pool, const 
 template <typename T>
 int launch_join(const float* part_o, const float2* part_ml, void* out, long long out_stride, int nq, int hd, const Shared& sh, const int* slots,
                 const float* sinks, cudaStream_t st) {
-    const int outputs = sh.B * nq, warps = sh.common_ranges + sh.own_ranges <= 8 ? 1 : JOIN_WARPS, per = JOIN_WARPS / warps;
-    const size_t smem = warps > 1 ? (size_t)JOIN_WARPS * hd * sizeof(float) : 0;
-    const dim3 grid((outputs + per - 1) / per);
+    const int outputs = sh.B * nq, parts = sh.common_ranges + sh.own_ranges;
+    if (parts <= FEW_PARTS) {
+        const long long pieces = (long long)outputs * (hd / 4);
+        const dim3 blocks((unsigned)((pieces + JOIN_WARPS * 32 - 1) / (JOIN_WARPS * 32)));
+#define QNN_JOIN(PARTS)                                                                                                                          \
+    launch_pdl(attn_shared_join_few_kernel<T, PARTS>, blocks, dim3(JOIN_WARPS * 32), 0, st, part_o, part_ml, (T*)out, (size_t)out_stride, pieces, nq, hd, sh, \
+               slots, sinks)
+        if (parts <= 2) QNN_JOIN(2);
+        else if (parts <= 4) QNN_JOIN(4);
+        else QNN_JOIN(FEW_PARTS);
+#undef QNN_JOIN
+        return (int)cudaGetLastError();
+    }
+    const size_t smem = (size_t)JOIN_WARPS * hd * sizeof(float);
 #define QNN_JOIN(PIECES)                                                                                                                         \
-    launch_pdl(attn_shared_join_kernel<T, PIECES>, grid, dim3(JOIN_WARPS * 32), smem, st, part_o, part_ml, (T*)out, (size_t)out_stride, outputs, nq, hd, sh, \
-               warps, slots, sinks)
+    launch_pdl(attn_shared_join_kernel<T, PIECES>, dim3(outputs), dim3(JOIN_WARPS * 32), smem, st, part_o, part_ml, (T*)out, (size_t)out_stride, nq, hd, sh, \
+               slots, sinks)
     if (hd <= 128) QNN_JOIN(1);
     else if (hd <= 256) QNN_JOIN(2);
     else QNN_JOIN(8);

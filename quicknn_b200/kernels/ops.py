@@ -2317,7 +2317,7 @@ class SharedKeys:
 
     ``groups`` (int32, [groups, 4] on the device): first row, number of rows, first position, position behind the last; the page
     tables of these rows name the same pages for those positions, as far as a row still holds them.  ``row_group`` (int32, one per row):
-    a row's group, or -1.  ``rows``, ``keys`` and ``own`` bound the rows of a group, the positions of a group and the keys that a row has
+    a row's group, or -1; a row is in one group at most.  ``rows``, ``keys`` and ``own`` bound the rows of a group, the positions of a group and the keys that a row has
     beside them: host numbers, from which the work is divided (``rows`` must hold; the others are a matter of speed)."""
 
     __slots__ = ("groups", "row_group", "n_groups", "rows", "keys", "own")
@@ -2359,7 +2359,9 @@ def shared_attention_plan(dtype: torch.dtype, n_rows: int, n_heads: int, n_kv: i
     if ranges is None:
         keys, own = max(shared.keys, 1), max(shared.own, 1)
         if window:
-            keys, own = min(keys, window), min(own, window)
+            keys = min(keys, window)
+            if own > window:                       # a bound without the window: of what a row sees the common keys are a part
+                own = window - keys + 128
         sms = _sm_count("cuda")
         resident = sms * max(1, min(8, 512 // head_dim))                                   # CTAs at a time
         common = shared.n_groups * (-(-shared.rows * heads // tile)) * n_kv                # walks over common keys
@@ -2371,7 +2373,8 @@ def shared_attention_plan(dtype: torch.dtype, n_rows: int, n_heads: int, n_kv: i
             # by small ones on what is left, bound by memory.  As few of the former as are done in time; where own keys are few, as many
             # as make them short.
             p = min(range(1, 65), key=lambda n: _spread(alone * n, resident, own / n) + parts * n)
-            time = _spread(alone * p, resident, own / p)
+            seen = min(own, window - keys + 128) if window else own                         # (as far as the common keys leave a window any)
+            time = _spread(alone * p, resident, seen / p)
             walk = lambda n: -(-common * n // sms) * (0.25 * (-(-keys // n)) + 200.0)  # noqa: E731
             s = next((n for n in range(1, 9) if walk(n) <= 0.6 * time), 0) or min(range(1, 65), key=lambda n: walk(n) + parts * n)
             ranges = (min(s, -(-keys // 64)), p)
