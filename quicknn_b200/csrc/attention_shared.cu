@@ -350,13 +350,19 @@ attn_shared_mma_kernel(const __grid_constant__ CUtensorMap map, const KV kv, con
 }
 
 // ---- any head size, float32 or bfloat16 ----------------------------------------------------------------------------------------
-// Tiles of 32 keys as float32 in shared memory (rows an odd number of floats apart).  A warp keeps GEN_Q queries: a lane forms their scores with one
+// Tiles of 32 keys as float32 in shared memory (rows an odd number of 16-byte pieces apart).  A warp keeps GEN_Q queries: a lane forms their scores with one
 // key, the weights go to shared memory, and then the lanes take the head's elements, so that what is read of K and V serves all
 // the warp's queries.  Exact exponentials and tanh in float32.
 constexpr int GEN_WARPS = 4, GEN_Q = 4, GEN_QT = GEN_WARPS * GEN_Q;
 
+__device__ __forceinline__ float redux_max(float x) {         // the largest of the warp's that is a number
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+    return r;
+}
+
 template <typename T, int DPL>                                // elements of a head per lane, at most
-__global__ void __launch_bounds__(GEN_WARPS * 32)
+__global__ void __launch_bounds__(GEN_WARPS * 32, DPL <= 2 ? 6 : 1)
 attn_shared_generic_kernel(const T* __restrict__ q, size_t q_stride, const T* __restrict__ k_pool, const T* __restrict__ v_pool,
                            const Cells cells, const Shared sh, int nq, int nkv, int hd, int tile_keys, float scale, float cap,
                            float* __restrict__ part_o, float2* __restrict__ part_ml, const float* __restrict__ slopes) {
@@ -376,7 +382,7 @@ attn_shared_generic_kernel(const T* __restrict__ q, size_t q_stride, const T* __
     const int queries = min(GEN_QT, it.rows * G - it.query0);
     pdl_wait();
     if (queries <= 0) return;
-    const int pitch = hd + 1;
+    const int pitch = (hd / 4 | 1) * 4;
     float* sk = sm;
     float* sv = sk + tile_keys * pitch;
     float* sq = sv + tile_keys * pitch;                       // [GEN_QT][hd], times the scale; zeros for queries that are not there
@@ -412,7 +418,7 @@ attn_shared_generic_kernel(const T* __restrict__ q, size_t q_stride, const T* __
             const int j = i / chunks, c = i % chunks, p = it.position(t + j / TILE) + j % TILE;
             if (p < it.lo || p >= it.hi) {                    // zero weights, and zeros for them to meet
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) sv[j * pitch + c * VEC + e] = 0.f;
+                for (int e = 0; e < VEC; e += 4) *reinterpret_cast<float4*>(sv + j * pitch + c * VEC + e) = make_float4(0.f, 0.f, 0.f, 0.f);
                 continue;
             }
             const int pn = p >> cells.page_shift, page = table[cells.ring_pages > 0 ? pn % cells.ring_pages : pn];
@@ -424,9 +430,9 @@ attn_shared_generic_kernel(const T* __restrict__ q, size_t q_stride, const T* __
             kv.unpack(a);
             vv.unpack(b);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                sk[j * pitch + c * VEC + e] = a[e];
-                sv[j * pitch + c * VEC + e] = b[e];
+            for (int e = 0; e < VEC; e += 4) {
+                *reinterpret_cast<float4*>(sk + j * pitch + c * VEC + e) = make_float4(a[e], a[e + 1], a[e + 2], a[e + 3]);
+                *reinterpret_cast<float4*>(sv + j * pitch + c * VEC + e) = make_float4(b[e], b[e + 1], b[e + 2], b[e + 3]);
             }
         }
         __syncthreads();
@@ -439,21 +445,21 @@ attn_shared_generic_kernel(const T* __restrict__ q, size_t q_stride, const T* __
             const float* qr = sq + warp * GEN_Q * hd;
 #pragma unroll 4
             for (int d = 0; d < hd; d += 4) {
-                const float k0 = kr[d], k1 = kr[d + 1], k2 = kr[d + 2], k3 = kr[d + 3];
+                const float4 k = *reinterpret_cast<const float4*>(kr + d);
 #pragma unroll
                 for (int i = 0; i < GEN_Q; ++i) {
                     const float4 x = *reinterpret_cast<const float4*>(qr + i * hd + d);
-                    s[i] = fmaf(x.w, k3, fmaf(x.z, k2, fmaf(x.y, k1, fmaf(x.x, k0, s[i]))));
+                    s[i] = fmaf(x.w, k.w, fmaf(x.z, k.z, fmaf(x.y, k.y, fmaf(x.x, k.x, s[i]))));
                 }
             }
         }
 #pragma unroll
         for (int i = 0; i < GEN_Q; ++i) {
             s[i] = softcap_t<T>(s[i], cap) - slope[i] * (float)(newest[i] - pos);
-            const float top = fmaxf(mx[i], warp_max(valid ? s[i] : -CUDART_INF_F));
+            const float top = fmaxf(mx[i], redux_max(valid ? s[i] : -CUDART_INF_F));
             const float keep = mx[i] == -CUDART_INF_F ? 0.f : fexp<T>(mx[i] - top);
             w[i] = valid && (top != -CUDART_INF_F || s[i] != s[i]) ? fexp<T>(s[i] - top) : 0.f;
-            l[i] = l[i] * keep + warp_sum(w[i]);
+            l[i] = l[i] * keep + w[i];                        // the lane's keys
             mx[i] = top;
 #pragma unroll
             for (int d = 0; d < DPL; ++d) o[i][d] *= keep;
@@ -479,6 +485,7 @@ attn_shared_generic_kernel(const T* __restrict__ q, size_t q_stride, const T* __
         const int m = warp * GEN_Q + i;
         if (m >= queries) break;
         const size_t at = part_of(it, sh, it.query0 + m, kh, G, nq);
+        l[i] = warp_sum(l[i]);
         if (l[i] > 0.f || l[i] != l[i])                       // (a NaN among the scores has to come out)
 #pragma unroll
             for (int d = 0; d < DPL; ++d)
@@ -677,7 +684,7 @@ template <typename T, int DPL>
 int launch_generic(const void* q, long long q_stride, const void* k_pool, const void* v_pool, const Cells& cells, const Shared& sh, int items, int nq,
                    int nkv, int hd, float scale, float cap, float* part_o, float2* part_ml, const float* slopes, cudaStream_t st) {
     const int keys = hd <= 512 ? 32 : 16;
-    const size_t smem = ((size_t)2 * keys * (hd + 1) + (size_t)GEN_QT * hd + GEN_WARPS * 32 * 4) * sizeof(float);
+    const size_t smem = ((size_t)2 * keys * ((hd / 4) | 1) * 4 + (size_t)GEN_QT * hd + GEN_WARPS * 32 * 4) * sizeof(float);
     auto kern = attn_shared_generic_kernel<T, DPL>;
     static OncePerDevice asked;
     if (const int rc = allow_shared(asked, kern, 220 * 1024)) return rc;
@@ -776,8 +783,8 @@ QNN_API int qnn_attn_decode_shared(const void* q, long long q_stride, int dtype,
     } else {
 #define QNN_GENERIC(T, DPLV) \
     launch_generic<T, DPLV>(q, q_stride, k_pool, v_pool, cells, sh, (int)items, nq, nkv, hd, scale, cap, part_o, ml, slopes, st)
-        if (dtype == QNN_DT_BF16) rc = hd <= 64 ? QNN_GENERIC(bf16, 2) : (hd <= 256 ? QNN_GENERIC(bf16, 8) : QNN_GENERIC(bf16, 32));
-        else rc = hd <= 64 ? QNN_GENERIC(float, 2) : (hd <= 256 ? QNN_GENERIC(float, 8) : QNN_GENERIC(float, 32));
+        if (dtype == QNN_DT_BF16) rc = hd <= 32 ? QNN_GENERIC(bf16, 1) : hd <= 64 ? QNN_GENERIC(bf16, 2) : (hd <= 256 ? QNN_GENERIC(bf16, 8) : QNN_GENERIC(bf16, 32));
+        else rc = hd <= 32 ? QNN_GENERIC(float, 1) : hd <= 64 ? QNN_GENERIC(float, 2) : (hd <= 256 ? QNN_GENERIC(float, 8) : QNN_GENERIC(float, 32));
 #undef QNN_GENERIC
     }
     if (rc) return rc;

@@ -2363,7 +2363,8 @@ def shared_attention_plan(dtype: torch.dtype, n_rows: int, n_heads: int, n_kv: i
             if own > window:                       # a bound without the window: of what a row sees the common keys are a part
                 own = window - keys + 128
         sms = _sm_count("cuda")
-        resident = sms * max(1, min(8, 512 // head_dim))                                   # CTAs at a time
+        tensor_cores = dtype == torch.bfloat16 and head_dim in (64, 128, 256)
+        resident = sms * (min(8, 512 // head_dim) if tensor_cores else 6 if head_dim <= 64 else 2 if head_dim <= 256 else 1)      # CTAs at a time
         common = shared.n_groups * (-(-shared.rows * heads // tile)) * n_kv                # walks over common keys
         alone = n_rows * (-(-heads // tile)) * n_kv                                        # walks over own keys
         # the times below are in keys of a walk; the parts are written and read as float32
@@ -2379,7 +2380,7 @@ def shared_attention_plan(dtype: torch.dtype, n_rows: int, n_heads: int, n_kv: i
             s = next((n for n in range(1, 9) if walk(n) <= 0.6 * time), 0) or min(range(1, 65), key=lambda n: walk(n) + parts * n)
             ranges = (min(s, -(-keys // 64)), p)
         else:
-            best, cost = None, SHARED_ITEM_COST / (1 if dtype == torch.bfloat16 and head_dim in (64, 128, 256) else 4)
+            best, cost = None, SHARED_ITEM_COST / (1 if tensor_cores else 4)
             for c in _SHARED_CHUNKS:
                 s, p = -(-keys // c), -(-own // c)
                 if s > 64 or p > 64:
