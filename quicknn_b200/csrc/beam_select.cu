@@ -7,8 +7,9 @@
 // Within a beam the order of the scores is that of the logits, so one pass over the logits is enough for everything but a few of them:
 //   1. a warp per segment of a row (SEGMENT logits) leaves the segment's maximum and sum of exp(z - maximum);
 //   2. a block per request joins them to log(sum exp) of every beam, turns the segments' maxima into scores, and takes as a threshold the
-//      `take`-th largest of 128 groups' maxima, so that at least `take` segments reach it.  As each of these holds a score that reaches it, so do the `take` best of all; they lie in the segments
-//      that reach it, which are read again (a few KB) into a short list, whose best are found by counting.
+//      `take`-th largest of 128 groups' maxima, so that at least `take` segments reach it.  As each of these holds a score that reaches it, so do
+//      the `take` best of all; they lie in the segments that reach it, which are read again (a few KB) into a short list, whose best are
+//      found by counting.  Where a request has few logits, that block does the first pass too, and the groups are of logits.
 // Scores are formed in 64 bits: those of different beams may differ by less than 32 bits resolve after a sum over the vocabulary.
 // A logit that is not finite is no continuation and not in the sum (bit 0 of the error word says so); nor is any of a beam whose score is
 // -inf or NaN.  Where fewer than `take` are left, the places behind them hold score -inf, beam -1, token -1.
@@ -21,7 +22,10 @@ using namespace qnn;
 namespace {
 
 constexpr int SELECT_MOST = 64;               // continuations per request, at most
-constexpr int SELECT_THREADS = 1024;
+// Of the second kernel's block.  It is short code that every warp runs once, so what it takes is instructions times warps: 4 beams x 1000 words 6.2 us with
+// 512, 7.7 with 1024; 10 beams x 1015 9.6 (256: 13).  Of its 11,000 cycles (8 beams x 99,521) 4,500 go to the logarithms of the sums, 2,000 to the
+// threshold, 3,000 to the second look, 1,500 to the order.
+constexpr int THREADS = 512;
 constexpr int LIST = 2048;                    // places of the short list
 constexpr int MOST_REACHED = 512;             // segments that are looked at again
 
@@ -65,8 +69,10 @@ struct Segment {
             }
         }
     }
-    // the maximum and sum of segment i, whose logits are here, and asks for those of segment `next`
-    __device__ __forceinline__ float2 stats(const float* __restrict__ logits, int V, int segments, int total, int i, int next, int* __restrict__ error_flag) {
+    // the maximum and sum of segment i, whose logits are here, and asks for those of segment `next`; `keep`: a place for the logits, -inf for
+    // those that do not count
+    __device__ __forceinline__ float2 stats(const float* __restrict__ logits, int V, int segments, int total, int i, int next, int* __restrict__ error_flag,
+                                            float4* __restrict__ keep = nullptr) {
         const int lane = threadIdx.x & 31;
         float z[PER * 4];
 #pragma unroll
@@ -123,6 +129,9 @@ struct Segment {
             s = warp_sum(s);
             if (__any_sync(0xffffffffu, bad) && lane == 0 && error_flag != nullptr) atomicOr(error_flag, 1);
         }
+        if (keep != nullptr)
+#pragma unroll
+            for (int j = 0; j < PER; ++j) keep[j * 32 + lane] = make_float4(z[j * 4], z[j * 4 + 1], z[j * 4 + 2], z[j * 4 + 3]);
         return make_float2(m, s);
     }
 };
@@ -146,22 +155,45 @@ __device__ __forceinline__ double warp_sum(double v) {
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
-// finite floats as unsigned numbers of the same order
-__device__ __forceinline__ unsigned ordered(float f) {
-    const unsigned u = __float_as_uint(f);
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
-}
-__device__ __forceinline__ float unordered(unsigned u) { return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u); }
+// a score in 32 bits, finite
+__device__ __forceinline__ float rounded(double score) { return fmaxf((float)score, -FLT_MAX); }
 __device__ __forceinline__ bool before(double a, unsigned ia, double b, unsigned ib) { return a > b || (a == b && ia < ib); }
+
+// The `take`-th largest of 128 groups' maxima, value i of n in group i % 128, found by counting, into `result` (which stays as it is where
+// fewer groups hold anything above -inf).  By the whole block; what it reads is written, and what it writes is there, in all threads.
+constexpr int GROUPS = 128;
+template <typename F>
+__device__ __forceinline__ void nth_of_groups(int n, int take, F value, float* group_best, float& result) {
+    constexpr int EACH = THREADS / GROUPS;    // threads a group
+    const int g = threadIdx.x / EACH, e = threadIdx.x % EACH;
+    __syncthreads();
+    float most = -CUDART_INF_F;
+    for (int i = g + e * GROUPS; i < n; i += THREADS) most = fmaxf(most, value(i));
+#pragma unroll
+    for (int o = 1; o < EACH; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (e == 0) group_best[g] = most;
+    __syncthreads();
+    int rank = 0;                             // each of a group's threads counts against its share
+#pragma unroll 16
+    for (int o = e; o < GROUPS; o += EACH) {
+        const float other = group_best[o];
+        rank += other > most || (other == most && o < g);
+    }
+#pragma unroll
+    for (int o = 1; o < EACH; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+    if (rank == take - 1 && e == 0 && most > -CUDART_INF_F) result = most;
+    __syncthreads();
+}
 
 struct Found {
     double score[LIST];
     unsigned at[LIST];                        // beam * V + token
 };
 
-// ALONE: a request's logits are few enough for this block to do the first pass as well (`stats` is not used then).
+// ALONE: a request's logits are few enough for this block to do the first pass as well (`stats` is not used then), and to keep them: the threshold
+// is that of groups of single logits (of a few segments' maxima it would be a low one and let thousands pass).
 template <int SEGMENT, bool ALONE>
-__global__ void __launch_bounds__(SELECT_THREADS)
+__global__ void __launch_bounds__(THREADS)
 beam_pick_kernel(const float* __restrict__ logits, int V, int beams, int take, int segments, const float* __restrict__ scores,
                  const float2* __restrict__ stats, float* __restrict__ out_scores, int* __restrict__ out_beams, int* __restrict__ out_tokens,
                  const int* __restrict__ status_in, int* __restrict__ error_flag) {
@@ -173,35 +205,36 @@ beam_pick_kernel(const float* __restrict__ logits, int V, int beams, int take, i
     extern __shared__ __align__(16) unsigned char smem[];
     Found* found = reinterpret_cast<Found*>(smem);
     double* base = reinterpret_cast<double*>(found + 1);      // [beams] t_b - log(sum exp)
-    unsigned* best = reinterpret_cast<unsigned*>(base + beams);   // [beams * segments] the segments' best scores, ordered
-    constexpr int WARPS = SELECT_THREADS / 32, GROUPS = 128, KEPT = 4;
+    float* best = reinterpret_cast<float*>(base + (beams + 1) / 2 * 2);   // [beams * segments] the segments' best scores; -inf: none
+    constexpr int WARPS = THREADS / 32, KEPT = 4;
     __shared__ float part_m[WARPS];
     __shared__ double part_s[WARPS];
-    __shared__ unsigned group_best[GROUPS], threshold_s;
+    __shared__ float group_best[GROUPS], threshold_s;
     __shared__ int reached[MOST_REACHED], n_reached, n_found;
     __shared__ double last_score;
     __shared__ unsigned last_at;
     const int q = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const size_t row0 = (size_t)q * beams;
     const float2* mine_stats = stats + row0 * segments;       // of this request's beams
+    float4* logits_here = reinterpret_cast<float4*>(best + (beams * segments + 3) / 4 * 4);
+    float2* here = reinterpret_cast<float2*>(logits_here + beams * segments * (SEGMENT / 4));
     if (ALONE) {
-        float2* here = reinterpret_cast<float2*>(best + (beams * segments + 1) / 2 * 2);
         Segment<SEGMENT> seg;
         const int total = beams * segments;
         seg.ask(logits + row0 * V, V, segments, total, warp);
         for (int i = warp; i < total; i += WARPS) {
-            const float2 ms = seg.stats(logits + row0 * V, V, segments, total, i, i + WARPS, error_flag);
+            const float2 ms = seg.stats(logits + row0 * V, V, segments, total, i, i + WARPS, error_flag, logits_here + i * (SEGMENT / 4));
             if (lane == 0) here[i] = ms;
         }
         mine_stats = here;
     }
     if (threadIdx.x == 0) {
         n_found = n_reached = 0;
-        threshold_s = 1u;                     // fewer groups than wanted: all that hold anything
+        threshold_s = -FLT_MAX;               // fewer groups than wanted: all that hold anything
     }
     if (ALONE) __syncthreads();
-    // log(sum exp) of every beam, by as many warps as there are for each; a lane keeps its segments' numbers where they fit
-    const int share = beams >= WARPS ? 1 : WARPS / beams;
+    // log(sum exp) of every beam, by a warp each or, where it has many segments, by as many as there are; a lane keeps its segments' numbers where they fit
+    const int share = max(1, min(WARPS / beams, (segments + 32 * KEPT - 1) / (32 * KEPT)));
     for (int b0 = 0; b0 < beams; b0 += WARPS / share) {
         const int b = b0 + warp / share, p = warp % share, i0 = p * 32 + lane, step = share * 32;
         const bool mine = warp / share < WARPS / share && b < beams;
@@ -237,12 +270,15 @@ beam_pick_kernel(const float* __restrict__ logits, int V, int beams, int take, i
             if (mine)
                 for (int i = 0; i < share; ++i) s += part_s[warp / share * share + i];
         }
+        // (one lane a beam takes the logarithm, which is long in 64 bits)
+        if (mine && p == 0 && lane == 0) base[b] = m != -CUDART_INF_F && t > -CUDART_INF && t < CUDART_INF ? t - (double)m - log(s) : -CUDART_INF;
+        __syncthreads();
         if (mine) {
-            const bool alive = m != -CUDART_INF_F && t > -CUDART_INF && t < CUDART_INF;
-            const double add = alive ? t - (double)m - log(s) : -CUDART_INF;
-            if (p == 0 && lane == 0) base[b] = add;
+            const double add = base[b];
             const auto note = [&](int i, float z) {
-                best[b * segments + i] = alive && z != -CUDART_INF_F ? ordered((float)(add + (double)z)) : 0u;      // 0: none
+                const bool holds = add != -CUDART_INF && z != -CUDART_INF_F;
+                best[b * segments + i] = holds ? rounded(add + (double)z) : -CUDART_INF_F;
+                if (ALONE) here[b * segments + i].x = holds ? (float)add : -CUDART_INF_F;       // (nobody else reads these numbers)
             };
 #pragma unroll
             for (int k = 0; k < KEPT; ++k)
@@ -251,65 +287,84 @@ beam_pick_kernel(const float* __restrict__ logits, int V, int beams, int take, i
         }
         if (b0 + WARPS / share < beams) __syncthreads();      // the partial results have been read
     }
-    // The threshold: segment i is in group i % 128; the `take`-th largest of the groups' maxima (found by counting).
     const int n = beams * segments;
-    __syncthreads();
-    unsigned most = 0u;                       // eight threads a group
-    for (int i = (threadIdx.x >> 3) + (threadIdx.x & 7) * GROUPS; i < n; i += SELECT_THREADS) most = max(most, best[i]);
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, 4));
-    if ((threadIdx.x & 7) == 0) group_best[threadIdx.x >> 3] = most;
-    __syncthreads();
-    {
-        const int g = threadIdx.x >> 3;       // each of the eight counts against an eighth
-        const unsigned top = most;
-        int rank = 0;
+    // Logits of a beam below this are out, whatever the roundings (of those that are not, the scores are formed in 64 bits).
+    const auto limit_of = [&](double add, float threshold) {
+        const double top = (double)threshold, exactly = top - add;
+        return threshold > -FLT_MAX ? rounded(exactly - 1e-5 * (fabs(exactly) + fabs(top))) : -FLT_MAX;
+    };
+    if (ALONE) nth_of_groups(n * SEGMENT, take, [&](int i) { return fminf(here[i / SEGMENT].x + reinterpret_cast<const float*>(logits_here)[i], FLT_MAX); },
+                             group_best, threshold_s);
+    else nth_of_groups(n, take, [&](int i) { return best[i]; }, group_best, threshold_s);
+    const float threshold = threshold_s;
+    if (ALONE) {
+        for (int l = warp; l < n; l += WARPS) {
+            if (best[l] == -CUDART_INF_F) continue;
+            const int b = l / segments;
+            const double add = base[b];
+            const float limit = limit_of(add, threshold);
+            const int v0 = segment_start(logits + (row0 + b) * V, l - b * segments, SEGMENT);
 #pragma unroll
-        for (int j = 0; j < GROUPS / 8; ++j) {
-            const int o = j * 8 + (threadIdx.x & 7);
-            const unsigned other = group_best[o];
-            rank += other > top || (other == top && o < g);
+            for (int j = 0; j < SEGMENT / 32; ++j) {
+                const float z = reinterpret_cast<const float*>(logits_here)[l * SEGMENT + j * 32 + lane];
+                if (!(z >= limit)) continue;                  // (limit is finite, what is no continuation -inf)
+                const int at = atomicAdd(&n_found, 1);
+                if (at < LIST) {
+                    found->score[at] = add + (double)z;
+                    found->at[at] = (unsigned)b * (unsigned)V + (unsigned)(v0 + j * 32 + lane);
+                }
+            }
         }
-        rank += __shfl_xor_sync(0xffffffffu, rank, 1);
-        rank += __shfl_xor_sync(0xffffffffu, rank, 2);
-        rank += __shfl_xor_sync(0xffffffffu, rank, 4);
-        if (rank == take - 1 && (threadIdx.x & 7) == 0 && top > 1u) threshold_s = top;
-    }
-    __syncthreads();
-    const unsigned threshold = threshold_s;
-    const float threshold_f = unordered(threshold);
-    for (int i = threadIdx.x; i < n; i += SELECT_THREADS)
-        if (best[i] >= threshold) {
-            const int at = atomicAdd(&n_reached, 1);
-            if (at < MOST_REACHED) reached[at] = i;
-        }
-    __syncthreads();
-    // (of more than the list holds every segment is looked at)
-    const int n_look = n_reached <= MOST_REACHED ? n_reached : n;
-    for (int l = warp; l < n_look; l += WARPS) {
-        const int i = n_reached <= MOST_REACHED ? reached[l] : l;
-        if (best[i] < threshold) continue;
-        const int b = i / segments;
-        const float* row = logits + (row0 + b) * V;
-        const int v0 = segment_start(row, i - b * segments, SEGMENT);
-        const double add = base[b];
-        // logits below this are out, whatever the roundings (most of them, and the others are looked at in 64 bits)
-        const double exactly = (double)threshold_f - add;
-        const float limit = threshold > 1u ? (float)(exactly - 1e-5 * (fabs(exactly) + fabs((double)threshold_f))) : -CUDART_INF_F;
-        float z[SEGMENT / 32];
+    } else {
+        for (int i = threadIdx.x; i < n; i += THREADS)
+            if (best[i] >= threshold) {
+                const int at = atomicAdd(&n_reached, 1);
+                if (at < MOST_REACHED) reached[at] = i;
+            }
+        __syncthreads();
+        // (of more than the list holds every segment is looked at)
+        const int n_look = n_reached <= MOST_REACHED ? n_reached : n;
+        for (int l = warp; l < n_look; l += WARPS) {
+            const int i = n_reached <= MOST_REACHED ? reached[l] : l;
+            if (best[i] < threshold) continue;
+            const int b = i / segments;
+            const float* row = logits + (row0 + b) * V;
+            const int v0 = segment_start(row, i - b * segments, SEGMENT);
+            const double add = base[b];
+            const float limit = limit_of(add, threshold);
+            float4 z[SEGMENT / 128];
+            const bool whole = v0 >= 0 && v0 + SEGMENT <= V;
+            if (whole) {
+                const float4* src = reinterpret_cast<const float4*>(row + v0) + lane;
 #pragma unroll
-        for (int j = 0; j < SEGMENT / 32; ++j) z[j] = row[min(max(v0 + j * 32 + lane, 0), V - 1)];
+                for (int j = 0; j < SEGMENT / 128; ++j) z[j] = src[j * 32];
+            } else {
 #pragma unroll
-        for (int j = 0; j < SEGMENT / 32; ++j) {
-            const int v = v0 + j * 32 + lane;
-            if (v < 0 || v >= V || !isfinite(z[j]) || z[j] < limit) continue;
-            const double s = add + (double)z[j];
-            if (ordered((float)s) < threshold) continue;
-            const int at = atomicAdd(&n_found, 1);
-            if (at < LIST) {
-                found->score[at] = s;
-                found->at[at] = (unsigned)b * (unsigned)V + (unsigned)v;
+                for (int j = 0; j < SEGMENT / 128; ++j) {
+                    float x[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int v = v0 + (j * 32 + lane) * 4 + e;
+                        x[e] = v >= 0 && v < V ? row[v] : -CUDART_INF_F;
+                    }
+                    z[j] = make_float4(x[0], x[1], x[2], x[3]);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < SEGMENT / 128; ++j) {
+                if (!(fmaxf(fmaxf(z[j].x, z[j].y), fmaxf(z[j].z, z[j].w)) >= limit)) continue;      // (the maximum of those that are numbers)
+                const float x[4] = {z[j].x, z[j].y, z[j].z, z[j].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (!(x[e] >= limit) || x[e] > FLT_MAX) continue;
+                    const double s = add + (double)x[e];
+                    if (rounded(s) < threshold) continue;
+                    const int at = atomicAdd(&n_found, 1);
+                    if (at < LIST) {
+                        found->score[at] = s;
+                        found->at[at] = (unsigned)b * (unsigned)V + (unsigned)(v0 + (j * 32 + lane) * 4 + e);
+                    }
+                }
             }
         }
     }
@@ -331,7 +386,7 @@ beam_pick_kernel(const float* __restrict__ logits, int V, int beams, int take, i
                 ot[rank] = (int)(a % (unsigned)V);
             }
         }
-        for (int i = have + threadIdx.x; i < take; i += SELECT_THREADS) {
+        for (int i = have + threadIdx.x; i < take; i += THREADS) {
             os[i] = -CUDART_INF_F;
             ob[i] = ot[i] = -1;
         }
@@ -342,7 +397,7 @@ beam_pick_kernel(const float* __restrict__ logits, int V, int beams, int take, i
     for (int k = 0; k < take; ++k) {
         double s_best = -CUDART_INF;
         unsigned a_best = 0xffffffffu;
-        for (int i = warp; i < n; i += SELECT_THREADS / 32) {
+        for (int i = warp; i < n; i += THREADS / 32) {
             if (best[i] < threshold) continue;
             const int b = i / segments;
             const float* row = logits + (row0 + b) * V;
@@ -376,7 +431,7 @@ beam_pick_kernel(const float* __restrict__ logits, int V, int beams, int take, i
         }
         __syncthreads();
         if (threadIdx.x == 0) {
-            for (int w = 1; w < SELECT_THREADS / 32; ++w)
+            for (int w = 1; w < THREADS / 32; ++w)
                 if (before(found->score[w], found->at[w], s_best, a_best)) {
                     s_best = found->score[w];
                     a_best = found->at[w];
@@ -392,9 +447,9 @@ beam_pick_kernel(const float* __restrict__ logits, int V, int beams, int take, i
 }
 
 // Logits per segment.  Small vocabularies get short ones, so that the threshold, the `take`-th best of 128 groups, stays near the best.
-// Where 512 would give every warp of the device several, 1024 keep more in flight.
+// Where 512 would keep every warp of the device busy, 1024 leave half as many numbers behind (8 x 256,000: 10.3 us, 12.1 by 512).
 int least_segment(int V) { return V < 16384 ? 128 : 512; }
-int segment_of(int rows, int V) { return least_segment(V) == 512 && (long long)rows * V > 148LL * 32 * 512 ? 1024 : least_segment(V); }
+int segment_of(int rows, int V) { return least_segment(V) == 512 && (long long)rows * V > 148LL * 16 * 512 ? 1024 : least_segment(V); }
 int segments_of(int V, int segment) { return (V + 3 + segment - 1) / segment; }
 
 }  // namespace
@@ -410,10 +465,11 @@ QNN_API int qnn_beam_select(const float* logits, const float* scores, int reques
     if (beams < 1 || V < 1 || take < 1 || take > SELECT_MOST || ((uintptr_t)logits & 3)) return QNN_ERR_ARGUMENT;
     if ((long long)requests * beams > 65535 || (long long)beams * V >= 0xffffffffLL) return QNN_ERR_UNSUPPORTED;
     const int rows = requests * beams, segment = segment_of(rows, V), segments = segments_of(V, segment);
-    // A block of 32 warps does it all up to 64 segments, two a warp: a launch less (4 beams x 1000 words: host 15.7 -> 13.5 us a call, device 8.0 -> 7.7)
-    const bool alone = segment == 128 && beams * segments <= 64;
-    const size_t smem = sizeof(Found) + (size_t)beams * sizeof(double) + (size_t)(beams * segments + 1) / 2 * 2 * sizeof(unsigned) +
-                        (alone ? (size_t)beams * segments * sizeof(float2) : 0);
+    // One block does it all for few logits: a launch less, and a threshold from single logits.  us so and by two kernels: 4 beams x 1000, 8 best 6.2 /
+    // 8.0; 11 x 515, 22 best 9.4 / 15; 10 x 1015, 20 best 10.8 / 15.8 (where segments are few, the `take`-th of their maxima lets hundreds pass).
+    const bool alone = segment == 128 && (beams * segments <= 64 || beams * segments <= min(128, 4 * take));
+    const size_t smem = sizeof(Found) + (size_t)(beams + 1) / 2 * 2 * sizeof(double) + (size_t)(beams * segments + 3) / 4 * 4 * sizeof(unsigned) +
+                        (alone ? (size_t)beams * segments * (sizeof(float2) + 128 * sizeof(float)) : 0);
     if (smem > 200 * 1024 || (long long)rows * segments > 0x7fffffff) return QNN_ERR_UNSUPPORTED;
     const int total = rows * segments, wave = device_sms() * (segment >= 1024 ? 2 : 4);       // blocks of the first kernel at a time
     const int blocks = (total + 7) / 8 < wave ? (total + 7) / 8 : wave;
@@ -422,7 +478,7 @@ QNN_API int qnn_beam_select(const float* logits, const float* scores, int reques
     {                                                                                                                                          \
         static OncePerDevice asked;                                                                                                            \
         if (const int rc = allow_shared(asked, beam_pick_kernel<SEG, ALONE>, 200 * 1024)) return rc;                                           \
-        launch_pdl(beam_pick_kernel<SEG, ALONE>, dim3(requests), dim3(SELECT_THREADS), smem, st, logits, V, beams, take, segments, scores,      \
+        launch_pdl(beam_pick_kernel<SEG, ALONE>, dim3(requests), dim3(THREADS), smem, st, logits, V, beams, take, segments, scores,      \
                    (const float2*)stats, out_scores, out_beams, out_tokens, status_in, error_flag);                                            \
     }
 #define QNN_SELECT(SEG)                                                                                                                        \
