@@ -57,6 +57,14 @@ def test_against_a_sort(Q, W, V, take):
     check(*data(Q, W, V, Q + W + V), W, take)
 
 
+@pytest.mark.parametrize("Q,W,V,take", [(2, 11, 515, 22), (3, 15, 537, 30), (1, 10, 1015, 20), (2, 14, 418, 28), (1, 64, 130, 64), (2, 6, 349, 12), (1, 17, 900, 64),
+                                        (4, 9, 1653, 18), (1, 8, 99521, 16), (9, 17, 16384, 17)])
+@pytest.mark.parametrize("spread", [0.01, 4.0])
+def test_many_beams(Q, W, V, take, spread):
+    """few segments for the continuations that are wanted; beams whose every continuation is better than another's best"""
+    check(*data(Q, W, V, Q + W + V, spread), W, take)
+
+
 def test_scratch_of_many_rows_serves_fewer():
     V, most = 65537, 64
     scratch = torch.empty(ops.beam_select_scratch_bytes(most, V, 8), dtype=torch.uint8, device=DEV)

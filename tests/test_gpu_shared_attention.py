@@ -310,6 +310,21 @@ def test_a_captured_call_reads_lengths_and_groups_when_it_runs():
         b.lens = keep
 
 
+@pytest.mark.parametrize("nq,nkv,hd,rows,keys", [(8, 4, 256, 3, None), (8, 4, 96, 3, None), (8, 4, 256, 20, 1 << 20)])
+def test_pages_far_into_a_long_cache(nq, nkv, hd, rows, keys):
+    """elements of the pools behind the 2^31st, by every kernel"""
+    b = Batch([(0, 256, [300 + r for r in range(rows)])], nq, nkv, hd, BF, seed=24)
+    off = (1 << 31) // (nkv * PAGE * hd) + 3
+    far = []
+    for pool in (b.k, b.v):
+        t = torch.empty((off + pool.shape[0], nkv, PAGE, hd), device=DEV, dtype=BF)
+        t[off:] = pool
+        far.append(t)
+    b.k, b.v = far
+    b.table = np.where(b.table > 0, b.table + off, 0).astype(np.int32)
+    b.check(b.run(0.06, None, keys=keys), 0.06)
+
+
 def test_the_same_as_attention_that_shares_nothing():
     b = Batch([(0, 960, [961, 1000, 1111, 1400])], 8, 4, 256, BF, seed=23)
     got = b.run(0.0625, 50.0)
