@@ -2560,13 +2560,16 @@ def copy_slots(tensors: Sequence[torch.Tensor], src: Sequence[int], dst: Sequenc
         _check_moves(src, dst, 0, 1 << 31, "copy_slots")
         return
     rows, where, flat = 1 << 31, set(), []
-    for t in tensors:                        # (two rows at least: source and destination)
-        if not t.is_cuda or not t.dim() or not t.is_contiguous():
-            _check_moves(src, dst, 0, min([t.shape[0] if t.dim() else 0 for t in tensors]), "copy_slots")
+    for t in tensors:
+        shape, device = t.shape, t.get_device()
+        if device < 0 or not shape or not t.is_contiguous():
+            _check_moves(src, dst, 0, min([x.shape[0] if x.dim() else 0 for x in tensors]), "copy_slots")
             _req(t, "a tensor of copy_slots")
-        rows = min(rows, t.shape[0])
-        where.add(t.get_device())
-        flat += (t.data_ptr(), t.stride(0) * t.element_size() if t.numel() else 0)
+        n = shape[0]
+        if n < rows:
+            rows = n
+        where.add(device)
+        flat += (t.data_ptr(), t.nbytes // n if n else 0)
     _check_moves(src, dst, 0, rows, "copy_slots")
     if where != {_here()}:
         _on_current_device(*tensors)
