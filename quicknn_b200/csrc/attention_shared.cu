@@ -12,8 +12,13 @@
 // (an Inf, a NaN) stays with the rows that see it.  The keys of [begin, end) outside C are among each row's own.
 //
 // Work is cut into items, a CTA each: (group, tile of query rows, range of C) and (row, tile of query heads, range of its own keys),
-// per kv head; keys are walked in tiles of 16 positions.  An item leaves (m, l, O) in scratch (m in units of log2), and a second kernel joins a row's items in ascending order:
-// results depend on the numbers of ranges, not on what runs when.
+// per kv head; keys are walked in tiles of 16 positions.  An item leaves (m, l, O) in scratch (m in units of log2), and a second kernel joins
+// a row's items in ascending order: results depend on the numbers of ranges, not on what runs when.
+//
+// Bounds, on one B200: memory where keys are many (128 rows of 16 kv heads of 128 behind 6144 common keys, up to 1500 of their own each: 143 us
+// for 910 MB, the kernel of the own keys at 6.5 TB/s; 16 groups of 4 rows, window 4096, 8 kv heads of 256: 92 us, 5.9 TB/s, where 162 registers and
+// 99 KB of ring leave two CTAs an SM), else the chain of dependent reads in front of the first key (slot, length, page, query) and the two launches:
+// 4 rows of 4 kv heads of 256 behind 448 keys 5.4 us, 8 rows behind 7936 keys 13.8 (5.8 of bytes).
 #include "attention_generic.cuh"
 #include "attention_shared.cuh"
 #include "tcgen05.cuh"
@@ -76,8 +81,10 @@ struct Layout {
 };
 
 template <int HD, int NT, bool BIAS>
-__device__ __forceinline__ void walk(const Item& it, int queries, const CUtensorMap& map, KV kv, const bf16* __restrict__ q, size_t q_stride, const Cells& cells, const Shared& sh, int kh, int nq, int nkv, const Scores& sc, float* __restrict__ part_o,
-                                     float2* __restrict__ part_ml, int* __restrict__ status, unsigned char* smem, const int* pages, int first_page, unsigned bars) {
+__device__ __forceinline__ void walk(const Item& it, int queries, const CUtensorMap& map, KV kv, const bf16* __restrict__ q, size_t q_stride,
+                                     const Cells& cells, const Shared& sh, int kh, int nq, int nkv, const Scores& sc, float* __restrict__ part_o,
+                                     float2* __restrict__ part_ml, int* __restrict__ status, unsigned char* smem, const int* pages, int first_page,
+                                     unsigned bars) {
     using L = Layout<HD>;
     constexpr int KSTEPS = HD / 16, QT = 8 * NT;
     const int G = nq / nkv;
@@ -350,9 +357,11 @@ attn_shared_mma_kernel(const __grid_constant__ CUtensorMap map, const KV kv, con
 }
 
 // ---- any head size, float32 or bfloat16 ----------------------------------------------------------------------------------------
-// Tiles of 32 keys as float32 in shared memory (rows an odd number of 16-byte pieces apart).  A warp keeps GEN_Q queries: a lane forms their scores with one
-// key, the weights go to shared memory, and then the lanes take the head's elements, so that what is read of K and V serves all
-// the warp's queries.  Exact exponentials and tanh in float32.
+// Tiles of 32 keys as float32 in shared memory (rows an odd number of 16-byte pieces apart).  A warp keeps GEN_Q queries: a lane forms their
+// scores with one key, the weights go to shared memory, and then the lanes take the head's elements, so that what is read of K and V serves
+// all the warp's queries.  Exact exponentials and tanh in float32.  Bound by instructions (half of them products, four for each row of 16 bytes read)
+// and the wait for a tile, which no other is fetched behind: six groups of 16 rows, 16 heads of 64 on 2 kv heads, 2112 keys 71 us (11 of
+// float32 arithmetic); three groups of 5 rows, 6 heads of 24 on one, 960 keys 8.5.
 constexpr int GEN_WARPS = 4, GEN_Q = 4, GEN_QT = GEN_WARPS * GEN_Q;
 
 __device__ __forceinline__ float redux_max(float x) {         // the largest of the warp's that is a number
@@ -495,8 +504,8 @@ attn_shared_generic_kernel(const T* __restrict__ q, size_t q_stride, const T* __
 }
 
 // ---- the parts of a row joined ---------------------------------------------------------------------------------------------------
-// JOIN_WARPS warps per (row, head): warp i adds parts i, i + JOIN_WARPS, ...; then the warps' sums in ascending order.  Weights are in the lanes' registers (part p: lane p % 32), the first parts are asked for before the weights are known.  Of parts
-// without keys (l = 0) nothing counts.
+// JOIN_WARPS warps per (row, head): warp i adds parts i, i + JOIN_WARPS, ...; then the warps' sums in ascending order.  Weights are in the
+// lanes' registers (part p: lane p % 32), the first parts are asked for before the weights are known.  Of parts without keys (l = 0) nothing counts.
 constexpr int JOIN_WARPS = 8, MOST_PARTS = 128;
 
 template <typename T, int PIECES>                             // pieces of 128 elements that a head has, at most
@@ -581,8 +590,7 @@ attn_shared_join_kernel(const float* __restrict__ part_o, const float2* __restri
 }
 
 // The same where a row has few parts: a thread per four elements of an output, which asks for all of them at once (a part that nobody has written is
-// read all the same and does not count).  59,520 outputs of 64 from two parts: 46 us with a
-// warp each, 13 so.
+// read all the same and does not count).  59,520 outputs of 64 from two parts: 46 us with a warp each, 13 so.
 constexpr int FEW_PARTS = 8;
 
 template <typename T, int PARTS>                              // at most
@@ -735,8 +743,9 @@ QNN_API int qnn_attn_shared_tile(int dtype, int hd, int queries, int walks, int 
 // longest (a matter of speed).  common_ranges / own_ranges: into how many ranges
 // a group's common keys and a row's own keys are cut.  Scratch: part_o B * nq * (common_ranges + own_ranges) * hd floats, part_ml twice as many
 // without hd; 16-byte aligned.  pool_pages: pages of
-// the pools; status: as in qnn_gemm_tcgen05 (bit 512: keys or values did not arrive).  page_size: a power of two of at least 16; ring: a multiple of it, or 0.  slots, slot_len, page_table, groups and
-// row_group are read before the kernel waits for the one launched in front of it on the stream: that one must not write them.
+// the pools; status: as in qnn_gemm_tcgen05 (bit 512: keys or values did not arrive).  page_size: a power of two of at least 16; ring: a
+// multiple of it, or 0.  slots, slot_len, page_table, groups and row_group are read before the kernel waits for the one launched in front of
+// it on the stream: that one must not write them.
 QNN_API int qnn_attn_decode_shared(const void* q, long long q_stride, int dtype, const void* k_pool, const void* v_pool, const int* page_table,
                                    int max_pages, int page_size, int ring, const int* slots, const int* slot_len, int B, const int* groups,
                                    int n_groups, int most_rows, int most_keys, const int* row_group, int nq, int nkv, int hd, float scale, float cap, int window,

@@ -3,7 +3,8 @@
 // nothing is uploaded before a launch and nothing has to outlive it.  Destinations are never sources (the caller sees to it), so the
 // order of the copies does not matter.
 //
-// Bound by memory: every byte is read once and written once.
+// Bound by memory: every byte is read once and written once.  32 of 64 slots, 153 MB read and written: 44.7 us, 6.8 TB/s with what
+// stays in L2 (5.7 TB/s of it at the memory); 63 pages of 13 lines 36.7 us, 5.8 TB/s.  Few bytes: one launch, 1.3 us, behind 9 us of host time.
 #include "common.cuh"
 
 using namespace qnn;
