@@ -360,8 +360,9 @@ attn_shared_mma_kernel(const __grid_constant__ CUtensorMap map, const KV kv, con
 // Tiles of 32 keys as float32 in shared memory (rows an odd number of 16-byte pieces apart).  A warp keeps GEN_Q queries: a lane forms their
 // scores with one key, the weights go to shared memory, and then the lanes take the head's elements, so that what is read of K and V serves
 // all the warp's queries.  Exact exponentials and tanh in float32.  Bound by instructions (half of them products, four for each row of 16 bytes read)
-// and the wait for a tile, which no other is fetched behind: six groups of 16 rows, 16 heads of 64 on 2 kv heads, 2112 keys 71 us (11 of
-// float32 arithmetic); three groups of 5 rows, 6 heads of 24 on one, 960 keys 8.5.
+// and the wait for a tile, which no other is fetched behind: six groups of 16 rows, 16 heads of 64 on 2 kv heads, 2112 keys 64 us (11 of
+// float32 arithmetic); three groups of 5 rows, 6 heads of 24 on one, 960 keys 8.1.  (Four pieces of keys and values asked for at once: 90 us, for
+// what it adds in instructions.)
 constexpr int GEN_WARPS = 4, GEN_Q = 4, GEN_QT = GEN_WARPS * GEN_Q;
 
 __device__ __forceinline__ float redux_max(float x) {         // the largest of the warp's that is a number
@@ -373,7 +374,7 @@ __device__ __forceinline__ float redux_max(float x) {         // the largest of 
 template <typename T, int DPL>                                // elements of a head per lane, at most
 __global__ void __launch_bounds__(GEN_WARPS * 32, DPL <= 2 ? 6 : 1)
 attn_shared_generic_kernel(const T* __restrict__ q, size_t q_stride, const T* __restrict__ k_pool, const T* __restrict__ v_pool,
-                           const Cells cells, const Shared sh, int nq, int nkv, int hd, int tile_keys, float scale, float cap,
+                           const Cells cells, const Shared sh, int nq, int nkv, int hd, int tile_keys, bool staged, float scale, float cap,
                            float* __restrict__ part_o, float2* __restrict__ part_ml, const float* __restrict__ slopes) {
     constexpr int VEC = Vec16<T>::N;
     extern __shared__ __align__(16) float sm[];
@@ -389,13 +390,16 @@ attn_shared_generic_kernel(const T* __restrict__ q, size_t q_stride, const T* __
         it = own_item(sh, cells, rest / own_tiles, rest % own_tiles, x % sh.own_ranges, GEN_QT);
     }
     const int queries = min(GEN_QT, it.rows * G - it.query0);
-    pdl_wait();
-    if (queries <= 0) return;
     const int pitch = (hd / 4 | 1) * 4;
     float* sk = sm;
     float* sv = sk + tile_keys * pitch;
     float* sq = sv + tile_keys * pitch;                       // [GEN_QT][hd], times the scale; zeros for queries that are not there
     float4* sw = reinterpret_cast<float4*>(sq + GEN_QT * hd) + warp * 32;      // the warp's weights: key, then query
+    int* pages = reinterpret_cast<int*>(reinterpret_cast<float4*>(sq + GEN_QT * hd) + GEN_WARPS * 32);      // the item's page ids, where there is room
+    int first_page = 0;
+    if (staged && queries > 0 && it.t0 < it.t1) first_page = load_pages(it, cells, pages);
+    pdl_wait();
+    if (queries <= 0) return;
     static_assert(GEN_Q == 4, "a float4 of weights");
     for (int i = threadIdx.x; i < GEN_QT * hd; i += blockDim.x) {
         const int m = it.query0 + i / hd, d = i % hd;
@@ -418,30 +422,39 @@ attn_shared_generic_kernel(const T* __restrict__ q, size_t q_stride, const T* __
 #pragma unroll
         for (int d = 0; d < DPL; ++d) o[i][d] = 0.f;
     }
-    const int chunks = hd / VEC, page_mask = (1 << cells.page_shift) - 1;
+    const int chunks = hd / VEC, j0 = threadIdx.x / chunks, c0 = threadIdx.x % chunks, step_j = blockDim.x / chunks, step_c = blockDim.x % chunks;
+    const int page_mask = (1 << cells.page_shift) - 1;
     for (int t = it.t0; t < it.t1; t += tile_keys / TILE) {
         const int n = min(tile_keys, (it.t1 - t) * TILE);
         __syncthreads();                                      // the tiles before have been read
         const int* table = cells.page_table + (size_t)it.slot * cells.max_pages;
-        for (int i = threadIdx.x; i < n * chunks; i += blockDim.x) {
-            const int j = i / chunks, c = i % chunks, p = it.position(t + j / TILE) + j % TILE;
-            if (p < it.lo || p >= it.hi) {                    // zero weights, and zeros for them to meet
+        for (int j = j0, c = c0; j < n;) {
+            const int p = it.position(t + j / TILE) + j % TILE;
+            float* const kd = sk + j * pitch + c * VEC;
+            float* const vd = sv + j * pitch + c * VEC;
+            if (p >= it.lo && p < it.hi) {
+                const int pn = p >> cells.page_shift, page = staged ? pages[pn - first_page] : table[cells.ring_pages > 0 ? pn % cells.ring_pages : pn];
+                const size_t off = ((((size_t)page * nkv + kh) << cells.page_shift) + (p & page_mask)) * hd + c * VEC;
+                Vec16<T> kv, vv;
+                kv.load(k_pool + off);
+                vv.load(v_pool + off);
+                float a[VEC], b[VEC];
+                kv.unpack(a);
+                vv.unpack(b);
 #pragma unroll
-                for (int e = 0; e < VEC; e += 4) *reinterpret_cast<float4*>(sv + j * pitch + c * VEC + e) = make_float4(0.f, 0.f, 0.f, 0.f);
-                continue;
+                for (int e = 0; e < VEC; e += 4) {
+                    *reinterpret_cast<float4*>(kd + e) = make_float4(a[e], a[e + 1], a[e + 2], a[e + 3]);
+                    *reinterpret_cast<float4*>(vd + e) = make_float4(b[e], b[e + 1], b[e + 2], b[e + 3]);
+                }
+            } else {                                          // zero weights, and zeros for them to meet
+#pragma unroll
+                for (int e = 0; e < VEC; e += 4) *reinterpret_cast<float4*>(vd + e) = make_float4(0.f, 0.f, 0.f, 0.f);
             }
-            const int pn = p >> cells.page_shift, page = table[cells.ring_pages > 0 ? pn % cells.ring_pages : pn];
-            const size_t off = ((((size_t)page * nkv + kh) << cells.page_shift) + (p & page_mask)) * hd + c * VEC;
-            Vec16<T> kv, vv;
-            kv.load(k_pool + off);
-            vv.load(v_pool + off);
-            float a[VEC], b[VEC];
-            kv.unpack(a);
-            vv.unpack(b);
-#pragma unroll
-            for (int e = 0; e < VEC; e += 4) {
-                *reinterpret_cast<float4*>(sk + j * pitch + c * VEC + e) = make_float4(a[e], a[e + 1], a[e + 2], a[e + 3]);
-                *reinterpret_cast<float4*>(sv + j * pitch + c * VEC + e) = make_float4(b[e], b[e + 1], b[e + 2], b[e + 3]);
+            c += step_c;
+            j += step_j;
+            if (c >= chunks) {
+                c -= chunks;
+                ++j;
             }
         }
         __syncthreads();
@@ -466,12 +479,15 @@ attn_shared_generic_kernel(const T* __restrict__ q, size_t q_stride, const T* __
         for (int i = 0; i < GEN_Q; ++i) {
             s[i] = softcap_t<T>(s[i], cap) - slope[i] * (float)(newest[i] - pos);
             const float top = fmaxf(mx[i], redux_max(valid ? s[i] : -CUDART_INF_F));
-            const float keep = mx[i] == -CUDART_INF_F ? 0.f : fexp<T>(mx[i] - top);
-            w[i] = valid && (top != -CUDART_INF_F || s[i] != s[i]) ? fexp<T>(s[i] - top) : 0.f;
-            l[i] = l[i] * keep + w[i];                        // the lane's keys
-            mx[i] = top;
+            if (top > mx[i]) {                                // (the same in all lanes)
+                const float keep = mx[i] == -CUDART_INF_F ? 0.f : fexp<T>(mx[i] - top);
+                mx[i] = top;
+                l[i] *= keep;
 #pragma unroll
-            for (int d = 0; d < DPL; ++d) o[i][d] *= keep;
+                for (int d = 0; d < DPL; ++d) o[i][d] *= keep;
+            }
+            w[i] = valid && (top != -CUDART_INF_F || s[i] != s[i]) ? fexp<T>(s[i] - top) : 0.f;
+            l[i] += w[i];                                     // the lane's keys
         }
         sw[lane] = make_float4(w[0], w[1], w[2], w[3]);
         __syncwarp();
@@ -692,12 +708,15 @@ template <typename T, int DPL>
 int launch_generic(const void* q, long long q_stride, const void* k_pool, const void* v_pool, const Cells& cells, const Shared& sh, int items, int nq,
                    int nkv, int hd, float scale, float cap, float* part_o, float2* part_ml, const float* slopes, cudaStream_t st) {
     const int keys = hd <= 512 ? 32 : 16;
-    const size_t smem = ((size_t)2 * keys * ((hd / 4) | 1) * 4 + (size_t)GEN_QT * hd + GEN_WARPS * 32 * 4) * sizeof(float);
+    size_t smem = ((size_t)2 * keys * ((hd / 4) | 1) * 4 + (size_t)GEN_QT * hd + GEN_WARPS * 32 * 4) * sizeof(float);
+    const size_t pages = ((size_t)cells.max_pages + 2) * sizeof(int);
+    const bool staged = hd <= 256 && smem + pages <= 220 * 1024;
+    if (staged) smem += pages;
     auto kern = attn_shared_generic_kernel<T, DPL>;
     static OncePerDevice asked;
     if (const int rc = allow_shared(asked, kern, 220 * 1024)) return rc;
     launch_pdl(kern, dim3(items, nkv), dim3(GEN_WARPS * 32), smem, st, (const T*)q, (size_t)q_stride, (const T*)k_pool, (const T*)v_pool, cells, sh, nq,
-               nkv, hd, keys, scale, cap, part_o, part_ml, slopes);
+               nkv, hd, keys, staged, scale, cap, part_o, part_ml, slopes);
     return (int)cudaGetLastError();
 }
 

@@ -2342,7 +2342,7 @@ class SharedPlan(NamedTuple):
     kernels: int = 2             # launches of a call
 
 
-SHARED_ITEM_COST = 64.0          # what a CTA of that attention costs beside its keys, in keys; of the kernel for any head size a quarter
+SHARED_ITEM_COST = 64.0          # what a CTA of that attention costs beside its keys, in keys; of the kernel for any head size a half
 
 
 def shared_attention_plan(dtype: torch.dtype, n_rows: int, n_heads: int, n_kv: int, head_dim: int, shared: SharedKeys,
@@ -2380,7 +2380,7 @@ def shared_attention_plan(dtype: torch.dtype, n_rows: int, n_heads: int, n_kv: i
             s = next((n for n in range(1, 9) if walk(n) <= 0.6 * time), 0) or min(range(1, 65), key=lambda n: walk(n) + parts * n)
             ranges = (min(s, -(-keys // 64)), p)
         else:
-            best, cost = None, SHARED_ITEM_COST / (1 if tensor_cores else 4)
+            best, cost = None, SHARED_ITEM_COST / (1 if tensor_cores else 2)
             for c in _SHARED_CHUNKS:
                 s, p = -(-keys // c), -(-own // c)
                 if s > 64 or p > 64:
