@@ -16,9 +16,9 @@
 // a row's items in ascending order: results depend on the numbers of ranges, not on what runs when.
 //
 // Bounds, on one B200: memory where keys are many (128 rows of 16 kv heads of 128 behind 6144 common keys, up to 1500 of their own each: 143 us
-// for 910 MB, the kernel of the own keys at 6.5 TB/s; 16 groups of 4 rows, window 4096, 8 kv heads of 256: 92 us, 5.9 TB/s, where 162 registers and
-// 99 KB of ring leave two CTAs an SM), else the chain of dependent reads in front of the first key (slot, length, page, query) and the two launches:
-// 4 rows of 4 kv heads of 256 behind 448 keys 5.4 us, 8 rows behind 7936 keys 13.8 (5.8 of bytes).
+// for 910 MB, the kernel of the own keys at 6.5 TB/s; 16 groups of 4 rows, window 4096, 8 kv heads of 256: 91 us,
+// 6.0 TB/s), else the chain of dependent reads in front of the first key (slot, length, page, query) and the two launches:
+// 4 rows of 4 kv heads of 256 behind 448 keys 5.5 us, 8 rows behind 7936 keys 13.4 (5.8 of bytes).
 #include "attention_generic.cuh"
 #include "attention_shared.cuh"
 #include "tcgen05.cuh"
@@ -44,12 +44,13 @@ __device__ __forceinline__ int load_pages(const Item& it, const Cells& c, int* p
 //     S^T[16 keys x 8 q] = K Q^T,    O^T[hd x 8 q] += V^T P^T,
 // here with NT column tiles (8 NT queries) for every fragment of K and V that ldmatrix brings.  A warp walks its own tiles of 16 keys: one
 // lane asks the copy engine for them (a tile lies within a page; boxes of 64 elements x 16 positions, 128-byte swizzle, so that ldmatrix does
-// not conflict), STAGES deep, an mbarrier each.  (Rows copied one by one to padded rows, without a tensor map: 16 x 4 rows under a window of
-// 4096 126 us instead of 93; cp.async by every lane 114.)  Nothing but the last merge is shared between the warps of a CTA.  P^T is the transpose
-// of S^T's accumulator, eight by eight (movmatrix).  The exponentials are taken against a reference that is raised only when a score
+// not conflict), STAGES deep, an mbarrier each: two, so that 8, 6 and 3 CTAs of head size 64, 128 and 256 fit an SM (three stages, 8, 4 and 2:
+// 11 groups of 82 rows with up to 26 keys of their own, 4 kv heads of 128 45 us instead of 38; 14 of 74 with up to 81, 8 kv heads 95 instead of
+// 81; long walks the same).  (Rows copied one by one to padded rows, without a tensor map: 16 x 4 rows under a window of 4096 126 us instead of
+// 93; cp.async by every lane 114.)  Nothing but the last merge is shared between the warps of a CTA.  P^T is the transpose of S^T's accumulator, eight by eight (movmatrix).  The exponentials are taken against a reference that is raised only when a score
 // exceeds it by more than 8 (in log2): the stale reference cancels in the division, P stays below 2^8.
 constexpr float REFERENCE_STEP = 8.f;
-constexpr int WARPS = 2, STAGES = 3;
+constexpr int WARPS = 2, STAGES = 2;
 
 __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], unsigned addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"

@@ -2364,7 +2364,8 @@ def shared_attention_plan(dtype: torch.dtype, n_rows: int, n_heads: int, n_kv: i
                 own = window - keys + 128
         sms = _sm_count("cuda")
         tensor_cores = dtype == torch.bfloat16 and head_dim in (64, 128, 256)
-        resident = sms * (min(8, 512 // head_dim) if tensor_cores else 6 if head_dim <= 64 else 2 if head_dim <= 256 else 1)      # CTAs at a time
+        # CTAs at a time that pay (of the tensor cores' kernel 8, 6 and 3 fit an SM; more ranges for the last of them cost more than they bring)
+        resident = sms * (min(8, 512 // head_dim) if tensor_cores else 6 if head_dim <= 64 else 2 if head_dim <= 256 else 1)
         common = shared.n_groups * (-(-shared.rows * heads // tile)) * n_kv                # walks over common keys
         alone = n_rows * (-(-heads // tile)) * n_kv                                        # walks over own keys
         # the times below are in keys of a walk; the parts are written and read as float32
@@ -2373,6 +2374,7 @@ def shared_attention_plan(dtype: torch.dtype, n_rows: int, n_heads: int, n_kv: i
             # Two kernels side by side: common keys by CTAs that take most of an SM (a quarter of a walk's time per key, from 200 on), own keys
             # by small ones on what is left, bound by memory.  As few of the former as are done in time; where own keys are few, as many
             # as make them short.
+            resident = sms * {64: 8, 128: 6, 256: 3}[head_dim]
             p = min(range(1, 65), key=lambda n: _spread(alone * n, resident, own / n) + parts * n)
             seen = min(own, window - keys + 128) if window else own                         # (as far as the common keys leave a window any)
             time = _spread(alone * p, resident, seen / p)
