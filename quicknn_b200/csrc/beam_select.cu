@@ -278,7 +278,7 @@ beam_pick_kernel(const float* __restrict__ logits, int V, int beams, int take, i
             const auto note = [&](int i, float z) {
                 const bool holds = add != -CUDART_INF && z != -CUDART_INF_F;
                 best[b * segments + i] = holds ? rounded(add + (double)z) : -CUDART_INF_F;
-                if (ALONE) here[b * segments + i].x = holds ? (float)add : -CUDART_INF_F;       // (nobody else reads these numbers)
+                if (ALONE) reinterpret_cast<double*>(here)[b * segments + i] = holds ? add : -CUDART_INF;       // (nobody else reads these numbers)
             };
 #pragma unroll
             for (int k = 0; k < KEPT; ++k)
@@ -293,8 +293,13 @@ beam_pick_kernel(const float* __restrict__ logits, int V, int beams, int take, i
         const double top = (double)threshold, exactly = top - add;
         return threshold > -FLT_MAX ? rounded(exactly - 1e-5 * (fabs(exactly) + fabs(top))) : -FLT_MAX;
     };
-    if (ALONE) nth_of_groups(n * SEGMENT, take, [&](int i) { return fminf(here[i / SEGMENT].x + reinterpret_cast<const float*>(logits_here)[i], FLT_MAX); },
-                             group_best, threshold_s);
+    // The threshold is compared with the segments' best scores and with scores of other beams, so single logits, too, become scores in 64 bits that are
+    // rounded once.  (t_b - log(sum exp) rounded before the sum would move all of a beam's scores together, by more than their distances to
+    // another's where logits are large.)
+    if (ALONE) nth_of_groups(n * SEGMENT, take, [&](int i) {
+                                 const double s = reinterpret_cast<const double*>(here)[i / SEGMENT] + (double)reinterpret_cast<const float*>(logits_here)[i];
+                                 return s > -CUDART_INF ? rounded(s) : -CUDART_INF_F;
+                             }, group_best, threshold_s);
     else nth_of_groups(n, take, [&](int i) { return best[i]; }, group_best, threshold_s);
     const float threshold = threshold_s;
     if (ALONE) {
@@ -308,9 +313,11 @@ beam_pick_kernel(const float* __restrict__ logits, int V, int beams, int take, i
             for (int j = 0; j < SEGMENT / 32; ++j) {
                 const float z = reinterpret_cast<const float*>(logits_here)[l * SEGMENT + j * 32 + lane];
                 if (!(z >= limit)) continue;                  // (limit is finite, what is no continuation -inf)
+                const double s = add + (double)z;
+                if (rounded(s) < threshold) continue;
                 const int at = atomicAdd(&n_found, 1);
                 if (at < LIST) {
-                    found->score[at] = add + (double)z;
+                    found->score[at] = s;
                     found->at[at] = (unsigned)b * (unsigned)V + (unsigned)(v0 + j * 32 + lane);
                 }
             }
@@ -393,7 +400,7 @@ beam_pick_kernel(const float* __restrict__ logits, int V, int beams, int take, i
         return;
     }
     // More scores at the threshold than the list holds (thousands of equal ones): `take` rounds over the segments that reach it, each for
-    // the best behind the one before.
+    // the best behind the one before.  (Thousands reach it, so no round ends with nothing.)
     for (int k = 0; k < take; ++k) {
         double s_best = -CUDART_INF;
         unsigned a_best = 0xffffffffu;

@@ -170,3 +170,46 @@ def test_refusals():
     out = (torch.empty(2, 4, device=DEV), torch.empty(2, 4, dtype=torch.int32, device=DEV), torch.empty(2, 5, dtype=torch.int32, device=DEV))
     with pytest.raises(ValueError):
         ops.beam_select(logits, scores, 3, 4, scratch, out=out)
+
+
+@pytest.mark.parametrize("level", [0.1, 10.0, 12.0, 30.0, -4.7])
+@pytest.mark.parametrize("W,V,take", [(1, 3000, 8), (1, 4000, 64), (4, 900, 32), (3, 700, 24), (1, 40000, 8)])
+def test_one_value_everywhere(level, W, V, take):
+    """the threshold and the segments' best scores are the same number, however it is rounded"""
+    logits = torch.full((2 * W, V), level, device=DEV)
+    check(logits, torch.tensor([-0.3 * b for b in range(W)] * 2, device=DEV), W, take)
+
+
+@pytest.mark.parametrize("level", [0.1, 10.0, 30.0, 4096.0])
+def test_thousands_of_logits_a_few_steps_apart(level):
+    """all within what the limit of the short list allows for roundings, so they do not fit it"""
+    V = 3000
+    g = torch.Generator().manual_seed(int(level))
+    base = torch.tensor(level).view(torch.int32) + torch.randint(0, 5, (2, V), generator=g, dtype=torch.int32)
+    check(base.view(torch.float32).to(DEV), torch.zeros(2, device=DEV), 1, 16)
+
+
+@pytest.mark.parametrize("far,spread", [(4096.0, 0.03), (20000.0, 0.03), (1e6, 0.3)])
+@pytest.mark.parametrize("scores", [(0.0, 0.0), (-5.0, -5.003)])
+def test_beams_whose_logits_lie_apart(far, spread, scores):
+    """Beam 0's logits stand far above beam 1's; their continuations score alike.  Where two beams' scores are closer than what the sums of
+    exponentials may be off by (2^-20 each), their order is open, and the draw says nothing."""
+    said = 0
+    for seed in range(60):
+        x = spread * torch.randn(2, 400, generator=torch.Generator().manual_seed(seed))
+        x[0] += far
+        t = torch.tensor(scores)
+        s, b, _ = (a[0] for a in wanted(x, t, 2, 9))
+        if any(b[i] != b[i + 1] and s[i] - s[i + 1] < 2.0 ** -18 for i in range(8)):
+            continue
+        said += 1
+        check(x.to(DEV), t.to(DEV), 2, 8)
+    assert said > 40
+
+
+@pytest.mark.parametrize("W,V,take", [(1, 3000, 8), (3, 300, 12), (2, 20000, 16)])
+def test_fewer_continuations_than_wanted(W, V, take):
+    logits, scores = data(2, W, V, 7)
+    logits[:, 3:] = float("-inf")
+    logits[W:, 1:] = float("-inf")
+    check(logits, scores, W, take)
