@@ -720,15 +720,16 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         const bool good = alive && !__any_sync(0xffffffffu, has_failed(bars));
         if (good) {
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            // weights of the two halves against the larger reference maximum (a half without keys has sum 0)
-            const bool have0 = l_sum > 0.f, have1 = l_other > 0.f;
+            // weights of the two halves against the larger reference maximum (a half without keys has sum 0; one with a NaN among
+            // its scores has a NaN, which has to come out)
+            const bool have0 = l_sum != 0.f, have1 = l_other != 0.f;
             const float mm = fmaxf(have0 ? m_used : -CUDART_INF_F, have1 ? m_other : -CUDART_INF_F);
             const float w0 = have0 ? exp2_fast((m_used - mm) * k2) : 0.f;
             const float w1 = have1 ? exp2_fast((m_other - mm) * k2) : 0.f;
             // a head's sink joins the denominator once, against the same reference (k2 holds log2(e))
             const float l_row = l_sum * w0 + l_other * w1;
             const float l_all = sinks != nullptr ? l_row + exp2_fast(sinks[h] * LOG2E - mm * k2) : l_row;
-            const float inv = l_row > 0.f ? 1.f / l_all : 0.f;
+            const float inv = l_row != 0.f ? 1.f / l_all : 0.f;
             const float f0 = w0 * inv, f1 = w1 * inv;
             unsigned char* orow = sOut + rloc * (HD * 2);
             const unsigned char* prow = sK + rloc * (HD * 4);
