@@ -41,6 +41,7 @@
 // Tensor memory: S 128 columns, O one column per head element, Q hd / 2 columns.  All softmax arithmetic is float32.
 // Keys of other sequences that a tile drags in are masked; rows beyond the sequence are never stored.
 // Every mbarrier wait is bounded in time; on expiry a status word is set and the CTA winds down.
+#include "capped_exp2.cuh"
 #include "common.cuh"
 #include "tcgen05.cuh"
 #include <math_constants.h>
@@ -76,71 +77,6 @@ __device__ __forceinline__ void umma_bf16_a_tmem(unsigned tmem_d, unsigned tmem_
 }
 constexpr float RESCALE_STEP = 8.f;
 constexpr int MERGE_ML_BYTES = BM * 8;               // (reference maximum, sum) per row that rank 1 of a pair hands to rank 0
-
-__device__ __forceinline__ float tanh_fast(float x) {
-    float r;
-    asm("tanh.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-__device__ __forceinline__ float exp2_fast(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-// 2^x on the FMA and integer pipes, for |x| < 126: x = n + f with n the nearest integer (the sum with 1.5 * 2^23
-// leaves n in the low mantissa bits), 2^f by a cubic on [-0.5, 0.5] (relative error 7.5e-5, a thirtieth of
-// bfloat16's rounding), n added to the exponent field.  The special-function unit does 16 operations a clock per
-// SM and a capped score needs two (tanh, 2^x): taking some of the exponentials here relieves it.  Measured with
-// 0, 2, 4, 6, 8 of every 8 columns done this way, 8 heads of 256, one prompt: 2048 tokens 36.8 / 36.1 / 35.1 / 35.2 /
-// 38.4 us, 8192 tokens 243 / 241 / 238 / 239 / 253 us; 32 heads of 128 at 8192: 831 / 815 / 796 / 800 / 869 us.
-constexpr int POLY = 4;            // of every 8 columns of a row
-
-// Two floats in a register pair: one instruction does both, each rounded like the single operation.
-__device__ __forceinline__ uint64_t two(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void one_by_one(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-// (a, b) <- exp(cap tanh(score / cap)) of two scores; `poly`: 2^x by the polynomial described at POLY
-__device__ __forceinline__ uint64_t capped_exp2(float& a, float& b, uint64_t k1, uint64_t k2, bool poly) {
-    float x, y;
-    one_by_one(mul2(two(a, b), k1), x, y);
-    const uint64_t t = two(tanh_fast(x), tanh_fast(y));
-    if (poly) {
-        const uint64_t magic = two(12582912.f, 12582912.f), minus = two(-1.f, -1.f);
-        const uint64_t xf = fma2(t, k2, magic);
-        const uint64_t f = fma2(t, k2, fma2(xf, minus, magic));
-        uint64_t q = fma2(f, two(0.055171407759189606f, 0.055171407759189606f), two(0.24261075258255005f, 0.24261075258255005f));
-        q = fma2(q, f, two(0.6932609677314758f, 0.6932609677314758f));
-        q = fma2(q, f, two(0.9999281167984009f, 0.9999281167984009f));
-        float qa, qb, na, nb;
-        one_by_one(q, qa, qb);
-        one_by_one(xf, na, nb);
-        a = __int_as_float(__float_as_int(qa) + (__float_as_int(na) << 23));
-        b = __int_as_float(__float_as_int(qb) + (__float_as_int(nb) << 23));
-    } else {
-        one_by_one(mul2(t, k2), x, y);
-        a = exp2_fast(x);
-        b = exp2_fast(y);
-    }
-    return two(a, b);
-}
 
 struct __align__(8) Barriers {
     uint64_t q_full;
@@ -522,10 +458,7 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
                         rs23 = add2(rs23, two(s[c + 2], s[c + 3]));
                     }
                 }
-                float r0s, r1s, r2s, r3s;
-                one_by_one(rs01, r0s, r1s);
-                one_by_one(rs23, r2s, r3s);
-                l_sum += (r0s + r1s) + (r2s + r3s);
+                l_sum += capped_sum(rs01, rs23);
             } else {
             float mx4[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
             // the distance bias of the tile's first column; a column adds slope_u times its place in the tile, so the
@@ -534,7 +467,7 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
 #pragma unroll
             for (int c = 0; c < BN; ++c) {
                 const float bias = fmaf(slope_u, (float)c, bias0);         // (float)c is a constant of the unrolled loop
-                s[c] = cap > 0.f ? tanh_fast(s[c] * k1) + bias : fmaf(s[c], k1, bias);
+                s[c] = cap > 0.f ? tanh_approx(s[c] * k1) + bias : fmaf(s[c], k1, bias);
             }
             if (!interior) {
 #pragma unroll

@@ -1,6 +1,7 @@
 // What the attention of rows that share pages is made of: which keys a group of rows has in common, the items that the work is cut into,
 // and where their results go.  See attention_shared.cu.
 #pragma once
+#include "capped_exp2.cuh"
 #include "common.cuh"
 #include "tcgen05.cuh"
 #include <math_constants.h>
@@ -11,11 +12,7 @@ namespace shared {
 constexpr int TILE = 16;                      // positions
 constexpr float LOG2E = 1.4426950408889634f;
 
-__device__ __forceinline__ float exp2_fast(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
+using tc::exp2_fast;
 
 struct Shared {
     const int4* groups;                       // first row, rows, first position, position behind the last

@@ -15,6 +15,7 @@
 // 256 17 us.  The keys themselves come from memory once per 128 query rows.
 // Every mbarrier wait is bounded in time; on expiry a status word is set and the CTA winds down.
 #include "attention_shared.cuh"
+#include "capped_exp2.cuh"
 #include "tcgen05.cuh"
 #include <math_constants.h>
 
@@ -28,7 +29,6 @@ constexpr int BM = 128, BN = 64, UMMA_K = 16, MAX_STAGES = 6, THREADS = 384;
 constexpr int P_BYTES = BM * BN * 2;
 constexpr int S_COL = 0, O_COL = 128;         // tensor-memory columns of S (two halves of 64) and of O; Q follows O
 constexpr float STEP = 8.f;                   // how far (in e) a maximum may rise before O is rescaled
-constexpr int POLY = 4;                       // of every 8 exponentials, those taken on the FMA pipe (with a softcap)
 // Depth of the rings.  Up to head size 128 they leave room for a CTA of the rows' own keys on the same SM.
 __host__ __device__ constexpr int k_stages(int hd) { return hd >= 128 ? 2 : 4; }                        // pairs of pages
 __host__ __device__ constexpr int v_stages(int hd) { return hd >= 256 ? 2 : (hd >= 128 ? 3 : 6); }       // pages
@@ -40,54 +40,6 @@ __device__ __forceinline__ void umma_a_tmem(unsigned tmem_d, unsigned tmem_a, ui
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
         ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
 }
-// two floats in a register pair: one instruction for both, each rounded like the single operation
-__device__ __forceinline__ uint64_t two(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void one_by_one(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-// (a, b) <- exp(cap tanh(score / cap)); `poly`: 2^x as n + f, f in [-1/2, 1/2], 2^f by a cubic (relative error 7.5e-5, a thirtieth of
-// bfloat16's rounding), n into the exponent field; |x| < 126
-__device__ __forceinline__ uint64_t capped_exp2(float& a, float& b, uint64_t k1, uint64_t k2, bool poly) {
-    float x, y;
-    one_by_one(mul2(two(a, b), k1), x, y);
-    const uint64_t t = two(tanh_approx(x), tanh_approx(y));
-    if (poly) {
-        const uint64_t magic = two(12582912.f, 12582912.f), minus = two(-1.f, -1.f);
-        const uint64_t xf = fma2(t, k2, magic);
-        const uint64_t f = fma2(t, k2, fma2(xf, minus, magic));
-        uint64_t q = fma2(f, two(0.055171407759189606f, 0.055171407759189606f), two(0.24261075258255005f, 0.24261075258255005f));
-        q = fma2(q, f, two(0.6932609677314758f, 0.6932609677314758f));
-        q = fma2(q, f, two(0.9999281167984009f, 0.9999281167984009f));
-        float qa, qb, na, nb;
-        one_by_one(q, qa, qb);
-        one_by_one(xf, na, nb);
-        a = __int_as_float(__float_as_int(qa) + (__float_as_int(na) << 23));
-        b = __int_as_float(__float_as_int(qb) + (__float_as_int(nb) << 23));
-    } else {
-        one_by_one(mul2(t, k2), x, y);
-        a = exp2_fast(x);
-        b = exp2_fast(y);
-    }
-    return two(a, b);
-}
-
 struct __align__(8) Barriers {
     uint64_t q_tmem;          // Q is in tensor memory
     uint64_t k_full[MAX_STAGES], k_empty[MAX_STAGES];
@@ -377,7 +329,9 @@ attn_shared_tcgen05_kernel(const __grid_constant__ CUtensorMap map, const KV kv,
                     rs23 = add2(rs23, two(s[c + 2], s[c + 3]));
                 }
             }
-            {
+            if (FIXED) {
+                l_sum += capped_sum(rs01, rs23);
+            } else {
                 float a, b, c, d;
                 one_by_one(rs01, a, b);
                 one_by_one(rs23, c, d);

@@ -43,3 +43,32 @@ def test_prompt_whose_tiles_two_blocks_share(hd):
 @pytest.mark.parametrize("hd", [64, 128, 256])
 def test_prompts_of_single_blocks(hd):
     check_prompt([130, 1, 300], hd, None, (0, 5, 129, 130, 131, 300, 430))
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("cap", [50.0, 90.0])
+def test_prompts_with_a_softcap(hd, cap):
+    """with a softcap up to 70 the columns of a tile take their exponentials in two ways, four neighbours each"""
+    check_prompt([130, 1, 300], hd, cap, tuple(range(8)) + (64, 70, 129, 130, 131 + 66, 300, 430))
+    check_prompt([1500], hd, cap, (0, 65, 129, 130, 197, 390, 1300, 1499))
+
+
+@pytest.mark.parametrize("nq,nkv,hd", [(8, 4, 256), (8, 2, 128), (16, 2, 64)])
+@pytest.mark.parametrize("cap", [None, 50.0, 90.0])
+@pytest.mark.parametrize("keys", [1, 1 << 20])
+def test_rows_that_share_pages(nq, nkv, hd, cap, keys):
+    """by the kernel of few rows and that of many (which the bound of the keys chooses)"""
+    from test_gpu_shared_attention import BF, Batch
+    b = Batch([(0, 192, [193 + i for i in range(40)])], nq, nkv, hd, BF, alone=[77], seed=hd)
+    clean = b.run(hd ** -0.5, cap, (2, 1), keys=keys).view(b.B, nq, hd)
+    assert torch.isfinite(clean).all()
+    for at in tuple(range(8)) + (63, 64, 70, 127, 128, 191):
+        page, cell = int(b.table[b.slots[0], at // 64]), at % 64
+        held = b.k[page, 1, cell, 5].clone()
+        b.k[page, 1, cell, 5] = float("nan")
+        got = b.run(hd ** -0.5, cap, (2, 1), keys=keys).view(b.B, nq, hd)
+        b.k[page, 1, cell, 5] = held
+        mine = slice(nq // nkv, 2 * (nq // nkv))
+        assert torch.isnan(got[:40, mine]).all(), at
+        got[:40, mine] = clean[:40, mine]
+        assert torch.equal(got, clean), at
