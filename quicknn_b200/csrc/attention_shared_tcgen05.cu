@@ -402,7 +402,7 @@ attn_shared_tcgen05_kernel(const __grid_constant__ CUtensorMap map, const KV kv,
             const size_t at = have ? part_of(it, sh, m, kh, G, nq) : 0;
             if (group == 0 && have) {
                 float l_other = l_second[rloc];
-                if (!FIXED && nt > 1) l_other *= exp2_fast((m_second[rloc] - m_used) * k2);
+                if (!FIXED && l_other != 0.f) l_other *= exp2_fast((m_second[rloc] - m_used) * k2);      // (without a weight it has no reference)
                 part_ml[at] = make_float2(FIXED ? 0.f : m_used * k2, l_sum + l_other);
             }
             // Half of the head by each group, through the K ring (16-byte pieces XOR-ed with the row), so that whole rows are written.

@@ -72,3 +72,36 @@ def test_rows_that_share_pages(nq, nkv, hd, cap, keys):
         assert torch.isnan(got[:40, mine]).all(), at
         got[:40, mine] = clean[:40, mine]
         assert torch.equal(got, clean), at
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("pages", [3, 5])
+def test_pages_whose_scores_are_all_minus_infinity(hd, pages):
+    """Keys of the first pages score -inf for every query: they have no weight.  The last page, which has no neighbour, is the first with a
+    maximum, a low one."""
+    from test_gpu_shared_attention import BF, Batch
+    n = pages * 64
+    b = Batch([(0, n, [n + 1 + i for i in range(20)])], 8, 4, hd, BF, seed=pages)
+    q = b.qkv[:, :8 * hd].view(b.B, 8, hd)
+    q[:, :, 0] = 2.0
+    table = torch.from_numpy(b.table[b.slots[0]].astype("int64")).to(DEV)
+    for k in b.k_of:
+        k[:n - 64, :, 0] = float("-inf")
+        k[n - 64:, :, 0] = -200.0
+    pos = torch.arange(n, device=DEV)
+    b.k[table[pos // 64], :, pos % 64] = b.k_of[0][:n]
+    for r in range(b.B):                                             # the rows' own keys score low as well
+        own = torch.arange(n, b.lens[r], device=DEV)
+        t = torch.from_numpy(b.table[b.slots[r]].astype("int64")).to(DEV)
+        b.k[t[own // 64], :, own % 64] = b.k_of[r][n:]
+    got = {keys: b.run(0.5, None, (1, 1), keys=keys) for keys in (1, 1 << 20)}
+    for keys, o in got.items():
+        assert torch.isfinite(o).all(), keys
+        for r in range(b.B):
+            k, v = b.k_of[r][n - 64:].double(), b.v_of[r][n - 64:].double()
+            s = torch.einsum("khd,pkd->khp", q[r].double().view(4, 2, hd), k) * 0.5
+            want = torch.einsum("khp,pkd->khd", torch.softmax(s, -1), v).reshape(-1)
+            # as in the tests of this attention: bfloat16 weights, exponents of up to 200 in float32, the result's rounding
+            size = torch.einsum("khp,pkd->khd", torch.softmax(s, -1), v.abs()).reshape(-1)
+            tol = (2.0 ** -8 + (hd * 400 * 0.5 + 4 * 250) * 2.0 ** -23 + 2.0 ** -19) * size + 2.0 ** -8 * want.abs()
+            assert ((o[r].double() - want).abs() <= tol).all(), (keys, r)
