@@ -254,7 +254,7 @@ class AttentionMixer(Mixer):
             return ()
         plan = self.shared_plan(step)
         if plan is not None:
-            return ("shared",) + plan[:2]
+            return ("shared", plan.common_ranges, plan.own_ranges, plan.kernels)      # (the last says which kernel takes the common keys)
         splits = self.decode_splits(step)
         blocks = splits * step.n_seqs * self.n_kv * ((self.n_heads // self.n_kv + 7) // 8)
         # the kernel's layout depends on the lengths at head size 256 and beyond one round of blocks

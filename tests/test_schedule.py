@@ -131,3 +131,27 @@ def test_a_kernel_that_ran_nothing_is_not_reported_as_one_that_gave_up_waiting()
     assert "shared memory" in wait_status_message(256) and "waiting" not in wait_status_message(256)
     both = wait_status_message(256 | 32)
     assert "gave up waiting (status 32;" in both and "shared memory" in both
+
+
+def test_steps_whose_common_keys_go_to_different_kernels_do_not_share_a_graph(monkeypatch):
+    """The division into ranges may be the same though one bound of the keys is for the kernel of few rows, the other for that of many."""
+    import torch
+    from quicknn_b200.engine.batch import StepSharing
+    from quicknn_b200.kernels import ops
+    monkeypatch.setattr(ops, "_sm_count", lambda device: 148)
+    monkeypatch.setattr(ops, "shared_attention_pays", lambda *a: True)
+    schedules, kernels = {}, {}
+    for n_groups, rows in ((8, 32), (1, 128), (4, 64), (8, 16)):
+        for n_kv, hd in ((4, 128), (8, 128), (4, 256), (2, 64)):
+            m = mixer(n_kv=n_kv, head_dim=hd)
+            for own in (128, 1024):
+                for keys in (512, 1024, 2048, 4096, 8192, 16384):
+                    sharing = StepSharing(n_groups, rows, keys, own)
+                    s = step(n_groups * rows, 16384, 1.0)
+                    s.sharing, s.act_dtype = sharing, torch.bfloat16
+                    plan = m.shared_plan(s)
+                    key = (n_groups, rows, n_kv, hd, m.schedule(s))
+                    kernels.setdefault(key, set()).add(plan.kernels)
+                    schedules.setdefault((n_groups, rows, n_kv, hd, plan[:2]), set()).add(plan.kernels)
+    assert any(len(k) > 1 for k in schedules.values())               # equal divisions for different kernels do occur
+    assert all(len(k) == 1 for k in kernels.values())
