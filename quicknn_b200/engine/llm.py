@@ -122,6 +122,7 @@ class _PrefixBackend(_Backend):
         super().__init__(engine, sampler, max_batch if one_batch else max_batch - 1, run_ahead, seed)
         self.prefix, self.one_batch = prefix, one_batch
         self.base: Optional[int] = None
+        self.begun: List[int] = []                   # requests that have been started behind the prefix
         if not one_batch:
             self.max_tokens -= (len(prefix) + PAGE - 1) // PAGE * PAGE
 
@@ -135,7 +136,9 @@ class _PrefixBackend(_Backend):
             self.slots += eng.fork(self.slots * (n - 1))
         else:
             self.slots = eng.fork([self.base] * n)
-        return self._start(first_index, prompts, [p[len(self.prefix):] for p in prompts])
+        sampled = self._start(first_index, prompts, [p[len(self.prefix):] for p in prompts])
+        self.begun += range(first_index, first_index + n)
+        return sampled
 
     def close(self) -> None:
         if self.base is not None:
@@ -331,7 +334,7 @@ class LLM:
         """Generate for a list of prompts (lists of token ids).  Requests are run in batches of
         up to ``max_batch``, one batch after another.  ``prefix``: ids that stand in front of every prompt (each of which has at least
         one id of its own): they run once, every request goes on from there, and the attention of the replies' steps reads their keys
-        once for all requests.  The results count them as part of the prompts, reused ones.  With more requests than a batch holds the
+        once for all requests.  The results count them as part of the prompts, of requests that were started as reused ones.  With more requests than a batch holds the
         prefix keeps one of the ``max_batch`` sequences."""
         options = options or GenerationOptions()
         options.validate()
@@ -352,8 +355,8 @@ class LLM:
         try:
             results = generate(backend, prompts, options, stops, on_token, should_cancel)
             if prefix:
-                for r in results:
-                    r.reused_tokens = len(prefix)
+                for i in backend.begun:
+                    results[i].reused_tokens = len(prefix)
             return results
         finally:
             if prefix:
