@@ -68,6 +68,17 @@ def _req(t: torch.Tensor, name: str, dtype=None, dim=None) -> None:
         raise ValueError(f"{name} must have {dim} dimensions, got {tuple(t.shape)}")
 
 
+def _req_word(t: Optional[torch.Tensor], name: str, device: int) -> None:
+    """An int32 word on the device that a kernel reads or sets, or None."""
+    if t is None or (t.is_cuda and t.dtype is torch.int32 and t.numel() and t.get_device() == device):
+        return
+    if not t.is_cuda:
+        raise _lib.KernelError(f"{name} must be a CUDA tensor: quicknn_b200 has no CPU path")
+    if t.dtype is not torch.int32:
+        raise TypeError(f"{name} must be {torch.int32}, got {t.dtype}")
+    raise ValueError(f"{name} must hold a word on cuda:{device}, got {tuple(t.shape)} on {t.device}")
+
+
 def _rows(t: torch.Tensor, name: str, dtype=None) -> int:
     """Check rows that may lie further apart than they are wide (a range of columns of wider rows) and return their pitch."""
     if not t.is_cuda:
@@ -2537,6 +2548,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, take: in
                 raise ValueError(f"beam selection: the output {what} are {tuple(t.shape)}, not {(Q, take)}")
     if not here == logits.get_device() == scores.get_device() == scratch.get_device() == out[0].get_device():
         _on_current_device(logits, scores, scratch, *out)
+    _req_word(error_flag, "error_flag", here)
+    _req_word(status, "status", here)
     _lib.check(L.qnn_beam_select(logits.data_ptr(), scores.data_ptr(), Q, beams, V, take, scratch.data_ptr(), out[0].data_ptr(), out[1].data_ptr(),
                                  out[2].data_ptr(), _p(status), _p(error_flag), _stream()), "beam_select", 2)
     return out
