@@ -882,6 +882,8 @@ def sample(logits: torch.Tensor, top_k: int, temperature: float, top_p: float, p
         raise ValueError("sample: out_tokens / rng_state are shorter than the batch")
     if scratch.numel() * scratch.element_size() < sample_scratch_bytes(R, V, top_k):
         raise ValueError("sample: scratch is too small")
+    _req_word(error_flag, "error_flag", logits.get_device())
+    _req_word(status, "status", logits.get_device())
     L = _lib.load()
     _lib.check(L.qnn_sample(_p(logits), R, V, int(top_k), float(temperature), float(top_p), float(penalty),
                             _p(rng_state), _p(seen), _p(seen_rows), _p(scratch), _p(out_tokens), _p(error_flag),
@@ -918,6 +920,7 @@ def head_argmax(x: torch.Tensor, w: torch.Tensor, cap: Optional[float], cand: to
         raise ValueError(f"head_argmax: x is [*, {K}] but w is [*, {w.shape[1]}]")
     if cand.numel() < M * head_candidates(N) * 2:
         raise ValueError("head_argmax: the candidate buffer is too small")
+    _req_word(error_flag, "error_flag", x.get_device())
     L = _lib.load()
     if _takes_skinny_tcgen05(M, N, K):
         code = L.qnn_gemm_skinny_tcgen05_argmax(_p(x), _p(w), _p(cand), M, N, K, float(cap or 0.0), _p(error_flag),
@@ -942,6 +945,8 @@ def sample_candidates(cand: torch.Tensor, rows: int, ncand: int, vocab: int, top
     _req(rng_state, "rng_state", torch.int32, 1)
     if cand.numel() < rows * ncand * 2 or out_tokens.numel() < rows or rng_state.numel() < rows:
         raise ValueError("sample_candidates: a buffer is shorter than the batch")
+    _req_word(error_flag, "error_flag", cand.get_device())
+    _req_word(status, "status", cand.get_device())
     L = _lib.load()
     _lib.check(L.qnn_sample_candidates(_p(cand), rows, ncand, vocab, int(top_k), float(temperature), float(top_p),
                                        _p(rng_state), _p(seen), _p(seen_rows), _p(out_tokens), _p(error_flag),

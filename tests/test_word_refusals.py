@@ -44,3 +44,19 @@ def test_beam_selection(make, error):
     for word in ("error_flag", "status"):
         with pytest.raises(error):
             ops.beam_select(logits, scores, 2, 4, scratch, **{word: make()})
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("make,error", WRONG)
+def test_sampling(make, error):
+    logits, rng = torch.zeros(2, 50, device="cuda:0"), torch.ones(2, dtype=torch.int32, device="cuda:0")
+    out, cand = torch.zeros(2, dtype=torch.int32, device="cuda:0"), torch.zeros(2, 4, 2, device="cuda:0")
+    scratch = torch.empty(ops.sample_scratch_bytes(2, 50, 4), dtype=torch.uint8, device="cuda:0")
+    for words in ((make(), None), (None, make())):
+        with pytest.raises(error):
+            ops.sample(logits, 4, 1.0, 1.0, 1.0, rng, None, None, scratch, out, *words)
+        with pytest.raises(error):
+            ops.sample_candidates(cand, 2, 4, 50, 4, 1.0, 1.0, rng, None, None, out, *words)
+    with pytest.raises(error):
+        ops.head_argmax(torch.zeros(2, 64, dtype=torch.bfloat16, device="cuda:0"), torch.zeros(32, 64, dtype=torch.bfloat16, device="cuda:0"), None,
+                        torch.zeros(2 * ops.head_candidates(32) * 2, device="cuda:0"), make())
