@@ -358,3 +358,54 @@ def test_refusals():
         ops.SharedKeys(sh.groups[:, :3].contiguous(), sh.row_group, rows=2, keys=1, own=1)
     with pytest.raises(ValueError):
         ops.SharedKeys(sh.groups, sh.row_group, rows=0, keys=1, own=1)
+
+
+@pytest.mark.parametrize("nq,nkv,hd", [(8, 4, 256), (8, 2, 128), (16, 2, 64)])
+@pytest.mark.parametrize("cap", [None, 50.0])
+def test_many_rows_captured_behind_a_kernel_that_writes_their_queries(nq, nkv, hd, cap):
+    """Two calls of the two-kernel form on one scratch, each behind a kernel of this library that writes its queries, replayed back to back
+    with other lengths and groups: the kernel of the rows' own keys starts beside that of the common ones and must not be early."""
+    b = Batch([(0, 512, [513 + 3 * i for i in range(20)]), (0, 128, [150, 200, 129])], nq, nkv, hd, BF, alone=[70], seed=hd)
+    B, sh = b.B, b.shared(keys=1 << 20)
+    plan = ops.shared_attention_plan(BF, B, nq, nkv, hd, sh)
+    assert plan.kernels == 3
+    scratch = torch.full((plan.scratch_bytes // 4,), float("nan"), device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    rows = torch.randn((3 * B, b.qkv.shape[1]), device=DEV, generator=g).to(BF)          # rows 0 .. B - 1 are the step's
+    table, slots, lens = b.i32(b.table), b.i32(b.slots), b.i32(b.slot_len)
+
+    def call(k):
+        ops.copy_slots([rows], list(range(k * B, (k + 1) * B)), list(range(B)))
+        return ops.attn_decode_shared(rows[:B], nq, nkv, hd, b.k, b.v, table, PAGE, 0, slots, lens, sh, hd ** -0.5, cap, None, plan, scratch)
+
+    call(1)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = [call(1), call(2)]
+    whole, got = list(b.lens), []
+    steps = ((512, 0), (448, 0), (0, 0), (512, 100), (512, 0))
+    for end, cut in steps:                                           # nothing waits between the replays
+        sh.groups[0, 3] = end
+        lens[torch.from_numpy(b.slots[:20].astype(np.int64)).to(DEV)] = b.i32([n - cut for n in whole[:20]])
+        graph.replay()
+        got.append([o.clone() for o in outs])
+    torch.cuda.synchronize()
+    ops.raise_on_status(torch.device(DEV))
+    for (end, cut), pair in zip(steps, got):
+        b.lens = [n - cut for n in whole[:20]] + whole[20:]
+        for k, o in enumerate(pair):
+            b.qkv = rows[(k + 1) * B:(k + 2) * B]
+            b.check(o, hd ** -0.5, cap)
+    assert all(torch.equal(x, y) for x, y in zip(got[0], got[4]))
+
+
+@pytest.mark.parametrize("nq,nkv,hd,dtype,keys", [(8, 4, 256, BF, 1 << 20), (8, 2, 128, BF, 1 << 20), (16, 2, 64, BF, 1 << 20), (8, 2, 128, BF, 1), (6, 1, 24, FP, 1)])
+@pytest.mark.parametrize("cap", [None, 50.0])
+def test_same_bits_whatever_ran_before(nq, nkv, hd, dtype, keys, cap):
+    """results go by the numbers of ranges, not by what runs when or what the scratch holds"""
+    b = Batch([(0, 640, [641 + 5 * i for i in range(40)]), (0, 64, [90, 65])], nq, nkv, hd, dtype, alone=[300], seed=3)
+    one = b.run(hd ** -0.5, cap, (3, 2), keys=keys)
+    assert torch.isfinite(one).all()
+    for _ in range(20):
+        assert torch.equal(one, b.run(hd ** -0.5, cap, (3, 2), keys=keys))
