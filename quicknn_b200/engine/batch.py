@@ -30,14 +30,16 @@ class WholeSequences:
 class StepSharing:
     """The rows of a decode step whose sequences came from one another (``KVCache.fork``) and hold pages together: ``n_groups`` stretches
     of at most ``rows`` neighbouring rows; bounds of the keys that a group holds together and that a row has beside them, over all
-    groups of the cache (classes: powers of two); and, on the device, what the attention reads of them for each group of the cache
-    (``kernels.ops.SharedKeys``)."""
+    groups of the cache (classes: powers of two); how many positions of keys the rows need not read again where a group's are read once
+    (rounded down in steps of an eighth at most; None: as many as the bounds allow), by which a mixer decides whether they are; and, on the device, what the
+    attention reads of them for each group of the cache (``kernels.ops.SharedKeys``)."""
 
     n_groups: int
     rows: int
     keys: int
     own: int
     by_group: Tuple[Any, ...] = ()
+    spared: Optional[int] = None
 
 
 @dataclasses.dataclass

@@ -275,18 +275,20 @@ class Engine:
         row_group = [-1] * len(slots)
         for i, (r, n) in enumerate(runs):
             row_group[r:r + n] = [i] * n
-        tables, keys, own = [], 0, 64
+        tables, keys, own, spared = [], 0, 64, 0
         for g, ranges in zip(self.cache.groups, self.cache.shared_positions(slots, runs)):
             for (r, n), (begin, end) in zip(runs, ranges):
                 tables += (r, n, begin, end)
                 keys = max(keys, end - begin)
+            spared = max(spared, sum((n - 1) * (end - begin) for (_, n), (begin, end) in zip(runs, ranges)))
             tables += (0,) * (4 * (n_groups - len(runs)))
             for length, i in zip(lengths, row_group):
                 held = min(length, g.need.window) if g.ring else length
                 own = max(own, held - (ranges[i][1] - ranges[i][0] if i >= 0 else 0))
         if not keys:
             return None
-        return StepSharing(n_groups, most, up(keys), up(own)), np.asarray(tables, np.int32), np.asarray(row_group, np.int32)
+        low = max(spared.bit_length() - 4, 0)
+        return StepSharing(n_groups, most, up(keys), up(own), spared=spared >> low << low), np.asarray(tables, np.int32), np.asarray(row_group, np.int32)
 
     def _decode(self, slots, starts, tokens_dev, use_graph, tail, rows):
         n_seqs, B = len(slots), rows                 # B rows, of which the last B - n_seqs belong to no sequence
@@ -297,7 +299,7 @@ class Engine:
         # that lead to the same decisions share one); the schedule of a class is asked once
         shared = self._sharing(slots, [p + 1 for p in starts])
         bounds = shared[0] if shared is not None else None
-        held = (bounds.n_groups, bounds.rows, bounds.keys, bounds.own) if shared is not None else None
+        held = (bounds.n_groups, bounds.rows, bounds.keys, bounds.own, bounds.spared) if shared is not None else None
         shape = (B, longest, spread, held, tuple(sorted(self.tuning.items())))
         sched = self._schedules.get(shape)
         if sched is None:

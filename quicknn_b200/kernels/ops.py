@@ -13,6 +13,7 @@ for it, for comparisons.
 from __future__ import annotations
 
 import ctypes
+import math
 import os
 from typing import NamedTuple, Optional, Sequence, Tuple
 
@@ -2418,16 +2419,52 @@ def shared_attention_plan(dtype: torch.dtype, n_rows: int, n_heads: int, n_kv: i
 
 
 def shared_attention_pays(dtype: torch.dtype, n_heads: int, n_kv: int, head_dim: int, shared, window: Optional[int] = None) -> bool:
-    """Whether a decode step should read common keys once (``attn_decode_shared``) rather than once per row (``attn_decode``): from so many
-    common keys on.  Measured, us, once / per row, rows with up to 100 keys of their own: 2 rows, 4 kv heads of 256, two query heads each: 64 keys
-    5.5 / 5.9, 512 5.7 / 8.2, 4096 8.5 / 17.6; 8 rows: 64 7.5 / 6.5, 256 8.1 / 8.4, 512 8.8 / 10.3; 8 rows, 16 kv heads of 128: 256 9.4 / 7.6, 512
-    10.0 / 9.7, 1024 10.9 / 13.8; 32 rows, 4 kv heads of 64: 512 9.9 / 8.0, 1024 11.6 / 10.8, 2048 13.4 / 15.9.  The kernel for any head size:
-    6 heads of 24 on one, float32, 4 rows: 128 7.9 / 8.0, 1024 8.4 / 13.8; at head size 256 it keeps too little in flight: 8 rows 1024 29 / 27, 2048
-    39 / 44, eight groups of 4 rows never."""
-    keys, heads = min(shared.keys, window or shared.keys), n_heads // n_kv
+    """Whether a decode step should read common keys once (``attn_decode_shared``) rather than once per row (``attn_decode``).  ``shared``: bounds as
+    in ``SharedKeys``, beside which ``spared`` may say how many positions of keys the rows need not read again (else what the bounds allow).
+
+    Measured with the plans that a step's bounds lead to, us, once / per row, in 35 head shapes, 2 to 128 rows, 64 to 8192 common keys, up to 100 or
+    up to 1000 of a row's own.  Where the rule says once, that took 0.05 to 1.07 times as long (1.07: 16 rows, 4 kv heads of 128 with eight query heads
+    each, 1024 keys 12.6 / 11.8).
+    * bfloat16, heads of 256: once, always (2 rows, 4 kv heads, 128 keys 5.1 / 7.0; 16 rows, 256 keys 9.7 / 9.6; 128 rows, 8192 keys 37 / 484).
+    * heads of 64 and 128, in mma.sync: from some hundred keys on, or where much is spared (8 rows, 16 kv heads of 128: 384 keys 9.5 / 8.9, 512 9.6 / 9.7;
+      32 rows, 16 kv heads with a query head each, 512 10 / 24; 32 rows, 4 kv heads of 64: 384 8.6 / 7.1, 768 8.6 / 8.9).
+    * the same, with the common keys on tcgen05, whose start takes longer: 8 groups of 4 rows, 4 kv heads of 128 with eight query heads each: 768 keys 20.9 /
+      14.8, 2048 24 / 26; 32 rows, 8 kv heads of 64, 768 18.3 / 13.8, 1024 16.4 / 16.2; 128 rows, 4 of 64, 768 26.0 / 21.8, 8192 36 / 148.
+    * other head sizes on FMA units, which take the rows' own keys with places for 16 queries however few there are.  Up to 64 elements: with three query
+      heads or more on a kv head nearly always (6 heads of 24, 128 rows, 512 keys 17 / 45; 16 heads of 64 on 2 in float32: 16 rows, 256 keys 15.1 / 11.8,
+      8 rows, 2048 17.6 / 33); with one or two where the common keys outnumber a row's own (8 heads of 48, 8 groups of 4, 512 keys beside 1000 59 / 29;
+      128 rows, 8192 beside 100 147 / 528).  Up to 256: groups of many rows and eight times as many common keys (8 heads of 96 on 4, 16 rows, 2048 keys
+      beside 1000 64 / 37; 32 rows beside 100 50 / 55).  Above: never (16 heads of 320 on one, 8 rows, 4096 keys beside 1000 234 / 118)."""
+    heads, queries = n_heads // n_kv, shared.rows * (n_heads // n_kv)
+    if shared.rows < 2 or shared.n_groups < 1:
+        return False
+    most = (shared.rows - 1) * shared.n_groups                      # rows that need not read the common keys
+    spared = getattr(shared, "spared", None)
+    keys = shared.keys if spared is None else min(shared.keys, spared / most)       # of a group, in the mean (at least)
+    if window and keys + shared.own > window:                       # of what a window leaves, a row's own keys come first
+        keys = max(0, window - shared.own)
+    own = shared.own
     if dtype == torch.bfloat16 and head_dim in (64, 128, 256):
-        return keys >= (1024 if head_dim == 64 else 512)
-    return keys >= 256 if head_dim <= 64 else keys >= 2048 and shared.rows * heads >= 16 and shared.n_groups == 1
+        if head_dim == 256:
+            return keys >= 64
+        traffic = 4 * most * keys * n_kv * head_dim                 # bytes of keys and values that are not read again
+        if _lib.load().qnn_attn_shared_tile(BF16, head_dim, queries, shared.n_groups * n_kv, shared.keys) >= 128:
+            if head_dim == 64:
+                return traffic >= (104e6 if heads <= 4 else 64e6) or (heads <= 4 and keys >= 960)
+            return heads <= 4 or traffic >= 64e6 or (heads > 8 and keys >= 1024)
+        if head_dim == 64:
+            return keys >= 512 if heads > 4 else keys >= 640 or traffic >= 32e6
+        return keys >= 64 if heads > 4 else keys >= 440 or traffic >= 26e6
+    if head_dim > 256:
+        return False
+    if head_dim > 64:
+        rows = most / shared.n_groups * keys / max(shared.keys, 1) + 1              # (of a group, at least)
+        return keys >= max(1024, 8 * own) and rows >= 24 or keys >= max(512, 4 * own) and rows >= 48
+    if heads > 2:
+        return keys >= (64 if head_dim <= 56 else 384 if shared.rows >= 8 else 1024 if shared.rows >= 4 else math.inf)
+    if head_dim > 40:
+        return keys >= max(512, 4 * own) and shared.rows >= 4 or keys >= max(1024, 2 * own)
+    return dtype == torch.float32 and head_dim >= 32 and keys >= max(384, own)
 
 
 _SHARED_CHUNKS = tuple(sorted({16 * int(round(2 ** (i / 2))) for i in range(2, 28)}))       # 32 keys .. 128 K

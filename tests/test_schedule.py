@@ -155,3 +155,92 @@ def test_steps_whose_common_keys_go_to_different_kernels_do_not_share_a_graph(mo
                     schedules.setdefault((n_groups, rows, n_kv, hd, plan[:2]), set()).add(plan.kernels)
     assert any(len(k) > 1 for k in schedules.values())               # equal divisions for different kernels do occur
     assert all(len(k) == 1 for k in kernels.values())
+
+
+BF, FP = "bfloat16", "float32"
+# heads, kv heads, head size, groups, rows of a group, positions that need not be read again, most common keys, most own keys; us with the common keys read
+# once, and once per row: one B200, the plans of a step's bounds
+MEASURED = [
+    (BF, 8, 4, 256, 1, 128, 1040384, 8192, 100, 36.8, 483.7), (BF, 8, 4, 256, 1, 16, 3840, 256, 100, 9.7, 9.6),
+    (BF, 16, 8, 256, 1, 8, 1344, 192, 100, 9.1, 9.0), (BF, 9, 1, 256, 1, 2, 1536, 1536, 100, 9.0, 9.2),
+    (BF, 32, 16, 128, 1, 128, 1040384, 8192, 100, 48.0, 936.9), (BF, 32, 16, 128, 1, 8, 2688, 384, 100, 9.5, 8.9),
+    (BF, 32, 16, 128, 1, 8, 3584, 512, 100, 9.6, 9.7), (BF, 32, 4, 128, 8, 4, 13248, 768, 100, 20.9, 14.8),
+    (BF, 32, 4, 128, 4, 4, 14976, 1408, 100, 17.6, 13.8), (BF, 32, 4, 128, 1, 128, 1040384, 8192, 100, 38.2, 275.7),
+    (BF, 32, 4, 128, 1, 16, 15360, 1024, 100, 12.6, 11.8), (BF, 8, 4, 128, 1, 32, 11904, 384, 100, 9.5, 8.6),
+    (BF, 16, 1, 128, 4, 32, 63488, 704, 100, 29.6, 25.1), (BF, 16, 1, 128, 1, 128, 97536, 768, 100, 30.4, 27.4),
+    (BF, 16, 1, 128, 4, 32, 732096, 7424, 100, 37.3, 133.2), (BF, 8, 4, 64, 1, 32, 11904, 384, 100, 8.6, 7.1),
+    (BF, 8, 4, 64, 1, 32, 23808, 768, 100, 8.6, 8.9), (BF, 32, 8, 64, 1, 32, 23808, 768, 100, 18.3, 13.8),
+    (BF, 32, 8, 64, 8, 4, 12288, 640, 100, 14.4, 12.0), (BF, 32, 8, 64, 1, 128, 1040384, 8192, 100, 32.9, 282.2),
+    (BF, 32, 8, 64, 1, 32, 31744, 1024, 100, 16.4, 16.2), (BF, 16, 4, 64, 1, 128, 97536, 768, 100, 26.0, 21.8),
+    (BF, 16, 4, 64, 1, 128, 1040384, 8192, 100, 35.5, 147.9), (BF, 8, 1, 64, 1, 128, 97536, 768, 100, 18.8, 12.4),
+    (BF, 8, 1, 64, 16, 4, 83136, 1984, 1000, 18.6, 14.7), (BF, 12, 12, 64, 1, 2, 64, 64, 100, 4.7, 3.6),
+    (FP, 6, 1, 24, 1, 128, 1040384, 8192, 100, 103.7, 372.0), (BF, 6, 2, 40, 1, 4, 768, 256, 1000, 11.3, 10.9),
+    (BF, 6, 2, 40, 1, 128, 1040384, 8192, 100, 125.8, 443.6), (BF, 8, 2, 56, 1, 4, 1536, 512, 1000, 13.2, 12.6),
+    (FP, 16, 2, 64, 1, 2, 8192, 8192, 100, 25.1, 18.6), (FP, 16, 2, 64, 1, 16, 3840, 256, 100, 15.1, 11.8),
+    (FP, 16, 2, 64, 1, 8, 14336, 2048, 100, 17.6, 33.1), (FP, 8, 8, 16, 8, 4, 8256, 512, 1000, 39.9, 15.9),
+    (FP, 8, 8, 16, 16, 4, 78336, 1984, 1000, 78.1, 47.3), (BF, 4, 4, 32, 16, 4, 38592, 1024, 1000, 37.1, 18.8),
+    (FP, 4, 4, 32, 16, 4, 17472, 512, 1000, 47.2, 30.5), (FP, 4, 4, 32, 1, 128, 1040384, 8192, 100, 68.1, 282.2),
+    (FP, 8, 8, 64, 8, 4, 8640, 512, 1000, 72.7, 42.0), (FP, 8, 8, 64, 1, 128, 1040384, 8192, 100, 179.7, 983.9),
+    (FP, 8, 4, 64, 1, 16, 3840, 256, 100, 14.9, 9.8), (FP, 8, 4, 64, 16, 4, 10560, 256, 1000, 54.3, 43.8),
+    (BF, 8, 8, 48, 8, 4, 8640, 512, 1000, 58.5, 29.4), (BF, 8, 8, 48, 1, 128, 1040384, 8192, 100, 146.9, 527.7),
+    (BF, 8, 4, 96, 1, 16, 30720, 2048, 1000, 63.5, 37.2), (BF, 8, 4, 96, 1, 8, 14336, 2048, 1000, 37.4, 22.6),
+    (BF, 8, 4, 96, 1, 32, 63488, 2048, 100, 50.0, 54.8), (BF, 8, 8, 80, 1, 32, 63488, 2048, 1000, 160.5, 94.0),
+    (BF, 8, 8, 80, 1, 128, 1040384, 8192, 100, 341.2, 935.9), (FP, 8, 4, 256, 1, 16, 30720, 2048, 1000, 168.5, 111.4),
+    (FP, 8, 4, 256, 1, 128, 1040384, 8192, 100, 807.8, 2047.8), (FP, 8, 2, 128, 1, 32, 63488, 2048, 1000, 87.1, 60.4),
+    (BF, 16, 1, 320, 1, 8, 28672, 4096, 1000, 233.6, 118.1), (BF, 16, 1, 576, 1, 4, 6144, 2048, 1000, 135.9, 120.0),
+    (BF, 8, 2, 512, 1, 128, 520192, 4096, 100, 1160.1, 779.0),
+]
+
+
+@pytest.mark.parametrize("case", MEASURED, ids=lambda c: "-".join(str(x) for x in c[:9]))
+def test_common_keys_are_read_once_where_it_was_measured_to_pay(case):
+    """Where the rule says once, that took at most 1.07 times as long; a gain of more than a third is not left.  (A step rounds the
+    positions that are spared down by up to an eighth.)"""
+    import torch
+    from quicknn_b200.engine.batch import StepSharing
+    from quicknn_b200.kernels import ops
+    dtype, heads, n_kv, hd, groups, rows, spared, keys, own, once, per_row = case
+    up = lambda n: 1 << max(n - 1, 0).bit_length()                          # noqa: E731
+    for least in (spared, spared * 7 // 8 + 1):
+        sharing = StepSharing(up(groups), up(rows), up(keys), up(own), spared=least)
+        pays = ops.shared_attention_pays(getattr(torch, dtype), heads, n_kv, hd, sharing)
+        if once > 1.07 * per_row:
+            assert not pays
+        if once < 0.66 * per_row:
+            assert pays
+    # without the number of spared positions the bounds say it; a user's own numbers may be exact
+    exact = StepSharing(groups, rows, keys, own)
+    assert ops.shared_attention_pays(getattr(torch, dtype), heads, n_kv, hd, exact) in (True, False)
+
+
+def test_a_window_that_a_rows_own_keys_fill_leaves_nothing_to_share():
+    import torch
+    from quicknn_b200.engine.batch import StepSharing
+    from quicknn_b200.kernels import ops
+    bf = torch.bfloat16
+    pays = lambda own, window: ops.shared_attention_pays(bf, 8, 4, 256, StepSharing(1, 8, 8192, own, spared=7 * 8000), window)      # noqa: E731
+    assert pays(128, None) and pays(128, 4096) and pays(2048, 4096) and not pays(4096, 4096) and not pays(8192, 1024)
+    assert not ops.shared_attention_pays(bf, 8, 4, 256, StepSharing(1, 1, 8192, 64, spared=0))
+    assert not ops.shared_attention_pays(bf, 8, 4, 256, StepSharing(0, 0, 0, 64))
+
+
+def test_a_step_counts_the_positions_that_need_not_be_read_again():
+    """From the numbers as they are, rounded down by less than an eighth; the bounds are powers of two."""
+    import torch
+    from quicknn_b200.cache import KVCache
+    from quicknn_b200.parts import CacheNeed
+    cache = KVCache([CacheNeed(1, 4, None)], [None], 8192, 16, 2048, torch.float32, "cpu")
+    eng = Engine.__new__(Engine)
+    eng.cache = cache
+    rows = []
+    for n, copies in ((700, 4), (130, 2), (60, 1)):
+        s = cache.allocate()
+        cache.extend([(s, n)])
+        mine = [s] + cache.fork([s] * (copies - 1))
+        cache.extend([(x, n + 1 + 70 * i) for i, x in enumerate(mine)])
+        rows += mine
+    sharing, tables, row_group = eng._sharing(rows, [cache.length(s) for s in rows])
+    assert (sharing.n_groups, sharing.rows, sharing.keys, sharing.own) == (2, 4, 1024, 512)
+    true = 3 * 640 + 1 * 128                                                # whole pages of 700 and 130 positions
+    assert true * 7 / 8 < sharing.spared <= true
+    assert tables.tolist() == [0, 4, 0, 640, 4, 2, 0, 128] and row_group.tolist() == [0, 0, 0, 0, 1, 1, -1]
