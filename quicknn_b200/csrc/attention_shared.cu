@@ -675,20 +675,33 @@ bool many_rows(int dtype, int hd, int queries, long long walks, int keys) {
     return on_tensor_cores(dtype, hd) && queries > 16 && (queries + 15) / 16 * walks * keys >= MANY_WORK;
 }
 
+// Shared memory of a CTA of the mma.sync kernel: rings, barriers, and the page ids of an item, with room for all of a sequence's.  The 8, 6 and 3 CTAs
+// an SM of head size 64, 128 and 256 fit up to page tables of 2500, 780 and 2150 pages (160,000, 50,000 and 137,000 positions); with longer ones
+// fewer do.
+template <int HD>
+size_t mma_bytes(int nt, int max_pages) { return 1024 + Layout<HD>::ring_bytes(nt) + Layout<HD>::BARRIERS + ((size_t)max_pages + 2) * sizeof(int); }
+constexpr size_t MMA_MOST_BYTES = 220 * 1024;
+
+// Whether the tensor cores take these sizes.  Page tables of more than 38,000 pages (2.4 million positions) leave no room for the tiles: they go to
+// the kernel for any head size, which then reads its page ids from the table.
+bool takes_tensor_cores(int dtype, int hd, int max_pages) {
+    if (!on_tensor_cores(dtype, hd)) return false;
+    return (hd == 64 ? mma_bytes<64>(2, max_pages) : hd == 128 ? mma_bytes<128>(2, max_pages) : mma_bytes<256>(2, max_pages)) <= MMA_MOST_BYTES;
+}
+
 template <int HD, int NT, bool BIAS, bool BESIDE>
 int launch_mma(const void* q, long long q_stride, const void* k_pool, const void* v_pool, long long pool_rows, const Cells& cells, const Shared& sh,
                int B, int nq, int nkv, const Scores& sc, float* part_o, float2* part_ml, int* status, cudaStream_t st) {
     const int G = nq / nkv, own_tile = G <= 8 ? 8 : 8 * NT;
     const long long common = BESIDE ? 0 : (long long)sh.n_groups * sh.common_tiles * sh.common_ranges, own = (long long)B * ((G + own_tile - 1) / own_tile) * sh.own_ranges;
     if (common + own > 0x7fffffff) return QNN_ERR_UNSUPPORTED;
-    const size_t smem = 1024 + Layout<HD>::ring_bytes(NT) + Layout<HD>::BARRIERS + ((size_t)cells.max_pages + 2) * sizeof(int);
-    if (smem > 220 * 1024) return QNN_ERR_UNSUPPORTED;
+    const size_t smem = mma_bytes<HD>(NT, cells.max_pages);
     CUtensorMap map;
     KV kv;
     if (const int rc = make_pools_map(&map, &kv, k_pool, v_pool, pool_rows, HD, TILE)) return rc;
     auto kern = attn_shared_mma_kernel<HD, NT, BIAS, BESIDE>;
     static OncePerDevice asked;
-    if (const int rc = allow_shared(asked, kern, 220 * 1024)) return rc;
+    if (const int rc = allow_shared(asked, kern, MMA_MOST_BYTES)) return rc;
     // (beside the kernel of the common keys also where the grid is larger than others are launched early with)
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(common + own), nkv);
@@ -779,8 +792,9 @@ QNN_API int qnn_attn_decode_shared(const void* q, long long q_stride, int dtype,
     if (page_size < 16 || (page_size & (page_size - 1)) || ring < 0 || ring % page_size) return QNN_ERR_ARGUMENT;
     if (ring > 0 && (window <= 0 || window > ring || ring / page_size > max_pages)) return QNN_ERR_ARGUMENT;   // a ring holds no more
     const int G = nq / nkv, esize = dtype == QNN_DT_BF16 ? 2 : 4;
-    const bool many = n_groups > 0 && page_size >= 64 && many_rows(dtype, hd, most_rows * G, (long long)n_groups * nkv, most_keys);
-    const int tile = many ? MANY_TILE : (on_tensor_cores(dtype, hd) ? 8 * column_tiles(most_rows * G) : qnn_attn_shared_tile(dtype, hd, most_rows * G, 0, 0));
+    const bool tensor = takes_tensor_cores(dtype, hd, max_pages);
+    const bool many = tensor && n_groups > 0 && page_size >= 64 && many_rows(dtype, hd, most_rows * G, (long long)n_groups * nkv, most_keys);
+    const int tile = many ? MANY_TILE : tensor ? 8 * column_tiles(most_rows * G) : on_tensor_cores(dtype, hd) ? GEN_QT : qnn_attn_shared_tile(dtype, hd, most_rows * G, 0, 0);
     if (tile <= 0) return QNN_ERR_UNSUPPORTED;
     if ((q_stride * esize) % 16 || ((uintptr_t)q & 15) || ((uintptr_t)k_pool & 15) || ((uintptr_t)v_pool & 15) || ((uintptr_t)part_o & 15) ||
         ((uintptr_t)part_ml & 7) || ((uintptr_t)groups & 15) || ((uintptr_t)out & 15) || (out_stride * esize) % 16)
@@ -788,14 +802,14 @@ QNN_API int qnn_attn_decode_shared(const void* q, long long q_stride, int dtype,
     const Cells cells = {page_table, max_pages, 31 - __builtin_clz((unsigned)page_size), ring / page_size, slots, slot_len, window};
     const int common_tiles = (most_rows * G + tile - 1) / tile;
     const Shared sh = {(const int4*)groups, row_group, n_groups, B, common_ranges, own_ranges, common_tiles, most_rows};
-    const int own_tile = on_tensor_cores(dtype, hd) ? 8 : GEN_QT;
+    const int own_tile = tensor ? 8 : GEN_QT;
     const long long items = (long long)n_groups * common_tiles * common_ranges + (long long)B * ((G + own_tile - 1) / own_tile) * own_ranges;
     const long long pool_rows = pool_pages * nkv * page_size;         // of the pools as matrices of head rows
     if (items > 0x7fffffff || (long long)B * nq > 0x7fffffff || pool_rows <= 0 || pool_rows > 0x7fffffff) return QNN_ERR_UNSUPPORTED;
     const Scores sc = {scale, cap, slopes};
     float2* ml = (float2*)part_ml;
     int rc = QNN_ERR_UNSUPPORTED;
-    if (on_tensor_cores(dtype, hd)) {
+    if (tensor) {
         if (many) {
             const SharedLaunch a = {q, q_stride, k_pool, v_pool, pool_rows, cells, sh, nq, nkv, hd, sc, part_o, ml, status};
             if (const int err = launch_common_tcgen05(a, st)) return err;

@@ -409,3 +409,25 @@ def test_same_bits_whatever_ran_before(nq, nkv, hd, dtype, keys, cap):
     assert torch.isfinite(one).all()
     for _ in range(20):
         assert torch.equal(one, b.run(hd ** -0.5, cap, (3, 2), keys=keys))
+
+
+@pytest.mark.parametrize("nq,nkv,hd,dtype,rows,keys", [(8, 4, 256, BF, 3, None), (8, 2, 128, BF, 3, None), (16, 2, 64, BF, 3, None), (8, 2, 128, BF, 40, 1 << 20), (6, 1, 24, FP, 3, None),
+                                                       (4, 2, 96, BF, 3, None)])
+@pytest.mark.parametrize("window", [0, 300])
+def test_page_tables_for_millions_of_positions(nq, nkv, hd, dtype, rows, keys, window):
+    """more page ids than fit beside the tiles"""
+    b = Batch([(0, 448, [450 + 31 * r for r in range(rows)])], nq, nkv, hd, dtype, alone=[200], window=window, seed=hd)
+    wide = np.zeros((b.table.shape[0], 60000), dtype=np.int32)
+    wide[:, :b.table.shape[1]] = b.table
+    b.table = wide
+    b.check(b.run(hd ** -0.5, 50.0, keys=keys), hd ** -0.5, 50.0)
+
+
+@pytest.mark.parametrize("nq,nkv,hd", [(8, 4, 256), (4, 2, 64)])
+def test_rings_of_millions_of_positions(nq, nkv, hd):
+    """of which sequences have filled little"""
+    b = Batch([(0, 448, [450, 500, 700])], nq, nkv, hd, BF, window=60000 * 64, ring=0, seed=hd)
+    wide = np.zeros((b.table.shape[0], 60000), dtype=np.int32)
+    wide[:, :b.table.shape[1]] = b.table
+    b.table, b.ring = wide, 60000 * 64
+    b.check(b.run(hd ** -0.5), hd ** -0.5)
