@@ -458,11 +458,21 @@ beam_pick_kernel(const float* __restrict__ logits, int V, int beams, int take, i
 int least_segment(int V) { return V < 16384 ? 128 : 512; }
 int segment_of(int rows, int V) { return least_segment(V) == 512 && (long long)rows * V > 148LL * 16 * 512 ? 1024 : least_segment(V); }
 int segments_of(int V, int segment) { return (V + 3 + segment - 1) / segment; }
+// One block does it all for few logits: a launch less, and a threshold from single logits.  us so and by two kernels: 4 beams x 1000, 8 best 6.4 /
+// 8.0; 11 x 515, 22 best 9.4 / 15; 10 x 1015, 20 best 10.8 / 15.8 (where segments are few, the `take`-th of their maxima lets hundreds pass).
+bool one_block(int segment, int segments, int take) { return segment == 128 && (segments <= 64 || segments <= (4 * take < 128 ? 4 * take : 128)); }
 
 }  // namespace
 
 // the most segments that a row is cut into, however many rows there are
 QNN_API int qnn_beam_select_segments(int V) { return V <= 0 ? 0 : segments_of(V, least_segment(V)); }
+
+// Launches of a call with these sizes.
+QNN_API int qnn_beam_select_kernels(int requests, int beams, int V, int take) {
+    if (requests <= 0 || V <= 0) return 0;
+    const int segment = segment_of(requests * beams, V);
+    return one_block(segment, beams * segments_of(V, segment), take) ? 1 : 2;
+}
 
 // logits: [requests * beams, V] float32; scores: [requests * beams]; the outputs [requests, take].  Scratch: requests * beams *
 // qnn_beam_select_segments(V) float2.  take <= 64; beams * V < 2^32.
@@ -472,9 +482,7 @@ QNN_API int qnn_beam_select(const float* logits, const float* scores, int reques
     if (beams < 1 || V < 1 || take < 1 || take > SELECT_MOST || ((uintptr_t)logits & 3)) return QNN_ERR_ARGUMENT;
     if ((long long)requests * beams > 65535 || (long long)beams * V >= 0xffffffffLL) return QNN_ERR_UNSUPPORTED;
     const int rows = requests * beams, segment = segment_of(rows, V), segments = segments_of(V, segment);
-    // One block does it all for few logits: a launch less, and a threshold from single logits.  us so and by two kernels: 4 beams x 1000, 8 best 6.2 /
-    // 8.0; 11 x 515, 22 best 9.4 / 15; 10 x 1015, 20 best 10.8 / 15.8 (where segments are few, the `take`-th of their maxima lets hundreds pass).
-    const bool alone = segment == 128 && (beams * segments <= 64 || beams * segments <= min(128, 4 * take));
+    const bool alone = one_block(segment, beams * segments, take);
     const size_t smem = sizeof(Found) + (size_t)(beams + 1) / 2 * 2 * sizeof(double) + (size_t)(beams * segments + 3) / 4 * 4 * sizeof(unsigned) +
                         (alone ? (size_t)beams * segments * (sizeof(float2) + 128 * sizeof(float)) : 0);
     if (smem > 200 * 1024 || (long long)rows * segments > 0x7fffffff) return QNN_ERR_UNSUPPORTED;

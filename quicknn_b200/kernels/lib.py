@@ -158,6 +158,7 @@ _SIGNATURES: Dict[str, list] = {
     "qnn_attn_decode_shared": [c_vp, c_ll, c_int, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_vp, c_vp, c_int, c_vp, c_int, c_int, c_int, c_vp, c_int,
                                c_int, c_int, c_float, c_float, c_int, c_int, c_int, c_vp, c_vp, c_vp, c_ll, c_vp, c_vp, c_ll, c_vp, c_vp],
     "qnn_beam_select_segments": [c_int],
+    "qnn_beam_select_kernels": [c_int, c_int, c_int, c_int],
     "qnn_beam_select": [c_vp, c_vp, c_int, c_int, c_int, c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp],
     "qnn_copy_slots": [c_vp, c_int, c_vp, c_int, c_vp],
     "qnn_copy_pages": [c_vp, c_vp, c_int, c_ll, c_int, c_int, c_int, c_int, c_vp, c_int, c_vp],

@@ -2593,7 +2593,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, take: in
     _req_word(error_flag, "error_flag", here)
     _req_word(status, "status", here)
     _lib.check(L.qnn_beam_select(logits.data_ptr(), scores.data_ptr(), Q, beams, V, take, scratch.data_ptr(), out[0].data_ptr(), out[1].data_ptr(),
-                                 out[2].data_ptr(), _p(status), _p(error_flag), _stream()), "beam_select", 2)
+                                 out[2].data_ptr(), _p(status), _p(error_flag), _stream()), "beam_select", L.qnn_beam_select_kernels(Q, beams, V, take))
     return out
 
 

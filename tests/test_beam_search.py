@@ -125,3 +125,12 @@ def test_refusals():
         beam_search(Toy(max_tokens=128), [[1]], o)                                   # three beams hold three pages
     toy = Toy(max_tokens=3 * 64)
     assert len(beam_search(toy, [[1], [2]], o)) == 2 and toy.finished == 2           # one request at a time
+
+
+def test_launches_of_the_selection_are_counted_as_they_are():
+    """one kernel where a request has few logits, else two, none without a request"""
+    from quicknn_b200.kernels import lib
+    kernels = lib.load().qnn_beam_select_kernels
+    assert [kernels(*sizes) for sizes in ((1, 4, 1000, 8), (16, 4, 1000, 8), (1, 1, 3000, 8), (1, 11, 515, 22), (1, 64, 130, 64))] == [1] * 5
+    assert [kernels(*sizes) for sizes in ((1, 8, 256000, 16), (16, 5, 255029, 10), (1, 1, 16384, 2), (1, 8, 16383, 16))] == [2] * 4
+    assert kernels(0, 4, 1000, 8) == 0
