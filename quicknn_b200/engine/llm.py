@@ -114,28 +114,33 @@ class _Backend(GenerationBackend):
 
 
 class _PrefixBackend(_Backend):
-    """The backend of requests behind one common text: the text runs once, on a sequence that every request forks.  With ``one_batch``
-    the last of its users is the sequence itself; otherwise it keeps a slot until ``close``."""
+    """The backend of requests behind one common text: the text runs once, on a sequence that every request forks.  With ``kept`` it
+    keeps a slot and its pages until ``close``; without, every batch runs it on a sequence that is then its first request's."""
 
     def __init__(self, engine: Engine, sampler: Sampler, max_batch: int, run_ahead: bool, seed: Optional[int], prefix: List[int],
-                 one_batch: bool):
-        super().__init__(engine, sampler, max_batch if one_batch else max_batch - 1, run_ahead, seed)
-        self.prefix, self.one_batch = prefix, one_batch
+                 kept: bool):
+        super().__init__(engine, sampler, max_batch - 1 if kept else max_batch, run_ahead, seed)
+        self.prefix, self.kept = prefix, kept
         self.base: Optional[int] = None
         self.begun: List[int] = []                   # requests that have been started behind the prefix
-        if not one_batch:
-            self.max_tokens -= (len(prefix) + PAGE - 1) // PAGE * PAGE
+        if kept:
+            self.max_tokens -= self.pages_of(prefix)
+
+    @staticmethod
+    def pages_of(prefix: Sequence[int]) -> int:
+        """Positions of the pages that the prefix takes."""
+        return (len(prefix) + PAGE - 1) // PAGE * PAGE
 
     def begin(self, first_index: int, prompts: Sequence[Sequence[int]]) -> np.ndarray:
         eng, n = self.engine, len(prompts)
         if self.base is None:
             self.base = eng.new_sequence()
             eng.step([(self.base, self.prefix)], [()])
-        if self.one_batch:
+        if self.kept:
+            self.slots = eng.fork([self.base] * n)
+        else:
             self.slots, self.base = [self.base], None
             self.slots += eng.fork(self.slots * (n - 1))
-        else:
-            self.slots = eng.fork([self.base] * n)
         sampled = self._start(first_index, prompts, [p[len(self.prefix):] for p in prompts])
         self.begun += range(first_index, first_index + n)
         return sampled
@@ -335,7 +340,7 @@ class LLM:
         up to ``max_batch``, one batch after another.  ``prefix``: ids that stand in front of every prompt (each of which has at least
         one id of its own): they run once, every request goes on from there, and the attention of the replies' steps reads their keys
         once for all requests.  The results count them as part of the prompts, of requests that were started as reused ones.  With more requests than a batch holds the
-        prefix keeps one of the ``max_batch`` sequences."""
+        prefix keeps one of the ``max_batch`` sequences; where a request has no room in the cache beside it, every batch runs it anew."""
         options = options or GenerationOptions()
         options.validate()
         stops = self.stop_ids if stop_ids is None else list(stop_ids)
@@ -346,10 +351,16 @@ class LLM:
                     raise PromptError(f"request {i}: an empty prompt")
             prompts = [prefix + list(p) for p in prompts]
             cache = self.engine.cache
-            one = len(plan_batches([len(p) for p in prompts], options, self.max_batch, cache.max_tokens, self.engine.max_seq)) <= 1
-            if not one and self.max_batch < 2:
+            lens = [len(p) for p in prompts]
+            kept = len(plan_batches(lens, options, self.max_batch, cache.max_tokens, self.engine.max_seq)) > 1
+            if kept and self.max_batch < 2:
                 raise PromptError("several batches behind one prefix need a max_batch of 2 at least: the prefix keeps a sequence")
-            backend = _PrefixBackend(self.engine, self._sampler(options), self.max_batch, self.run_ahead, options.seed, prefix, one)
+            try:                                         # whether every request fits beside the prefix
+                if kept:
+                    plan_batches(lens, options, self.max_batch - 1, cache.max_tokens - _PrefixBackend.pages_of(prefix), self.engine.max_seq)
+            except PromptError:
+                kept = False
+            backend = _PrefixBackend(self.engine, self._sampler(options), self.max_batch, self.run_ahead, options.seed, prefix, kept)
         else:
             backend = _Backend(self.engine, self._sampler(options), self.max_batch, self.run_ahead, options.seed)
         try:

@@ -1,4 +1,5 @@
-"""What the results of requests behind a common prefix say of it when a run is cancelled, over an engine that is not there."""
+"""Requests behind a common prefix over an engine that is not there: what their results say of it when a run is cancelled, and caches
+that do not hold a request beside the prefix."""
 from types import SimpleNamespace
 
 import numpy as np
@@ -61,3 +62,13 @@ def test_without_a_prefix_nothing_is_reused(fake, monkeypatch):
     monkeypatch.setattr(module._Backend, "_start", lambda self, first, prompts, new: np.full(len(prompts), 7))
     got = fake.generate([[1, 2]] * 2, GenerationOptions.greedy(1), stop_ids=[])
     assert [r.reused_tokens for r in got] == [0, 0]
+
+
+@pytest.mark.parametrize("max_tokens,max_batch,runs", [(512, 3, 3), (576, 3, 1), (1024, 3, 1), (4096, 2, 1)])
+def test_a_request_that_has_no_room_beside_the_prefix_runs_without_it(fake, max_tokens, max_batch, runs):
+    """Each request may grow to 512 positions, the prefix takes a page of 64.  A cache that holds a request alone runs the prefix for every
+    batch; one that holds both runs it once."""
+    fake.engine.cache.max_tokens, fake.max_batch = max_tokens, max_batch
+    got = fake.generate([[1, 2]] * 3, GenerationOptions.greedy(480), prefix=[5] * 30, stop_ids=[7])
+    assert [r.finish_reason for r in got] == ["eos"] * 3 and [r.reused_tokens for r in got] == [30] * 3
+    assert fake.engine.prefixes_run == runs and sorted(fake.engine.free) == [0, 1, 2]
