@@ -2,7 +2,6 @@
 from __future__ import annotations
 
 import dataclasses
-import math
 from typing import List, Optional, Sequence
 
 import numpy as np
@@ -31,8 +30,9 @@ class BeamOptions:
             p.append(f"beams must be in 1..{ops.BEAM_MOST}")
         if self.max_new_tokens < 1:
             p.append("max_new_tokens must be >= 1")
-        if not isinstance(self.length_penalty, (int, float)) or not math.isfinite(self.length_penalty):
-            p.append("length_penalty must be finite")
+        # (lengths to the power of more than 32 either way leave the range of a float)
+        if not isinstance(self.length_penalty, (int, float)) or not abs(self.length_penalty) <= 32:
+            p.append("length_penalty must be in -32..32")
         if not 1 <= self.replies <= max(self.beams, 1):
             p.append("replies must be in 1..beams")
         return p

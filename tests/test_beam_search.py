@@ -134,3 +134,13 @@ def test_launches_of_the_selection_are_counted_as_they_are():
     assert [kernels(*sizes) for sizes in ((1, 4, 1000, 8), (16, 4, 1000, 8), (1, 1, 3000, 8), (1, 11, 515, 22), (1, 64, 130, 64))] == [1] * 5
     assert [kernels(*sizes) for sizes in ((1, 8, 256000, 16), (16, 5, 255029, 10), (1, 1, 16384, 2), (1, 8, 16383, 16))] == [2] * 4
     assert kernels(0, 4, 1000, 8) == 0
+
+
+@pytest.mark.parametrize("penalty", [33, 200.0, -200.0, 10 ** 400, float("inf"), float("nan"), "1"])
+def test_length_penalties_whose_powers_are_no_numbers_are_refused(penalty):
+    """200 ** 200.0 overflows and a score over 200 ** -200.0 divides by zero: in the middle of a search"""
+    with pytest.raises(OptionsError):
+        BeamOptions(length_penalty=penalty).validate()
+    BeamOptions(length_penalty=32).validate()
+    BeamOptions(length_penalty=-32.0).validate()
+    assert 0 < (2 ** 31) ** 32.0 < float("inf") and (2 ** 31) ** -32.0 > 0
