@@ -22,9 +22,9 @@ using namespace qnn;
 namespace {
 
 constexpr int SELECT_MOST = 64;               // continuations per request, at most
-// Of the second kernel's block.  It is short code that every warp runs once, so what it takes is instructions times warps: 4 beams x 1000 words 6.2 us with
-// 512, 7.7 with 1024; 10 beams x 1015 9.6 (256: 13).  Of its 11,000 cycles (8 beams x 99,521) 4,500 go to the logarithms of the sums, 2,000 to the
-// threshold, 3,000 to the second look, 1,500 to the order.
+// Of the second kernel's block.  It is short code that every warp runs once, so what it takes is instructions times warps: 4 beams x 1000 words 6.4 us
+// with 512 (when that took 6.2, 1024 took 7.7); 10 beams x 1015 10.8 (when that took 9.6, 256 took 13).  Of its 11,000 cycles (8 beams x 99,521)
+// 4,500 go to the logarithms of the sums, 2,000 to the threshold, 3,000 to the second look, 1,500 to the order.
 constexpr int THREADS = 512;
 constexpr int LIST = 2048;                    // places of the short list
 constexpr int MOST_REACHED = 512;             // segments that are looked at again

@@ -13,6 +13,7 @@ for it, for comparisons.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 import os
 from typing import NamedTuple, Optional, Sequence, Tuple
@@ -2557,6 +2558,13 @@ def beam_select_scratch_bytes(rows: int, vocab: int, take: int) -> int:
     return 8 * rows * int(_lib.load().qnn_beam_select_segments(vocab))
 
 
+@functools.lru_cache(maxsize=256)
+def _beam_select_sizes(requests: int, beams: int, vocab: int, take: int) -> Tuple[int, int]:
+    """(scratch bytes, launches) of a call with these sizes."""
+    L = _lib.load()
+    return 8 * requests * beams * int(L.qnn_beam_select_segments(vocab)), int(L.qnn_beam_select_kernels(requests, beams, vocab, take))
+
+
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, take: int, scratch: torch.Tensor,
                 out: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]] = None, error_flag: Optional[torch.Tensor] = None,
                 status: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -2564,8 +2572,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, take: in
 
     ``logits`` [requests * beams, vocab] float32, ``scores`` [requests * beams] float32 (the beams' sums of log-probabilities; -inf: a beam
     that is not there).  Returns (scores, beams, tokens), each [requests, take], best first: score + log softmax(logits) of a continuation
-    (formed in 64 bits, rounded once), its beam within the request and its token; equal scores in the order of (beam, token).  Places that
-    nothing is left for hold -inf, -1, -1.  A logit that is not finite is never chosen and sets bit 0 of ``error_flag``; ``status`` joins the
+    (formed in 64 bits, rounded once; the sum of a beam's exponentials is one of float32 exponentials, which moves the logarithm that all
+    of the beam's scores share by less than 2^-20), its beam within the request and its token; equal scores in the order of (beam, token).  A
+    request of more than about 45 million logits is refused (5 million where the vocabulary is below 16,384).  Places that nothing is left for hold -inf, -1, -1.  A logit that is not finite is never chosen and sets bit 0 of ``error_flag``; ``status`` joins the
     error word as in ``sample``."""
     here, f32, i32 = _here(), torch.float32, torch.int32
     _req(logits, "logits", f32, 2)
@@ -2574,12 +2583,12 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, take: in
     R, V = logits.shape
     if beams < 1 or R % beams or scores.numel() != R:
         raise ValueError(f"beam selection: {R} rows and {scores.numel()} scores are not requests of {beams} beams")
-    L = _lib.load()
     if not 1 <= take <= BEAM_MOST:
         raise ValueError(f"beam selection returns 1..{BEAM_MOST} continuations per request, not {take}")
-    if scratch.numel() * scratch.element_size() < 8 * R * L.qnn_beam_select_segments(V):
-        raise ValueError("beam selection: scratch is too small")
     Q = R // beams
+    need, launches = _beam_select_sizes(Q, beams, V, take)
+    if scratch.numel() * scratch.element_size() < need:
+        raise ValueError("beam selection: scratch is too small")
     if out is None:
         tokens = logits.new_empty((Q, take), dtype=i32)
         out = (logits.new_empty((Q, take)), torch.empty_like(tokens), tokens)
@@ -2590,10 +2599,11 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, take: in
                 raise ValueError(f"beam selection: the output {what} are {tuple(t.shape)}, not {(Q, take)}")
     if not here == logits.get_device() == scores.get_device() == scratch.get_device() == out[0].get_device():
         _on_current_device(logits, scores, scratch, *out)
-    _req_word(error_flag, "error_flag", here)
-    _req_word(status, "status", here)
-    _lib.check(L.qnn_beam_select(logits.data_ptr(), scores.data_ptr(), Q, beams, V, take, scratch.data_ptr(), out[0].data_ptr(), out[1].data_ptr(),
-                                 out[2].data_ptr(), _p(status), _p(error_flag), _stream()), "beam_select", L.qnn_beam_select_kernels(Q, beams, V, take))
+    if error_flag is not None or status is not None:
+        _req_word(error_flag, "error_flag", here)
+        _req_word(status, "status", here)
+    _lib.check(_lib.load().qnn_beam_select(logits.data_ptr(), scores.data_ptr(), Q, beams, V, take, scratch.data_ptr(), out[0].data_ptr(), out[1].data_ptr(),
+                                 out[2].data_ptr(), _p(status), _p(error_flag), _stream()), "beam_select", launches)
     return out
 
 
