@@ -2423,7 +2423,7 @@ def shared_attention_pays(dtype: torch.dtype, n_heads: int, n_kv: int, head_dim:
     """Whether a decode step should read common keys once (``attn_decode_shared``) rather than once per row (``attn_decode``).  ``shared``: bounds as
     in ``SharedKeys``, beside which ``spared`` may say how many positions of keys the rows need not read again (else what the bounds allow).
 
-    Measured with the plans that a step's bounds lead to, us, once / per row, in 35 head shapes, 2 to 128 rows, 64 to 8192 common keys, up to 100 or
+    Measured with the plans that a step's bounds lead to, us, once / per row, in 45 head shapes, 2 to 128 rows, 64 to 8192 common keys, up to 100 or
     up to 1000 of a row's own.  Where the rule says once, that took 0.05 to 1.07 times as long (1.07: 16 rows, 4 kv heads of 128 with eight query heads
     each, 1024 keys 12.6 / 11.8).
     * bfloat16, heads of 256: once, always (2 rows, 4 kv heads, 128 keys 5.1 / 7.0; 16 rows, 256 keys 9.7 / 9.6; 128 rows, 8192 keys 37 / 484).
@@ -2435,7 +2435,9 @@ def shared_attention_pays(dtype: torch.dtype, n_heads: int, n_kv: int, head_dim:
       heads or more on a kv head nearly always (6 heads of 24, 128 rows, 512 keys 17 / 45; 16 heads of 64 on 2 in float32: 16 rows, 256 keys 15.1 / 11.8,
       8 rows, 2048 17.6 / 33); with one or two where the common keys outnumber a row's own (8 heads of 48, 8 groups of 4, 512 keys beside 1000 59 / 29;
       128 rows, 8192 beside 100 147 / 528).  Up to 256: groups of many rows and eight times as many common keys (8 heads of 96 on 4, 16 rows, 2048 keys
-      beside 1000 64 / 37; 32 rows beside 100 50 / 55).  Above: never (16 heads of 320 on one, 8 rows, 4096 keys beside 1000 234 / 118)."""
+      beside 1000 64 / 37; 32 rows beside 100 50 / 55).  Above: where a thousand queries and more read the same keys, heads of 576 (16 on one kv head, 128
+      rows, 4096 keys 2399 / 5123, 4 rows, 2048 keys 136 / 120) and float32 up to 384; never heads of 288 to 512 in bfloat16 (16 of 320 on one, 8 rows, 4096
+      keys beside 1000 234 / 118)."""
     heads, queries = n_heads // n_kv, shared.rows * (n_heads // n_kv)
     if shared.rows < 2 or shared.n_groups < 1:
         return False
@@ -2457,7 +2459,8 @@ def shared_attention_pays(dtype: torch.dtype, n_heads: int, n_kv: int, head_dim:
             return keys >= 512 if heads > 4 else keys >= 640 or traffic >= 32e6
         return keys >= 64 if heads > 4 else keys >= 440 or traffic >= 26e6
     if head_dim > 256:
-        return False
+        total = heads * (most * keys / max(shared.keys, 1) + shared.n_groups)       # queries of a kv head (at least)
+        return keys >= 512 and (head_dim > 512 and total >= 1024 if dtype == torch.bfloat16 else head_dim <= 384 and total >= 2048)
     if head_dim > 64:
         rows = most / shared.n_groups * keys / max(shared.keys, 1) + 1              # (of a group, at least)
         return keys >= max(1024, 8 * own) and rows >= 24 or keys >= max(512, 4 * own) and rows >= 48

@@ -188,7 +188,7 @@ MEASURED = [
     (BF, 8, 8, 80, 1, 128, 1040384, 8192, 100, 341.2, 935.9), (FP, 8, 4, 256, 1, 16, 30720, 2048, 1000, 168.5, 111.4),
     (FP, 8, 4, 256, 1, 128, 1040384, 8192, 100, 807.8, 2047.8), (FP, 8, 2, 128, 1, 32, 63488, 2048, 1000, 87.1, 60.4),
     (BF, 16, 1, 320, 1, 8, 28672, 4096, 1000, 233.6, 118.1), (BF, 16, 1, 576, 1, 4, 6144, 2048, 1000, 135.9, 120.0),
-    (BF, 8, 2, 512, 1, 128, 520192, 4096, 100, 1160.1, 779.0),
+    (BF, 8, 2, 512, 1, 128, 520192, 4096, 100, 1160.1, 779.0), (BF, 16, 1, 576, 1, 128, 520192, 4096, 100, 2398.8, 5122.9),
 ]
 
 
