@@ -363,7 +363,10 @@ attn_shared_mma_kernel(const __grid_constant__ CUtensorMap map, const KV kv, con
 // all the warp's queries.  Exact exponentials and tanh in float32.  Bound by instructions (half of them products, four for each row of 16 bytes read)
 // and the wait for a tile, which no other is fetched behind: six groups of 16 rows, 16 heads of 64 on 2 kv heads, 2112 keys 64 us (11 of
 // float32 arithmetic); three groups of 5 rows, 6 heads of 24 on one, 960 keys 8.1.  (Four pieces of keys and values asked for at once: 90 us, for
-// what it adds in instructions.)
+// what it adds in instructions.)  bfloat16 at other head sizes than the tensor cores': 6 heads of 40 on 2, 32 rows, 2048 keys 18 us; 8 heads of 96 on 4,
+// 32 rows, 2048 keys 50; 16 heads of 576 on one, 8 rows, 4096 keys 319.  An item holds 16 queries, so a row's own keys cost what 16 queries' would.
+// Above head size 256 an accumulator of 4 x 32 elements a lane does not fit 255 registers (444 bytes of spills in float32, 204 in bfloat16; 8 to 24
+// bytes up to head size 64, where six CTAs an SM are asked for), and above 64 an SM holds one or two CTAs.
 constexpr int GEN_WARPS = 4, GEN_Q = 4, GEN_QT = GEN_WARPS * GEN_Q;
 
 __device__ __forceinline__ float redux_max(float x) {         // the largest of the warp's that is a number

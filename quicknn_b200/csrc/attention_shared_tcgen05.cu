@@ -8,7 +8,8 @@
 // row) that take the lower and the upper page of each pair.  What differs: the query rows lie apart (row, head), so each thread brings its
 // own from global memory to tensor memory; every key counts for every row, so nothing is masked but the half of a last pair that is not
 // there; results go out as float32 with their reference and sum.
-// With a softcap up to 70 the exponentials are taken against 0 (FIXED), else against a running maximum that both groups share.
+// With a softcap up to 70 the exponentials are taken against 0 (FIXED), else against a running maximum that both groups share.  Weights are rounded
+// to bfloat16 before they meet V, as in the library's other attention on tensor cores: up to 2^-8 of a weight, as the results are.
 // Bounds: the softmax between two products of a pair (special functions, two a score with a softcap, some of the exponentials on the FMA pipe
 // instead: 54 % of their pipe; tensor cores 35 %), and about 8 us a CTA in front of its first and behind its last page.  32 CTAs over 6144 keys
 // (128 rows, 2 heads of 128 on each of 16 kv heads) 83 us beside 134 of the rows' own keys, which hide it; 64 queries on 4096 keys of 4 kv heads of
