@@ -403,8 +403,10 @@ class KVCache:
 
         Sequences part where one of them first writes beside the others, and behind that place every page is somebody's own; in a
         ring the pages in front of what the longest still holds are overwritten.  So the common pages of two sequences are a stretch
-        that begins where the longest's do, and its end is found by halving."""
+        that begins where the longest's do, and its end is found by halving.  Only a ring that was extended and cut back holds pages of its
+        own in front as well, those that the tokens would have overwritten: there the beginning is looked for page by page."""
         lengths = self.lengths_host[list(slots)].tolist()
+        cut = (self.longest_host[list(slots)] > self.lengths_host[list(slots)]).tolist()
         out = []
         for g in self.groups:
             n, found = g.pages_per_seq, []
@@ -413,8 +415,11 @@ class KVCache:
                 start = max(0, (max(mine) - 1) // PAGE - n + 1) if g.ring else 0
                 end = (min(mine) - 1) // PAGE + 1
                 lead = g.held[slots[first]]
+                front = g.ring and any(cut[first:first + rows])
                 for r in range(first + 1, first + rows):
                     held = g.held[slots[r]]
+                    while front and start < end and held[start % n] != lead[start % n]:
+                        start += 1
                     if end <= start or held[(end - 1) % n] == lead[(end - 1) % n]:
                         continue
                     lo, hi = start, end - 1                     # page hi is not common; pages below lo are

@@ -276,3 +276,52 @@ def test_tables_of_rows_that_just_forked():
     b, = c.fork([a])
     assert c.shared_positions([a, b], [(0, 2)]) == [[(0, 192)]] * len(c.groups)      # the partly filled page too, as yet
     assert np.array_equal(c.groups[0].table_host[a], c.groups[0].table_host[b])
+
+
+@pytest.mark.parametrize("order", [0, 1])
+def test_a_ring_that_was_extended_and_cut_back_shares_only_what_it_still_holds_in_the_same_pages(order):
+    """What undoes a step that could not be launched: the cells that its tokens would have gone into are copies of one sequence's own, at
+    the end and, where they have wrapped, in front of what is still common."""
+    t = Tape(make(window=192))
+    a = t.new()
+    t.say((a, 500))                                      # pages 5, 6 and 7 of a ring of three
+    b, = t.fork([a])
+    t.c.extend([(a, 520)])                               # a place in page 7, and page 8 in that of page 5
+    t.c.truncate([(a, 500)])
+    rows = [a, b][::1 - 2 * order]
+    for g, found in zip(t.c.groups, t.c.shared_positions(rows, [(0, 2)])):
+        assert found == ([(6 * PAGE, 7 * PAGE)] if g.ring else [(0, 7 * PAGE)])
+        assert rows_hold(t.c, rows, (0, 2), g, *found[0])
+    t.say((b, 13))
+    t.c.audit()
+    for g, found in zip(t.c.groups, t.c.shared_positions(rows, [(0, 2)])):
+        assert rows_hold(t.c, rows, (0, 2), g, *found[0])
+
+
+@pytest.mark.parametrize("window", [70, 192])
+@pytest.mark.parametrize("seed", range(4))
+def test_random_walk_with_steps_that_are_undone(window, seed):
+    rnd = random.Random(1000 + seed)
+    c = make(max_tokens=4096, max_slots=7, window=window)
+    live = []
+    for _ in range(200):
+        r = rnd.random()
+        try:
+            if r < 0.1 or not live:
+                live.append(c.allocate())
+            elif r < 0.3:
+                live += c.fork([rnd.choice(live) for _ in range(rnd.choice([1, 1, 2]))])
+            elif r < 0.4:
+                c.free(live.pop(rnd.randrange(len(live))))
+            else:
+                some = [(s, c.length(s)) for s in rnd.sample(live, rnd.randint(1, len(live))) if c.length(s) < 800]
+                c.extend([(s, n + rnd.choice([1, 1, 17, 64, 90, 200])) for s, n in some])
+                if r > 0.8:
+                    c.truncate(some)
+        except CacheFull:
+            pass
+        c.audit()
+        rows = sorted((s for s in live if c.length(s)), key=lambda s: (c._family[s], rnd.random()))
+        runs = c.families(rows)
+        for g, found in zip(c.groups, c.shared_positions(rows, runs)):
+            assert all(rows_hold(c, rows, run, g, *f) for run, f in zip(runs, found))
