@@ -2423,7 +2423,7 @@ def shared_attention_pays(dtype: torch.dtype, n_heads: int, n_kv: int, head_dim:
     """Whether a decode step should read common keys once (``attn_decode_shared``) rather than once per row (``attn_decode``).  ``shared``: bounds as
     in ``SharedKeys``, beside which ``spared`` may say how many positions of keys the rows need not read again (else what the bounds allow).
 
-    Measured with the plans that a step's bounds lead to, us, once / per row, in 45 head shapes, 2 to 128 rows, 64 to 8192 common keys, up to 100 or
+    Measured with the plans that a step's bounds lead to, us, once / per row, 7050 steps in 45 head shapes, 2 to 128 rows, 64 to 8192 common keys, up to 100 or
     up to 1000 of a row's own.  Where the rule says once, that took 0.05 to 1.07 times as long (1.07: 16 rows, 4 kv heads of 128 with eight query heads
     each, 1024 keys 12.6 / 11.8).  Of 1200 steps drawn beside these 580 were chosen, of which 15 took longer, 1.5 times at most (6 rows of 2 heads of 64
     on one kv head in float32; of the bfloat16 ones 1.25).
